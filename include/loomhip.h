@@ -49,6 +49,7 @@ extern "C" {
 #define LOOMHIP_Q8_0 8
 #define LOOMHIP_Q4_K 12
 #define LOOMHIP_Q6_K 14
+#define LOOMHIP_BF16 30 /* adapters (loomhip_lora) only */
 
 /* gating (src/gguf/moe.zig:36-44) */
 #define LOOMHIP_GATING_SOFTMAX 1
@@ -772,6 +773,102 @@ int loomhip_mla_layer_cached_dev(const loomhip_mla_attn *a, const float *const *
                                  const void *attn_out, const float *ffn_norm, float eps,
                                  const loomhip_moe_layer_ec *moe, loomhip_ec *ec, float *x, uint32_t *ids_out,
                                  void *stream);
+
+/* ---- batched serving on the device ------------------------------------------
+ * No counterpart in the reference (its server decodes greedily, one sequence
+ * or a few lanes over caches of their own): what a server with many requests
+ * of one model runs between the projections and the next token.  Tensors are
+ * device pointers on the library's device, which has to be the current one;
+ * work is ordered on `stream`.  The calls allocate nothing, keep nothing and
+ * copy nothing to the host, so they can be captured in a HIP graph and run at
+ * the same time on several streams or from several threads, each with a
+ * workspace of its own: `ws` (device, at a multiple of 16 bytes, contents
+ * undefined before and after) of at least the bytes the call's _ws function
+ * gives for the same sizes.  Calls that can run at the same time, captured
+ * graphs among them, must not share it.  Outputs must not overlap inputs
+ * except where said.  n == 0 is OK and does nothing. */
+
+/* Rows of an fp16 key or value cache: element (lane, row, head, i) of k and v
+ * at lane * lane_stride + row * row_stride + head * head_stride + i
+ * (elements).  The frame's [n][n_layers][ctx_len][kvd] cache at a layer:
+ * lane_stride n_layers * ctx_len * kvd, row_stride kvd, head_stride head_dim. */
+typedef struct {
+    const uint16_t *k, *v;
+    size_t rows;
+    size_t lane_stride, row_stride, head_stride;
+} loomhip_kv_rows;
+/* Attention of n lanes that share a prefix, the prefix read once for all of
+ * them: lane i's query token j of q_len[i] (NULL: n_q each) attends every row
+ * of `prefix` (one lane; lane_stride unused) and the first
+ * own_len[i] - q_len[i] + 1 + j rows of its own (its last q_len[i] rows are
+ * its query tokens', already appended: each sees itself and what came
+ * before).  q, out f32 [n][n_q][n_heads][head_dim] (rope applied; head h
+ * reads key head h / (n_heads / n_kv_heads)):
+ *   out = sum_t p_t v_t,  p = softmax over the row's t of scale * (q . k_t),
+ * zero where a row sees nothing.  out rows j >= q_len[i] are left as they
+ * were.  own_len and q_len are clamped into [0, own->rows] and [0, n_q]; rows
+ * of the cache past a query's own are not part of its result, whatever they
+ * hold (a cached NaN or infinity makes the rows that see it NaN).
+ * prefix->rows or own->rows may be 0 (no rows; pointers unused).
+ * head_dim a multiple of 8 up to 256, strides multiples of 8, pointers at a
+ * multiple of 16 bytes; DECLINED otherwise. */
+int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
+                            const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,
+                            size_t n_kv_heads, size_t head_dim, float scale, float *out, void *ws, size_t ws_bytes,
+                            void *stream);
+size_t loomhip_prefix_attn_ws(size_t prefix_rows, size_t own_rows, size_t n, size_t n_q, size_t n_heads,
+                              size_t n_kv_heads, size_t head_dim);
+
+/* Low-rank adapters of many requests beside one [rows][cols] projection
+ * (loomhip_matvec_dev's output, or any other): for every vector t of n
+ *   out_t = base_t + scale[e] * B_e (A_e x_t),  e = ids[t],
+ * base_t alone where ids[t] is not in [0, n_adapters).  a [n_adapters][rank]
+ * [cols], b [n_adapters][rows][rank] of `type` (F32, F16, BF16; adapters of
+ * lower rank zero-padded), scale f32, ids int32; x, base, out f32 rows at the
+ * given strides.  base may be out itself (in place) or NULL (zeros).  f32
+ * products and sums.  rank up to 256; DECLINED otherwise. */
+typedef struct {
+    int type;
+    size_t n_adapters, rank, rows, cols;
+    const void *a, *b;
+    const float *scale;
+} loomhip_lora;
+int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, const int32_t *ids, const float *base,
+                     size_t base_stride, size_t n, float *out, size_t out_stride, void *ws, size_t ws_bytes,
+                     void *stream);
+size_t loomhip_lora_ws(const loomhip_lora *l, size_t n);
+
+/* Token probabilities: probs[r] = softmax(logits[r] / temperature[r]) over
+ * `vocab` values (temperature f32 [n] or NULL: 1), rows at the given strides;
+ * probs may be logits itself with the same stride.  A temperature that is
+ * not positive (or so small that 1/T passes f32) gives 1 at the first maximum
+ * and 0 elsewhere, the frame's greedy pick.  A row of -inf alone gives zeros.
+ * n up to 65535 rows; DECLINED otherwise. */
+int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const float *temperature,
+                            float *probs, size_t out_stride, void *ws, size_t ws_bytes, void *stream);
+size_t loomhip_token_probs_ws(size_t n, size_t vocab);
+
+/* Verification of drafted tokens: lane i's n_draft[i] (NULL: k each; clamped
+ * into [0, k]) drafted tokens against the target's probabilities.  Token j,
+ * x = draft_tokens[i][j], is accepted while u_accept[i][j] * q_j(x) < p_j(x)
+ * (q = draft_probs[i][j], or 1 where draft_probs is NULL: a drafter that
+ * names one token).  After the first refusal, at row r, the lane's next token
+ * is drawn from max(p_r - q_r, 0) (without draft_probs: p_r without x; from
+ * p_r where that has nothing left), after none from p at row n_draft[i]: the
+ * lowest v whose running sum passes u_sample[i] times the row's sum (a number
+ * outside [0, 1) or NaN acts as the nearer end, NaN as 0).  Products,
+ * differences and sums in 64 bits.  target_probs [n][k + 1][vocab],
+ * draft_probs [n][k][vocab], draft_tokens int32 [n][k], u_accept [n][k],
+ * u_sample [n]; rows need not sum to 1; what is not positive and finite
+ * counts as 0, a token outside the vocabulary is refused.  tokens_out
+ * [n][k + 1]: the accepted tokens, the drawn one (-1: the row holds nothing
+ * to draw), then -1; n_accepted [n].  n up to 65535, k up to 4096; DECLINED
+ * otherwise. */
+int loomhip_verify_drafts_dev(const float *target_probs, const float *draft_probs, const int32_t *draft_tokens,
+                              const int32_t *n_draft, const float *u_accept, const float *u_sample, size_t n, size_t k,
+                              size_t vocab, int32_t *tokens_out, int32_t *n_accepted, void *ws, size_t ws_bytes,
+                              void *stream);
+size_t loomhip_verify_drafts_ws(size_t n, size_t vocab);
 
 #ifdef __cplusplus
 }

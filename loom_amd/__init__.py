@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(HERE, "libloomhip.so")
 HEADER = os.path.join(ROOT, "include", "loomhip.h")
 
 OK, DECLINED, ERR_ARG, ERR_HIP, ERR_INIT = 0, 1, -1, -2, -3
-F32, F16, Q4_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 8, 12, 14
+F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 2, 8, 12, 14, 30
 GATING_SOFTMAX, GATING_SIGMOID, GATING_SOFTMAX_TOPK = 1, 2, 3
 COMBINE_SELECTION, COMBINE_EXPERT_ASC, COMBINE_SELECTION_ADD = 0, 1, 2
 KT_GATE_UP, KT_DOWN, KT_DENSE, KT_ATTN, KT_HEAD, KT_QKV = 0, 1, 2, 3, 4, 5
@@ -243,6 +243,20 @@ class ExpertRefDesc(C.Structure):
     ]
 
 
+class KvRowsDesc(C.Structure):
+    """Mirror of ``loomhip_kv_rows`` in include/loomhip.h."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("rows", C.c_size_t), ("lane_stride", C.c_size_t),
+                ("row_stride", C.c_size_t), ("head_stride", C.c_size_t)]
+
+
+class LoraDesc(C.Structure):
+    """Mirror of ``loomhip_lora`` in include/loomhip.h."""
+
+    _fields_ = [("type", C.c_int), ("n_adapters", C.c_size_t), ("rank", C.c_size_t), ("rows", C.c_size_t),
+                ("cols", C.c_size_t), ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
+
+
 def header_symbols() -> list[str]:
     """Every function name declared in include/loomhip.h."""
     text = open(HEADER).read()
@@ -363,6 +377,15 @@ def lib() -> C.CDLL:
                                         WeightRefDesc, vp, sz]),
         "loomhip_mla_layer_cached_dev": (i, [C.POINTER(MlaAttnDesc), C.POINTER(vp), C.POINTER(vp), sz, sz, vp, vp, i,
                                              vp, vp, f, C.POINTER(MoeLayerEcDesc), vp, vp, vp, vp]),
+        "loomhip_prefix_attn_dev": (i, [C.POINTER(KvRowsDesc), C.POINTER(KvRowsDesc), vp, vp, vp, sz, sz, sz, sz, sz,
+                                        f, vp, vp, sz, vp]),
+        "loomhip_prefix_attn_ws": (sz, [sz, sz, sz, sz, sz, sz, sz]),
+        "loomhip_lora_dev": (i, [C.POINTER(LoraDesc), vp, sz, vp, vp, sz, sz, vp, sz, vp, sz, vp]),
+        "loomhip_lora_ws": (sz, [C.POINTER(LoraDesc), sz]),
+        "loomhip_token_probs_dev": (i, [vp, sz, sz, sz, vp, vp, sz, vp, sz, vp]),
+        "loomhip_token_probs_ws": (sz, [sz, sz]),
+        "loomhip_verify_drafts_dev": (i, [vp, vp, vp, vp, vp, vp, sz, sz, sz, vp, vp, vp, sz, vp]),
+        "loomhip_verify_drafts_ws": (sz, [sz, sz]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

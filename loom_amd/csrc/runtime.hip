@@ -296,6 +296,18 @@ int require_ready() {
     return LOOMHIP_OK;
 }
 
+int require_device() {
+    if (int rc = require_ready())
+        return rc;
+    int dev = -1;
+    const hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess)
+        return hip_fail(e, "hipGetDevice");
+    if (dev != g_ctx.device)
+        return fail(LOOMHIP_ERR_ARG, "the current device is %d, the library is initialised on %d", dev, g_ctx.device);
+    return LOOMHIP_OK;
+}
+
 } // namespace lh
 
 using namespace lh;

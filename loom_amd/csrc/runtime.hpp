@@ -41,6 +41,7 @@ extern Ctx g_ctx;
 int fail(int code, const char *fmt, ...);
 int hip_fail(hipError_t e, const char *what);
 int require_ready();
+int require_device(); // require_ready, and the library's device is the current one
 hipStream_t stream_of(void *s);
 int upload_weights(int t, const void *host, size_t rows, size_t cols, size_t planes, void **dev);
 void clear_weight_cache();
