@@ -24,6 +24,9 @@
 // the LDS transpose read (ds_read_b64_tr_b16) gives from row-major values.
 // The softmax of a query needs one exchange between the two half waves.
 #include "runtime.hpp"
+#include <cmath>
+#include <type_traits>
+#include <utility>
 
 namespace lh {
 
@@ -36,11 +39,11 @@ typedef float pa_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int PA_THREADS = 256;
 constexpr int PA_MAX_HD = 256;
-// p = 2^(s - m + PA_SHIFT): the running maximum m moves only where a score
-// passes it by more than PA_SLACK (in log2), so most tiles rescale nothing; p
-// stays below 2^14 (f16 ends at 2^16) and its low part stays normal down to
-// 2^-9 of the maximum, below that off by at most 2^-31 of it.
-constexpr float PA_SHIFT = 6.0f, PA_SLACK = 8.0f;
+// p = 2^(s - m + PA_SHIFT): the running maximum m moves only where eight
+// weights sum to more than PA_MOST, so most tiles rescale nothing; p stays
+// below 2^14 (f16 ends at 2^16) and its low part stays normal down to 2^-9 of
+// the maximum, below that off by at most 2^-31 of it.
+constexpr float PA_SHIFT = 6.0f, PA_MOST = 16384.0f;
 
 struct PrefixAttnParams {
     loomhip_kv_rows pre, own;
@@ -49,11 +52,12 @@ struct PrefixAttnParams {
     int n, n_q, n_heads, n_kv, hd;
     float scale;
     float *out;
-    // items: prefix [kv][split][row block], then own [lane][kv][split][row block]
-    int pre_blocks, pre_splits, pre_len; // row blocks of all lanes, splits, rows per split
+    // Items: prefix [kv][split][row block], then own [lane][kv][split][row block].  The prefix's split count depends on
+    // how many rows the lanes have (q_len is on the device): pa_pre_cut's, at most pre_splits, left in *cut.
+    int pre_splits, pre_items, xcd_slots;
     int own_blocks, own_splits, own_len_split;
-    int pre_items;
-    int slots;   // pre_splits + own_splits
+    int slots;   // own_splits + pre_splits, in that order
+    int *cut;
     float *part; // [row][slot][hd], row = (lane * n_q + token) * n_heads + head
     float2 *ml;  // [row][slot]
 };
@@ -78,36 +82,40 @@ __device__ __forceinline__ float pa_half_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// f(0), f(1), .. f(N - 1) with the number a constant.
+template <class F, int... I>
+__device__ __forceinline__ void pa_for(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void pa_for(F f) {
+    pa_for(f, std::make_integer_sequence<int, N>{});
+}
+
 // A work group's four waves as RW row groups of 32 queries by 4 / RW key
-// groups: a tile of TK cache rows, KPW of them for each wave.  RW = 4 shares a
-// tile among 128 queries; RW = 1 takes up to 32 queries (a lane's own rows, a
-// small batch) with its waves side by side along the keys.  AHEAD: the next
-// tile's loads are in registers while a tile is multiplied; where the tile's
-// 64 registers a thread would not fit beside the query and the sums, its work
-// groups' short ranges are loaded as they come.
+// groups: a tile of TK cache rows, KPW of them for each wave, in blocks of 32.
+// RW = 4 shares a tile among 128 queries; RW = 1 takes up to 32 queries (a
+// lane's own rows, a small batch) with its waves side by side along the keys.
+// PIPE: the tiles alternate between two LDS buffers, the loads of the one after
+// next in registers, and the next block's scores are multiplied while this
+// block's weights are formed; without it (short ranges, or a head whose query
+// and sums leave no registers) a tile is loaded as it comes.
+// LDS rows are padded so that fragment reads spread over the banks with every
+// address a constant from one register: keys are read as 16 bytes of eight
+// rows at a time, which 16 bytes more a row put 4 banks apart; values by 16
+// lanes as 32 bytes of four rows, which 32 bytes more put 8 banks apart.
 template <int HDP, int RW>
 struct PaCfg {
-    static constexpr int KW = 4 / RW, KPW = RW == 4 && HDP < 256 ? 64 : 32, TK = KW * KPW;
-    static constexpr bool AHEAD = RW > 1 && HDP < 256;
-    static constexpr int CH = HDP / 8;                    // 16-byte chunks of a row
-    static constexpr int NCH = TK * CH / PA_THREADS;      // chunks a thread stages, of keys and of values each
-    static constexpr int TILE_BYTES = TK * HDP * 2;       // keys, or values
-    static constexpr int MERGE_BYTES = KW > 1 ? 4 * 32 * HDP * 4 : 0;
-    static constexpr int BYTES = 2 * TILE_BYTES > MERGE_BYTES ? 2 * TILE_BYTES : MERGE_BYTES;
+    static constexpr int KW = 4 / RW, KPW = RW == 4 && HDP < 256 ? 64 : 32, TK = KW * KPW, NB = KPW / 32;
+    static constexpr bool PIPE = RW > 1 && HDP < 256;
+    static constexpr int CH = HDP / 8;               // 16-byte chunks of a row
+    static constexpr int NCH = TK * CH / PA_THREADS; // chunks a thread stages, of keys and of values each
+    static constexpr int KS = HDP * 2 + 16, VS = HDP * 2 + 32; // bytes from an LDS row to the next
+    static constexpr int VO = TK * KS, TILE = VO + TK * VS;    // where a tile's values start, its bytes
+    static constexpr int TILES = (PIPE ? 2 : 1) * TILE;
+    static constexpr int ROWS = 4 * 32 * HDP * 4; // queries on their way in (RW * 32 rows), records on their way out
+    static constexpr int BYTES = TILES > ROWS ? TILES : ROWS;
 };
-
-// Chunk positions inside an LDS row.  Keys are read as 16 bytes of 32 rows: a
-// lane's eight neighbours (eight rows) must fall on different 16-byte columns
-// of the 256 bytes of banks.  Values are read by 16 lanes as 32 bytes of four
-// rows: the four must fall on different 32-byte columns.
-template <int HDP>
-__device__ __forceinline__ int pa_k_pos(int row, int ch) {
-    return ch ^ (HDP == 64 ? (row >> 1) & 7 : row & 15);
-}
-template <int HDP>
-__device__ __forceinline__ int pa_v_pos(int row, int ch) {
-    return ch ^ (HDP == 64 ? ((row >> 1) & 3) << 1 : (row & 7) << 1);
-}
 
 // Query rows [row0, row0 + RW * 32) of the item (map: their global row, -1 past the end; lim: the first key each
 // does not see) against cache rows [k0, k1) at k / v (one head's rows, `stride` elements apart): records into slot
@@ -123,76 +131,112 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
     const int rw = wave % RW, kw = wave / RW;
     const int row = map[rw * 32 + col], limit = lim[rw * 32 + col] < k1 ? lim[rw * 32 + col] : k1;
     const int hd = P.hd;
-    char *const sk = smem, *const sv = smem + C::TILE_BYTES;
 
     // staging: thread t's chunks are t, t + 256, ..
     uint4 rk[C::NCH], rv[C::NCH];
+    constexpr int RSTEP = PA_THREADS / C::CH;        // rows from a thread's chunk to its next
     const int sch = tid % C::CH, srow = tid / C::CH; // its column of chunks, its first row
-    const auto stage_load = [&](const uint16_t *__restrict__ p, uint4 *to, int kt) {
-        const int left = sch * 8 < hd ? k1 - kt - srow : 0; // rows from its first on
-        const size_t off = (size_t)(kt + srow) * stride + sch * 8;
+    // Rows past the last and chunks past the head's end are the last one again: their scores are masked, their weights
+    // zero, their columns not written.
+    const int ssrc = (sch * 8 < hd ? sch : hd / 8 - 1) * 16;
+    uint32_t soff[C::NCH]; // byte offsets from the tile's first row
+    const auto place = [&](int last) { // rows up to `last` of the tile
 #pragma unroll
         for (int c = 0; c < C::NCH; c++) {
-            constexpr int STEP = PA_THREADS / C::CH;
-            to[c] = c * STEP < left ? *(const uint4 *)(p + off + (size_t)(c * STEP) * stride) : uint4{0, 0, 0, 0};
+            const int r = srow + c * RSTEP;
+            soff[c] = (uint32_t)(r < last ? r : last) * ((uint32_t)stride * 2) + ssrc;
         }
     };
-    const auto stage_keys = [&] {
+    const auto load = [&](const uint16_t *__restrict__ p, int kt, int c) {
+        return *(const uint4 *)((const char *)(p + (size_t)kt * stride) + soff[c]);
+    };
+    const auto load_tile = [&](const uint16_t *__restrict__ p, uint4 *to, int kt) {
+#pragma unroll
+        for (int c = 0; c < C::NCH; c++)
+            to[c] = load(p, kt, c);
+    };
+    const int k_st = srow * C::KS + sch * 16, v_st = C::VO + srow * C::VS + sch * 16;
+    const auto store_keys = [&](char *to, int c) { *(uint4 *)(to + k_st + c * RSTEP * C::KS) = rk[c]; };
+    const auto store_values = [&](char *to, int c) { *(uint4 *)(to + v_st + c * RSTEP * C::VS) = rv[c]; };
+    const auto store_tile = [&](char *to) {
 #pragma unroll
         for (int c = 0; c < C::NCH; c++) {
-            const int r = srow + c * (PA_THREADS / C::CH);
-            *(uint4 *)(sk + (r * C::CH + pa_k_pos<HDP>(r, sch)) * 16) = rk[c];
+            store_keys(to, c);
+            store_values(to, c);
         }
     };
-    // Values that some query does not see are left out of the product where they are not finite: they would reach
-    // it as 0 * v.  Returns whether there was one.
-    const auto stage_values = [&](int kt, bool edge) {
-        bool strange = false;
+    // Values that some query does not see are left out of the product where they are not finite: they would reach it
+    // as 0 * v.  strange: there was one.
+    bool strange = false;
+    const auto clean = [&](int kt) {
+        if (kt + C::TK > border) {
 #pragma unroll
-        for (int c = 0; c < C::NCH; c++) {
-            const int r = srow + c * (PA_THREADS / C::CH);
-            if (edge && kt + r >= border) {
-                uint32_t *w = (uint32_t *)&rv[c];
+            for (int c = 0; c < C::NCH; c++)
+                if (kt + srow + c * RSTEP >= border) {
+                    uint32_t *w = (uint32_t *)&rv[c];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool lo = (w[e] & 0x7c00u) == 0x7c00u, hi = (w[e] & 0x7c000000u) == 0x7c000000u;
-                    strange |= lo | hi;
-                    w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+                    for (int e = 0; e < 4; e++) {
+                        const bool lo = (w[e] & 0x7c00u) == 0x7c00u, hi = (w[e] & 0x7c000000u) == 0x7c000000u;
+                        strange |= lo | hi;
+                        w[e] &= (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu);
+                    }
                 }
-            }
-            *(uint4 *)(sv + (r * C::CH + pa_v_pos<HDP>(r, sch)) * 16) = rv[c];
         }
-        return strange;
     };
     if (tid == 0)
         *flag = 0;
-    if (C::AHEAD) {
-        stage_load(kp, rk, k0);
-        stage_load(vp, rv, k0);
+    place(k1 - 1 - k0);
+    if (HDP < 256) { // the first tile, in flight while the queries are split
+        load_tile(kp, rk, k0);
+        load_tile(vp, rv, k0);
     }
 
-    // the query: its largest element brought to 2^13 .. 2^14 by a power of two, split into two f16 parts
+    // The queries through LDS (a lane's loads of its own row would touch 32 rows each), then each its largest element
+    // brought to 2^13 .. 2^14 by a power of two and split into two f16 parts.
+    constexpr int QC = HDP / 4, QN = RW * 32 * QC / PA_THREADS; // 16-byte columns of a row, shifted by the row against
+                                                                // bank conflicts; columns a thread takes
+    constexpr int QB = QN < 8 ? QN : 8;                         // loads in flight
+    const int qc = tid % QC, qr = tid / QC;
+    const size_t qat = qc * 4 < hd ? qc * 4 : 0;
+#pragma unroll
+    for (int n0 = 0; n0 < QN; n0 += QB) {
+        pa_f4 v[QB];
+        int R[QB];
+#pragma unroll
+        for (int x = 0; x < QB; x++) {
+            R[x] = map[qr + (n0 + x) * (PA_THREADS / QC)];
+            v[x] = *(const pa_f4 *)(P.q + (size_t)(R[x] < 0 ? 0 : R[x]) * hd + qat);
+        }
+#pragma unroll
+        for (int x = 0; x < QB; x++) {
+            const int r = qr + (n0 + x) * (PA_THREADS / QC);
+            *(pa_f4 *)(smem + (r * QC + (qc + r) % QC) * 16) =
+                R[x] >= 0 && qc * 4 < hd ? v[x] : pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    __syncthreads();
     pa_h8 qh[STEPS], ql[STEPS];
     float cs; // scores in log2 units per unit of the split query's
     {
+        const int r = rw * 32 + col;
         float v[STEPS][8], amax = 0.0f;
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            const int d = s * 16 + half * 8;
-            const bool in = row >= 0 && d < hd;
-            const pa_f4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-            const pa_f4 a = in ? *(const pa_f4 *)(P.q + (size_t)row * hd + d) : z;
-            const pa_f4 b = in ? *(const pa_f4 *)(P.q + (size_t)row * hd + d + 4) : z;
+        for (int s = 0; s < STEPS; s++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[s][e] = a[e], v[s][4 + e] = b[e];
-                amax = fmaxf(amax, fmaxf(fabsf(a[e]), fabsf(b[e])));
+            for (int x = 0; x < 2; x++) {
+                const pa_f4 a = *(const pa_f4 *)(smem + (r * QC + (s * 4 + half * 2 + x + r) % QC) * 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[s][x * 4 + e] = a[e];
+                    amax = fmaxf(amax, fabsf(a[e]));
+                }
             }
-        }
         amax = pa_half_max(amax);
-        const int k = amax > 0.0f && amax < __builtin_inff() ? pa_clamp(13 - ilogbf(amax), -120, 120) : 0;
-        const float f = ldexpf(P.scale < 0.0f ? -1.0f : 1.0f, k);
-        cs = ldexpf(fabsf(P.scale) * 0x1.715476p+0f, -k);
+        // the power of two from amax's exponent (126 for the smallest: the query stays as small as it is)
+        const int e = (int)(__float_as_uint(amax) >> 23);
+        const int k = e > 0 && e < 255 ? pa_clamp(13 + 127 - e, -120, 120) : 0;
+        const float f = __uint_as_float((uint32_t)(127 + k) << 23) * (P.scale < 0.0f ? -1.0f : 1.0f);
+        cs = fabsf(P.scale) * 0x1.715476p+0f * __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
@@ -205,9 +249,8 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
     }
 
     const int kb = kw * C::KPW; // the wave's keys of a tile
-    const int k_at = ((kb + col) * C::CH + pa_k_pos<HDP>(kb + col, half)) * 16;
-    const int v_row = kb + 4 * half + ((lane & 15) >> 2), v_col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const int v_at = (v_row * C::CH + pa_v_pos<HDP>(v_row, v_col / 8)) * 16 + v_col % 8 * 2;
+    const int k_at = (kb + col) * C::KS + half * 16;
+    const int v_at = C::VO + (kb + 4 * half + ((lane & 15) >> 2)) * C::VS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     pa_f16 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; b++)
@@ -216,125 +259,286 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
             o[b][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
 
-    for (int kt = k0; kt < k1; kt += C::TK) {
-        const bool edge = kt + C::TK > border; // some row of the tile is not seen by every query
-        __syncthreads();
-        bool strange;
-        if constexpr (C::AHEAD) {
-            stage_keys();
-            strange = stage_values(kt, edge);
+    // Fragments: keys of block b and 16 columns of the head, values of 16 keys and 32 columns.
+    const auto key_frag = [&](const char *tile, int b, int st) {
+        return *(const pa_h8 *)(tile + k_at + b * 32 * C::KS + st * 32);
+    };
+    const auto value_frag = [&](char *tile, int b, int st, int db) {
+        const auto at = (__attribute__((address_space(3))) char *)(tile + v_at) + (b * 32 + st * 16) * C::VS + db * 64;
+        const pa_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4 *)at);
+        const pa_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4 *)(at + 8 * C::VS));
+        return __builtin_bit_cast(pa_h8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    // -inf for the keys of block b of the tile at kt that the lane's query does not see
+    const auto mask = [&](pa_f16 &s, int kt, int b) {
+        if (kt + C::TK > border || kt + C::TK > k1) {
+            const int seen = limit - kt - kb - b * 32 - 4 * half; // of the lane's keys, counted from its first
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float v = 8 * (i / 4) + i % 4 < seen ? s[i] : -__builtin_inff();
+                asm volatile("" : "+v"(v)); // kept inside the branch: the selects would run in every block
+                s[i] = v;
+            }
+        }
+    };
+    // Weights are taken against m, the running maximum of the scores of some block before: p = 2^(s - m + PA_SHIFT).
+    // No block's own maximum is formed: the sum of eight weights, which is wanted anyway, tells whether one of them is
+    // past what m allows (or no number); then m moves to this block's and the eight are formed again.
+    float sub = 0.0f; // PA_SHIFT - m
+    const auto grow = [&](const pa_f16 &s) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++)
+            mx = fmaxf(mx, s[i]);
+        const float m2 = fmaxf(m, pa_half_max(mx) * cs);
+        const float f = m == m2 ? 1.0f : __builtin_amdgcn_exp2f(m - m2); // -inf before the first seen key: 0
+        m = m2;
+        sub = PA_SHIFT - (m == -__builtin_inff() ? 0.0f : m);
+        l *= f;
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                o[b][i] *= f;
+        // a query that has seen nothing yet has no m: its first finite score has to come back here
+        if (m == -__builtin_inff())
+            sub = __builtin_inff();
+    };
+    // A block's weights, in two f16 parts: piece by piece, of each pair of values first the weights and their sum, then
+    // the parts.  Pieces 2 j and 2 j + 1 do the values 2 j; eight values make a half.
+    pa_h8 ph[2], pl[2];
+    float w0, w1, sum;
+    const auto piece = [&](const pa_f16 &s, int j) {
+        const int i = j & ~1;
+        if (j % 2 == 0) {
+            w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], cs, sub));
+            w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], cs, sub));
+            sum = i % 8 == 0 ? w0 + w1 : sum + (w0 + w1);
         } else {
-            stage_load(kp, rk, kt);
-            stage_keys();
-            stage_load(vp, rv, kt);
-            strange = stage_values(kt, edge);
+            const pa_h2 h = {(_Float16)w0, (_Float16)w1};
+            const float r0 = w0 - (float)h[0], r1 = w1 - (float)h[1];
+            const pa_h2 g = {(_Float16)r0, (_Float16)r1};
+            ph[i / 8][i % 8] = h[0], ph[i / 8][i % 8 + 1] = h[1];
+            pl[i / 8][i % 8] = g[0], pl[i / 8][i % 8 + 1] = g[1];
         }
-        if (edge && strange)
-            *flag = 1;
+    };
+    // After the eight of a half: taken again where m was too small for them.
+    const auto settle = [&](const pa_f16 &s, int x) {
+        if (__any(!(sum <= PA_MOST))) {
+            grow(s);
+            if (sub == __builtin_inff())
+                sub = 0.0f; // nothing seen: every weight is 2^-inf
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                piece(s, x * 8 + j);
+            if (m == -__builtin_inff())
+                sub = __builtin_inff();
+        }
+        l += sum;
+    };
+    // Scores of a block (S^T = K Q^T) and in their shadow the first half of the weights of the block before, and
+    // whatever `other` does at each step.  Products issue in order and each waits for the one before it, 32 cycles: the
+    // other work goes between them, about five vector instructions each (4.6 cycles).  Fragments are read AHEAD before
+    // their products: the first of them before the call, and here the first of the values of the products that follow.
+    constexpr int AHEAD = HDP == 128 ? 3 : 4, FRAGS = 2 * DB;
+    pa_h8 kf[STEPS], vf[FRAGS];
+    const auto keys_ahead = [&](const char *tile, int b) {
+#pragma unroll
+        for (int st = 0; st < AHEAD; st++)
+            kf[st] = key_frag(tile, b, st);
+    };
+    const auto values_ahead = [&](char *tile, int b) {
+#pragma unroll
+        for (int x = 0; x < AHEAD; x++)
+            vf[x] = value_frag(tile, b, x / DB, x % DB);
+    };
+    const auto scores = [&](const char *tile, int b, const pa_f16 &before, auto weigh, char *then_tile, int then_b,
+                            auto other) __attribute__((always_inline)) {
+        constexpr bool W = decltype(weigh)::value;
+        pa_f16 s;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            s[i] = 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
+        pa_for<STEPS>([&](auto step) {
+            constexpr int st = decltype(step)::value, PIECES = 8; // 8 of 16 values
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[st], qh[st], s, 0, 0, 0);
+            if constexpr (st + AHEAD < STEPS)
+                kf[st + AHEAD] = key_frag(tile, b, st + AHEAD);
+            else if constexpr (W) {
+                constexpr int x = st + AHEAD - STEPS;
+                vf[x] = value_frag(then_tile, then_b, x / DB, x % DB);
+            }
+            if constexpr (W)
+#pragma unroll
+                for (int j = st * PIECES / STEPS; j < (st + 1) * PIECES / STEPS; j++)
+                    piece(before, j);
+            __builtin_amdgcn_sched_barrier(0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[st], ql[st], s, 0, 0, 0);
+            other(step);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (W) {
+            asm volatile("" : "+v"(ph[0]), "+v"(pl[0])); // formed here, not past the next branch
+            settle(before, 0);
+        }
+        return s;
+    };
+    // O^T += V^T P^T of a block, in whose shadow the second half of its weights, `other`, and the first reads of the keys
+    // that come after.
+    const auto products = [&](char *tile, int b, const pa_f16 &now, const char *then_tile, int then_b, auto read_keys,
+                              auto other) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        pa_for<FRAGS>([&](auto frag) {
+            constexpr int x = decltype(frag)::value, st = x / DB, db = x % DB;
+            if constexpr (x == DB) {
+                asm volatile("" : "+v"(ph[1]), "+v"(pl[1]));
+                if constexpr (C::PIPE)
+                    settle(now, 1);
+                else
+                    l += sum;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const auto shadow = [&](int y) { // y of 0, 1
+                if (st == 0)
+#pragma unroll
+                    for (int j = 8 + (2 * db + y) * 4 / DB; j < 8 + (2 * db + y + 1) * 4 / DB; j++)
+                        piece(now, j);
+            };
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x], ph[st], o[db], 0, 0, 0);
+            if constexpr (x + AHEAD < FRAGS)
+                vf[x + AHEAD] = value_frag(tile, b, (x + AHEAD) / DB, (x + AHEAD) % DB);
+            else if constexpr (decltype(read_keys)::value)
+                kf[x + AHEAD - FRAGS] = key_frag(then_tile, then_b, x + AHEAD - FRAGS);
+            shadow(0);
+            __builtin_amdgcn_sched_barrier(0);
+            o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[x], pl[st], o[db], 0, 0, 0);
+            shadow(1);
+            other(frag);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    const auto nothing = [](auto) {};
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    const auto largest = [&](const pa_f16 &s) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++)
+            mx = fmaxf(mx, s[i]);
+        return mx;
+    };
+
+    __syncthreads(); // the queries are out of LDS
+    if constexpr (C::PIPE) {
+        char *cur = smem, *nxt = smem + C::TILE;
+        clean(k0);
+        store_tile(cur);
         __syncthreads();
-        if (C::AHEAD && kt + C::TK < k1) {
-            stage_load(kp, rk, kt + C::TK);
-            stage_load(vp, rv, kt + C::TK);
-        }
-
-        // scores of the wave's KPW keys
-        pa_f16 s[KB];
-#pragma unroll
-        for (int b = 0; b < KB; b++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                s[b][i] = 0.0f;
-#pragma unroll
-            for (int st = 0; st < STEPS; st++) {
-                // pa_k_pos of row kb + b * 32 + col, chunk 2 st + half: the row's part and st's by exclusive or
-                const pa_h8 a = *(const pa_h8 *)(sk + ((k_at ^ (st * 32)) + b * 32 * C::CH * 16));
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[st], s[b], 0, 0, 0);
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[st], s[b], 0, 0, 0);
+        const int kl = k0 + (k1 - k0 - 1) / C::TK * C::TK; // the last tile
+        int kn = k0 + C::TK < kl ? k0 + C::TK : kl;         // the next one
+        place(k1 - 1 - kn);
+        load_tile(kp, rk, kn);
+        load_tile(vp, rv, kn);
+        keys_ahead(cur, 0);
+        pa_f16 s = scores(cur, 0, pa_f16{}, no, nullptr, 0, nothing);
+        mask(s, k0, 0);
+        grow(s);
+        if (C::NB == 2)
+            keys_ahead(cur, 1);
+        // Past the last tile the next one's stores, loads and scores are the last one's again, used by nobody.
+        for (int kt = k0; kt < k1; kt += C::TK) {
+            clean(kn);
+            const int k2 = kn + C::TK < kl ? kn + C::TK : kl;
+            const auto store_next = [&](auto at) { // the next tile's buffer was last read before the barrier below
+                constexpr int i = decltype(at)::value;
+                if constexpr (i < C::NCH)
+                    store_keys(nxt, i);
+                else
+                    store_values(nxt, i - C::NCH);
+            };
+            const auto load_next = [&](auto at) {
+                constexpr int i = decltype(at)::value;
+                if constexpr (i < C::NCH)
+                    rk[i] = load(kp, k2, i);
+                else
+                    rv[i - C::NCH] = load(vp, k2, i - C::NCH);
+            };
+            static_assert(2 * C::NCH == STEPS && FRAGS == STEPS, "a store each step, a load each fragment");
+            const bool more = kt + C::TK < k1;
+            if (k2 + C::TK > k1)
+                place(k1 - 1 - k2);
+            if constexpr (C::NB == 2) {
+                pa_f16 s1 = scores(cur, 1, s, yes, cur, 0, store_next);
+                mask(s1, kt, 1);
+                __syncthreads(); // the next tile is there
+                products(cur, 0, s, nxt, 0, yes, load_next);
+                s = scores(nxt, 0, s1, yes, cur, 1, nothing);
+                if (more)
+                    mask(s, kn, 0);
+                products(cur, 1, s1, nxt, 1, yes, nothing);
+            } else {
+                store_tile(nxt);
+                __syncthreads();
+                keys_ahead(nxt, 0);
+                pa_f16 s1 = scores(nxt, 0, s, yes, cur, 0, nothing);
+                if (more)
+                    mask(s1, kn, 0);
+                products(cur, 0, s, nullptr, 0, no, load_next);
+                s = s1;
             }
-        }
-        if (edge || kt + C::TK > k1) {
-            const int seen = limit - kt - kb - 4 * half; // of the lane's keys, counted from its first
-#pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    s[b][i] = b * 32 + 8 * (i / 4) + i % 4 < seen ? s[b][i] : -__builtin_inff();
-        }
-        // the running maximum
-        float mx = s[0][0];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                mx = fmaxf(mx, s[b][i]);
-        mx = pa_half_max(mx) * cs;
-        if (__any(mx > m + PA_SLACK)) {
-            const float m2 = fmaxf(m, mx);
-            const float f = m == m2 ? 1.0f : __builtin_amdgcn_exp2f(m - m2); // -inf before the first seen key: 0
-            m = m2;
-            l *= f;
-#pragma unroll
-            for (int b = 0; b < DB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    o[b][i] *= f;
-        }
-        const float sub = PA_SHIFT - (m == -__builtin_inff() ? 0.0f : m);
-        // weights, in two f16 parts
-        pa_h8 ph[KB][2], pl[KB][2];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], cs, sub));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i + 1], cs, sub));
-                l += p0 + p1;
-                const pa_h2 h = __builtin_bit_cast(pa_h2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-                const float r0 = __builtin_fmaf((float)h[0], -1.0f, p0), r1 = __builtin_fmaf((float)h[1], -1.0f, p1);
-                const pa_h2 g = __builtin_bit_cast(pa_h2, __builtin_amdgcn_cvt_pkrtz(r0, r1));
-                ph[b][i / 8][i % 8] = h[0], ph[b][i / 8][i % 8 + 1] = h[1];
-                pl[b][i / 8][i % 8] = g[0], pl[b][i / 8][i % 8 + 1] = g[1];
-            }
-        // O^T += V^T P^T
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int st = 0; st < 2; st++)
-#pragma unroll
-                for (int db = 0; db < DB; db++) {
-                    // rows v_row + b * 32 + st * 16 (+ 8), column db * 32 + v_col: db's part by exclusive or
-                    const int at = (v_at ^ (db * 64)) + (b * 32 + st * 16) * C::CH * 16;
-                    pa_s4 a[2];
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-                        a[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) pa_s4 *)(sv + at + x * 8 * C::CH * 16));
-                    const pa_h8 va = __builtin_bit_cast(
-                        pa_h8, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[b][st], o[db], 0, 0, 0);
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[b][st], o[db], 0, 0, 0);
-                }
-    }
-    l = pa_half_sum(l);
-
-    // records: o as it stands relative to m (both carry PA_SHIFT)
-    if constexpr (C::KW == 1) {
-        if (row >= 0) {
-            const size_t rec = (size_t)row * P.slots + slot;
-            if (half == 0)
-                P.ml[rec] = make_float2(m, l);
-            float *dst = P.part + rec * hd;
-#pragma unroll
-            for (int db = 0; db < DB; db++)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int d = db * 32 + 2 * i + 4 * half;
-                    if (d < hd)
-                        *(pa_f4 *)(dst + d) = pa_f4{o[db][i], o[db][i + 1], o[db][i + 2], o[db][i + 3]};
-                }
+            __syncthreads(); // this tile is read
+            kn = k2;
+            char *const t = cur;
+            cur = nxt;
+            nxt = t;
         }
     } else {
-        // the key groups of a row group joined through LDS
+        for (int kt = k0; kt < k1; kt += C::TK) {
+            __syncthreads();
+            if (HDP == 256 || kt > k0) {
+                place(k1 - 1 - kt);
+                load_tile(kp, rk, kt);
+                if (HDP == 256)
+#pragma unroll
+                    for (int c = 0; c < C::NCH; c++)
+                        store_keys(smem, c);
+                load_tile(vp, rv, kt);
+            }
+            clean(kt);
+            if (HDP == 256)
+#pragma unroll
+                for (int c = 0; c < C::NCH; c++)
+                    store_values(smem, c);
+            else
+                store_tile(smem);
+            __syncthreads();
+            keys_ahead(smem, 0);
+            pa_f16 s = scores(smem, 0, pa_f16{}, no, nullptr, 0, nothing);
+            values_ahead(smem, 0);
+            mask(s, kt, 0);
+            float mx = s[0]; // a block a tile: its maximum is as cheap as the check
+#pragma unroll
+            for (int i = 1; i < 16; i++)
+                mx = fmaxf(mx, s[i]);
+            if (__any(mx * cs > m + (14.0f - PA_SHIFT)))
+                grow(s);
+            if (m == -__builtin_inff())
+                sub = 0.0f; // nothing seen: every weight is 2^-inf
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                piece(s, j);
+            l += sum;
+            products(smem, 0, s, nullptr, 0, no, nothing);
+        }
+    }
+    l = pa_half_sum(l);
+    if (strange)
+        *flag = 1;
+
+    // Records: o as it stands relative to m (both carry PA_SHIFT), through LDS, where the key groups of a row group are
+    // joined and from where whole rows are written (a lane holds 16 bytes here and there of its row).
+    {
         __shared__ float sm[4][32], sl[4][32];
         __syncthreads();
         if (half == 0)
@@ -356,29 +560,26 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
                     pa_f4{o[db][i] * f, o[db][i + 1] * f, o[db][i + 2] * f, o[db][i + 3] * f};
             }
         __syncthreads();
-        for (int at = tid; at < RW * 32 * (HDP / 4); at += PA_THREADS) {
-            const int rr = at / (HDP / 4), d = at % (HDP / 4) * 4; // row of the block, its column
-            const int R = map[rr];
-            if (R < 0 || d >= hd)
-                continue;
-            const int g = rr / 32, c = rr % 32;
+#pragma unroll
+        for (int n0 = 0; n0 < QN; n0++) {
+            const int rr = qr + n0 * (PA_THREADS / QC), R = map[rr], g = rr / 32, c = rr % 32;
             pa_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < C::KW; w++)
-                v += *(const pa_f4 *)((const float *)smem + (size_t)(g + w * RW) * 32 * HDP + c * HDP +
-                                      ((d / 4 + c) % (HDP / 4)) * 4);
-            const size_t rec = (size_t)R * P.slots + slot;
-            *(pa_f4 *)(P.part + rec * hd + d) = v;
-            if (d == 0) {
-                float mm = sm[g][c], ll = 0.0f;
+                v += *(const pa_f4 *)((const float *)smem + (size_t)(g + w * RW) * 32 * HDP + c * HDP + (qc + c) % QC * 4);
+            if (R >= 0 && qc * 4 < hd)
+                *(pa_f4 *)(P.part + ((size_t)R * P.slots + slot) * hd + qc * 4) = v;
+        }
+        if (tid < RW * 32 && map[tid] >= 0) {
+            const int g = tid / 32, c = tid % 32;
+            float mm = sm[g][c], ll = 0.0f;
 #pragma unroll
-                for (int w = 1; w < C::KW; w++)
-                    mm = fmaxf(mm, sm[g + w * RW][c]);
+            for (int w = 1; w < C::KW; w++)
+                mm = fmaxf(mm, sm[g + w * RW][c]);
 #pragma unroll
-                for (int w = 0; w < C::KW; w++)
-                    ll += sl[g + w * RW][c] * (sm[g + w * RW][c] == mm ? 1.0f : __builtin_amdgcn_exp2f(sm[g + w * RW][c] - mm));
-                P.ml[rec] = make_float2(mm, ll);
-            }
+            for (int w = 0; w < C::KW; w++)
+                ll += sl[g + w * RW][c] * (sm[g + w * RW][c] == mm ? 1.0f : __builtin_amdgcn_exp2f(sm[g + w * RW][c] - mm));
+            P.ml[(size_t)map[tid] * P.slots + slot] = make_float2(mm, ll);
         }
     }
     // The values taken out of the tiles, for the queries that see them: a weight of any size times them is no number.
@@ -395,49 +596,94 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
         }
 }
 
-// The block's rows of all lanes' live query rows (lane, token < q_len, head of the group), [r0, r0 + R): false if
-// the batch has no such rows.  Every thread takes lanes tid, tid + 256, ..; the running sum of their token counts
-// tells which of them fall into the block.
-template <int R>
-__device__ __forceinline__ bool pa_map_all(const PrefixAttnParams &P, int kvh, int r0, int *map, int *scan) {
-    const int G = P.n_heads / P.n_kv, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int r = tid; r < R; r += PA_THREADS)
-        map[r] = -1;
-    __syncthreads();
-    if (!P.q_len) {
-        const int rows = P.n * P.n_q * G;
-        for (int r = tid; r < R; r += PA_THREADS)
-            if (r0 + r < rows)
-                map[r] = (r0 + r) / G * P.n_heads + kvh * G + (r0 + r) % G;
-        __syncthreads();
-        return r0 < rows;
+// All lanes' live query rows in order: lane, token < q_len, head of the group.  Every thread takes lanes tid, tid + 256,
+// ..; the running sum of their token counts tells where a lane's rows are.
+struct PaTokens {
+    int L, end, all; // of the chunk of 256 lanes scanned last: the thread's lane's tokens, their end, all of them
+};
+__device__ __forceinline__ PaTokens pa_scan(const PrefixAttnParams &P, int i0, int *scan) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int i = i0 + tid, L = i < P.n ? pa_q_len(P, i) : 0;
+    int c = L;
+    for (int o = 1; o < 64; o *= 2) {
+        const int up = __shfl_up(c, o);
+        c += lane >= o ? up : 0;
     }
-    int before = 0; // tokens of the lanes already scanned
+    if (lane == 63)
+        scan[wave] = c;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < PA_THREADS / 64; w++) {
+        c += w < wave ? scan[w] : 0;
+        all += scan[w];
+    }
+    __syncthreads();
+    return {L, c, all};
+}
+__device__ __forceinline__ int pa_count(const PrefixAttnParams &P, int *scan, PaTokens &last) {
+    if (!P.q_len)
+        return P.n * P.n_q;
+    int all = 0;
     for (int i0 = 0; i0 < P.n; i0 += PA_THREADS) {
-        const int i = i0 + tid, L = i < P.n ? pa_q_len(P, i) : 0;
-        int c = L;
-        for (int o = 1; o < 64; o *= 2) {
-            const int up = __shfl_up(c, o);
-            c += lane >= o ? up : 0;
+        last = pa_scan(P, i0, scan);
+        all += last.all;
+    }
+    return all;
+}
+// The block's rows [r0, r0 + R), -1 past the last, by way of its tokens (tok: lane * n_q + token).
+template <int R>
+__device__ __forceinline__ void pa_map(const PrefixAttnParams &P, int kvh, int r0, int tokens, PaTokens t, int *map,
+                                       int *tok, int *scan) {
+    const int G = P.n_heads / P.n_kv, tid = threadIdx.x;
+    const int t0 = r0 / G, t1 = t0 + R < tokens ? t0 + R : tokens; // at least the block's tokens
+    if (P.q_len) {
+        int before = 0;
+        for (int i0 = 0; i0 < P.n && before < t1; i0 += PA_THREADS) {
+            if (P.n > PA_THREADS)
+                t = pa_scan(P, i0, scan);
+            const int first = before + t.end - t.L; // the lane's first token
+            for (int j = first < t0 ? t0 - first : 0; j < t.L && first + j < t1; j++)
+                tok[first + j - t0] = (i0 + tid) * P.n_q + j;
+            before += t.all;
         }
-        if (lane == 63)
-            scan[wave] = c;
         __syncthreads();
-        int all = 0;
-        for (int w = 0; w < PA_THREADS / 64; w++) {
-            c += w < wave ? scan[w] : 0;
-            all += scan[w];
-        }
-        __syncthreads();
-        const int first = (before + c - L) * G; // the lane's first row
-        for (int r = first < r0 ? r0 - first : 0; r < L * G && first + r < r0 + R; r++)
-            map[first + r - r0] = (i * P.n_q + r / G) * P.n_heads + kvh * G + r % G;
-        before += all;
-        if (before * G >= r0 + R)
-            break;
+    }
+    for (int r = tid; r < R; r += PA_THREADS) {
+        const int at = (r0 + r) / G, h = r0 + r - at * G;
+        map[r] = at < tokens ? (P.q_len ? tok[at - t0] : at) * P.n_heads + kvh * G + h : -1;
     }
     __syncthreads();
-    return r0 < before * G;
+}
+
+// The prefix's splits for `blocks` row blocks of every key head: a lane per candidate, the cheapest of
+//   rounds of the chip's work groups * (an item's start and end + its tiles) + records to be joined,
+// in the time of a 64-row tile, two work groups to a CU (3 us: measured start and end 8 us, 1024 records 0.3 us).
+constexpr float PA_ITEM = 3.0f, PA_RECORD = 0.09f / 1024.0f;
+__host__ __device__ inline int pa_split_len(int rows, int splits) {
+    return ((rows + splits - 1) / splits + 127) / 128 * 128;
+}
+// rows of the cache, splits s, items a split (x), work groups at a time, query rows of a split's records; infinite for a
+// count that leaves a split empty
+__host__ __device__ inline float pa_cost(int rows, int s, int x, int room, float records) {
+    const int len = pa_split_len(rows, s);
+    if ((int64_t)(s - 1) * len >= rows)
+        return __builtin_inff();
+    return (float)((x * s + room - 1) / room) * (PA_ITEM + (float)(len / 64)) + PA_RECORD * (float)s * records;
+}
+__device__ __forceinline__ int pa_pre_cut(const PrefixAttnParams &P, int blocks, int block_rows) {
+    const int s = (threadIdx.x & 63) + 1, x = P.n_kv * blocks;
+    float cost = pa_cost((int)P.pre.rows, s, x, P.xcd_slots * 8, (float)(x * block_rows));
+    if (s > 1 && (s > P.pre_splits || x * s > P.pre_items))
+        cost = __builtin_inff();
+    int best = s;
+    for (int o = 1; o < 64; o *= 2) {
+        const float c2 = __shfl_xor(cost, o);
+        const int b2 = __shfl_xor(best, o);
+        const bool take = c2 < cost || (c2 == cost && b2 < best);
+        cost = take ? c2 : cost;
+        best = take ? b2 : best;
+    }
+    return __builtin_amdgcn_readfirstlane(best);
 }
 
 template <int HDP, int RWP, int RWO>
@@ -448,21 +694,27 @@ __global__ __launch_bounds__(PA_THREADS, HDP == 256 ? 1 : 2) void prefix_attn_ke
     __shared__ int map[RM], lim[RM], scan[PA_THREADS / 64], flag;
     const int G = P.n_heads / P.n_kv, tid = threadIdx.x;
     if ((int)blockIdx.x < P.pre_items) {
-        // Work groups go to the eight XCDs in turn: the row blocks of one (key head, split) get numbers 8 apart, so
-        // they find its rows in one L2.
-        const int b = blockIdx.x, at = b >> 3;
-        const int ks = (b & 7) + 8 * (at / P.pre_blocks), rb = at % P.pre_blocks;
-        if (ks >= P.n_kv * P.pre_splits)
+        PaTokens last = {0, 0, 0};
+        const int tokens = pa_count(P, scan, last);
+        const int blocks = (tokens * G + RWP * 32 - 1) / (RWP * 32);
+        const int splits = P.q_len ? pa_pre_cut(P, blocks, RWP * 32) : P.pre_splits;
+        // Work groups go to the eight XCDs in turn: each XCD takes a run of items, so the row blocks of one (key head,
+        // split) find its rows in one L2.
+        const int all = P.n_kv * splits * blocks, per = (all + 7) / 8, at = blockIdx.x >> 3;
+        const int item = (blockIdx.x & 7) * per + at;
+        if (blockIdx.x == 0 && tid == 0)
+            *P.cut = splits;
+        if (at >= per || item >= all)
             return;
-        const int kvh = ks / P.pre_splits, sp = ks % P.pre_splits;
-        if (!pa_map_all<RWP * 32>(P, kvh, rb * RWP * 32, map, scan))
-            return;
-        const int rows = (int)P.pre.rows, k0 = sp * P.pre_len, k1 = k0 + P.pre_len < rows ? k0 + P.pre_len : rows;
+        const int ks = item / blocks, rb = item - ks * blocks, kvh = ks / splits, sp = ks - kvh * splits;
+        pa_map<RWP * 32>(P, kvh, rb * RWP * 32, tokens, last, map, lim, scan);
+        const int rows = (int)P.pre.rows, len = pa_split_len(rows, splits);
+        const int k0 = sp * len, k1 = k0 + len < rows ? k0 + len : rows;
         for (int r = tid; r < RWP * 32; r += PA_THREADS)
             lim[r] = k1;
         __syncthreads();
         pa_item<HDP, RWP>(P, P.pre.k + (size_t)kvh * P.pre.head_stride, P.pre.v + (size_t)kvh * P.pre.head_stride,
-                          P.pre.row_stride, k0, k1, k1, sp, map, lim, smem, &flag);
+                          P.pre.row_stride, k0, k1, k1, P.own_splits + sp, map, lim, smem, &flag);
     } else {
         int b = blockIdx.x - P.pre_items;
         const int rb = b % P.own_blocks;
@@ -478,17 +730,18 @@ __global__ __launch_bounds__(PA_THREADS, HDP == 256 ? 1 : 2) void prefix_attn_ke
             const bool in = r0 + r < L * G;
             const int j = (r0 + r) / G;
             map[r] = in ? (i * P.n_q + j) * P.n_heads + kvh * G + (r0 + r) % G : -1;
-            lim[r] = in ? pa_seen(len, L, j) : 0;
+            lim[r] = in ? pa_seen(len, L, j) : k1; // no query: nothing to take out, its scores are zero
         }
         __syncthreads();
         const size_t base = (size_t)i * P.own.lane_stride + (size_t)kvh * P.own.head_stride;
-        pa_item<HDP, RWO>(P, P.own.k + base, P.own.v + base, P.own.row_stride, k0, k1, pa_seen(len, L, 0),
-                          P.pre_splits + sp, map, lim, smem, &flag);
+        pa_item<HDP, RWO>(P, P.own.k + base, P.own.v + base, P.own.row_stride, k0, k1, pa_seen(len, L, 0), sp, map, lim,
+                          smem, &flag);
     }
 }
 
 // A row's records joined: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l, a wave per row.
 constexpr int PA_MERGE_ROWS = PA_THREADS / 64;
+template <int LPR>
 __global__ __launch_bounds__(PA_THREADS) void prefix_attn_merge_kernel(PrefixAttnParams P, int rows) {
     const int row = blockIdx.x * PA_MERGE_ROWS + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (row >= rows)
@@ -497,61 +750,93 @@ __global__ __launch_bounds__(PA_THREADS) void prefix_attn_merge_kernel(PrefixAtt
     if (j >= pa_q_len(P, i))
         return;
     const int len = pa_own_len(P, i);
-    // the slots that were written: the prefix's, and the own splits that start below the lane's length
-    const int own = P.own_splits ? (len + P.own_len_split - 1) / P.own_len_split : 0, slots = P.pre_splits + own;
+    // the slots that were written: the own splits that start below the lane's length, and the prefix's
+    const int own = P.own_splits ? (len + P.own_len_split - 1) / P.own_len_split : 0;
+    const int slots = own + (P.pre_splits ? *P.cut : 0), skip = P.own_splits - own;
     const float2 *ml = P.ml + (size_t)row * P.slots;
     const float *part = P.part + (size_t)row * P.slots * P.hd;
     float M = -__builtin_inff();
     for (int s = lane; s < slots; s += 64)
-        M = fmaxf(M, ml[s].x);
+        M = fmaxf(M, ml[s < own ? s : s + skip].x);
     M = wave_max(M);
+    // the wave's lanes as groups of LPR along the row, each with every GRP-th record
+    constexpr int GRP = 64 / LPR;
+    const int g = lane / LPR, d = lane % LPR * 4;
     float l = 0.0f;
     pa_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = 0; s < slots; s++) {
+#pragma unroll 4
+    for (int x = g; x < slots; x += GRP) {
+        const int s = x < own ? x : x + skip;
         const float2 r = ml[s];
+        const pa_f4 v = d < P.hd ? *(const pa_f4 *)(part + (size_t)s * P.hd + d) : pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
         const float w = r.x == M ? 1.0f : __builtin_amdgcn_exp2f(r.x - M);
         l += r.y * w;
-        if (lane * 4 < P.hd) {
-            const pa_f4 v = *(const pa_f4 *)(part + (size_t)s * P.hd + lane * 4);
-            o += v * w;
-        }
+        o += v * w;
+    }
+#pragma unroll
+    for (int x = LPR; x < 64; x *= 2) {
+        l += __shfl_xor(l, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            o[e] += __shfl_xor(o[e], x);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l; // nothing seen: zero
-    if (lane * 4 < P.hd)
-        *(pa_f4 *)(P.out + (size_t)row * P.hd + lane * 4) = o * inv;
+    if (g == 0 && d < P.hd)
+        *(pa_f4 *)(P.out + (size_t)row * P.hd + d) = o * inv;
 }
 
 // How a call is cut into items.
 struct PaPlan {
     int hdp, rwp, rwo;
-    int pre_blocks, pre_splits, pre_len, own_blocks, own_splits, own_len, slots;
+    int pre_splits, pre_items, xcd_slots, own_blocks, own_splits, own_len, slots;
     size_t rows;
 };
 static PaPlan pa_plan(size_t prefix_rows, size_t own_rows, size_t n, size_t n_q, size_t n_heads, size_t n_kv,
-                      size_t hd) {
+                      size_t hd, bool ragged) {
     PaPlan p = {};
-    const size_t G = n_heads / n_kv;
+    const size_t G = n_heads / n_kv, all = n * n_q * G, mine = n_q * G;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     p.rows = n * n_q * n_heads;
-    const size_t all = n * n_q * G, mine = n_q * G;
     p.rwp = all <= 32 ? 1 : all <= 64 ? 2 : 4;
     p.rwo = mine <= 32 ? 1 : 2;
-    constexpr size_t ITEMS = 512, MIN_ROWS = 128;
-    const auto cut = [](size_t rows, size_t others, int *splits, int *len) {
-        if (rows == 0)
-            return;
-        size_t s = (ITEMS + others - 1) / others, most = (rows + MIN_ROWS - 1) / MIN_ROWS;
-        s = s > most ? most : s < 1 ? 1 : s;
-        const size_t ln = ((rows + s - 1) / s + MIN_ROWS - 1) / MIN_ROWS * MIN_ROWS;
-        *len = (int)ln;
-        *splits = (int)((rows + ln - 1) / ln);
-    };
-    p.pre_blocks = (int)((all + 32 * p.rwp - 1) / (32 * p.rwp));
+    // the chip's work groups (two to a CU, one at head sizes over 128), shared by the tiles of the two kinds
+    const int slots = p.hdp == 256 ? 256 : 512;
     p.own_blocks = (int)((mine + 32 * p.rwo - 1) / (32 * p.rwo));
-    cut(prefix_rows, n_kv * p.pre_blocks, &p.pre_splits, &p.pre_len);
-    cut(own_rows, n * n_kv * p.own_blocks, &p.own_splits, &p.own_len);
+    const int pre_x = (int)(n_kv * ((all + 32 * p.rwp - 1) / (32 * p.rwp))), own_x = (int)(n * n_kv * p.own_blocks);
+    const double pre_work = (double)pre_x * ((prefix_rows + 63) / 64), own_work = (double)own_x * ((own_rows + 127) / 128);
+    const double share = prefix_rows ? pre_work / (pre_work + own_work) : 0.0;
+    const auto best = [&](size_t rows, int x, int room) {
+        int at = 1;
+        float least = __builtin_inff();
+        for (int s = 1; s <= 64; s++) {
+            const float cost = pa_cost((int)rows, s, x, room, (float)p.rows);
+            if (cost < least)
+                least = cost, at = s;
+        }
+        return at;
+    };
+    if (own_rows) {
+        const int room = (int)((1.0 - share) * slots);
+        p.own_splits = best(own_rows, own_x, room < 8 ? 8 : room);
+        p.own_len = pa_split_len((int)own_rows, p.own_splits);
+    }
+    if (prefix_rows) {
+        p.xcd_slots = (int)(share * slots / 8 < 1 ? 1 : share * slots / 8);
+        const int s = best(prefix_rows, pre_x, p.xcd_slots * 8);
+        p.pre_splits = s;
+        if (ragged) { // with fewer live rows there may be more of them: room for up to twice as many
+            const int most = (int)((prefix_rows + 127) / 128);
+            p.pre_splits = 2 * s + 2 < 64 ? 2 * s + 2 : 64;
+            p.pre_splits = p.pre_splits > most ? most : p.pre_splits;
+        }
+        const int64_t cap = (int64_t)pre_x * s > slots ? (int64_t)pre_x * s : slots;
+        p.pre_items = (int)((cap + 7) / 8 * 8);
+    }
     p.slots = p.pre_splits + p.own_splits;
     return p;
+}
+static size_t pa_ws_bytes(const PaPlan &p, size_t hd) {
+    return p.slots ? 16 + p.rows * p.slots * (hd * 4 + sizeof(float2)) : 0;
 }
 
 template <int HDP, int RWP>
@@ -603,8 +888,9 @@ size_t loomhip_prefix_attn_ws(size_t prefix_rows, size_t own_rows, size_t n, siz
                               size_t n_kv_heads, size_t head_dim) {
     if (!pa_served(n, n_q, n_heads, n_kv_heads, head_dim) || prefix_rows > PA_MAX_ROWS || own_rows > PA_MAX_ROWS)
         return 0;
-    const PaPlan p = pa_plan(prefix_rows, own_rows, n, n_q, n_heads, n_kv_heads, head_dim);
-    return p.rows * p.slots * (head_dim * 4 + sizeof(float2));
+    // the larger of the two plans: with q_len, and without
+    const PaPlan p = pa_plan(prefix_rows, own_rows, n, n_q, n_heads, n_kv_heads, head_dim, true);
+    return pa_ws_bytes(p, head_dim);
 }
 
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
@@ -627,13 +913,13 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: own rows without their lengths");
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
         return fail(LOOMHIP_DECLINED, "prefix_attn: q or out not at a multiple of 16 bytes");
-    const PaPlan p = pa_plan(prefix ? prefix->rows : 0, own ? own->rows : 0, n, n_q, n_heads, n_kv_heads, head_dim);
-    const size_t need = p.rows * p.slots * (head_dim * 4 + sizeof(float2));
+    const PaPlan p = pa_plan(prefix ? prefix->rows : 0, own ? own->rows : 0, n, n_q, n_heads, n_kv_heads, head_dim,
+                             q_len != nullptr);
+    const size_t need = pa_ws_bytes(p, head_dim);
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: the workspace takes %zu bytes at a multiple of 16, got %zu", need,
                     ws_bytes);
-    const size_t pre_items = p.pre_splits ? (n_kv_heads * p.pre_splits + 7) / 8 * 8 * p.pre_blocks : 0;
-    const size_t items = pre_items + n * n_kv_heads * p.own_splits * p.own_blocks;
+    const size_t items = p.pre_items + n * n_kv_heads * p.own_splits * p.own_blocks;
     if (items > 0xffffff)
         return fail(LOOMHIP_DECLINED, "prefix_attn: %zu work items not served", items);
     if (int rc = require_device())
@@ -653,16 +939,16 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
     P.hd = (int)head_dim;
     P.scale = scale;
     P.out = out;
-    P.pre_blocks = p.pre_blocks;
     P.pre_splits = p.pre_splits;
-    P.pre_len = p.pre_len;
+    P.pre_items = p.pre_items;
+    P.xcd_slots = p.xcd_slots;
     P.own_blocks = p.own_blocks;
     P.own_splits = p.own_splits;
     P.own_len_split = p.own_len;
-    P.pre_items = (int)pre_items;
     P.slots = p.slots;
-    P.part = (float *)ws;
-    P.ml = (float2 *)((char *)ws + p.rows * p.slots * head_dim * 4);
+    P.cut = (int *)ws;
+    P.part = (float *)((char *)ws + 16);
+    P.ml = (float2 *)(P.part + p.rows * p.slots * head_dim);
     hipStream_t st = stream_of(stream);
     if (items) {
         if (p.hdp == 64)
@@ -673,8 +959,13 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
             pa_launch<256>(p, P, items, st);
         note_launch();
     }
-    hipLaunchKernelGGL(prefix_attn_merge_kernel, dim3((p.rows + PA_MERGE_ROWS - 1) / PA_MERGE_ROWS), dim3(PA_THREADS), 0,
-                       st, P, (int)p.rows);
+    const dim3 mg((p.rows + PA_MERGE_ROWS - 1) / PA_MERGE_ROWS);
+    if (p.hdp == 64)
+        hipLaunchKernelGGL(prefix_attn_merge_kernel<16>, mg, dim3(PA_THREADS), 0, st, P, (int)p.rows);
+    else if (p.hdp == 128)
+        hipLaunchKernelGGL(prefix_attn_merge_kernel<32>, mg, dim3(PA_THREADS), 0, st, P, (int)p.rows);
+    else
+        hipLaunchKernelGGL(prefix_attn_merge_kernel<64>, mg, dim3(PA_THREADS), 0, st, P, (int)p.rows);
     note_launch();
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "prefix_attn launch");
