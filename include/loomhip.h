@@ -810,8 +810,9 @@ typedef struct {
  * of the cache past a query's own are not part of its result, whatever they
  * hold (a cached NaN or infinity makes the rows that see it NaN).
  * prefix->rows or own->rows may be 0 (no rows; pointers unused).
- * head_dim a multiple of 8 up to 256, strides multiples of 8, pointers at a
- * multiple of 16 bytes; DECLINED otherwise. */
+ * head_dim a multiple of 8 up to 256, strides multiples of 8 (rows at most
+ * 2^23 apart), pointers at a multiple of 16 bytes, n up to 65535, n_q up to
+ * 4096; DECLINED otherwise. */
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
                             const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,
                             size_t n_kv_heads, size_t head_dim, float scale, float *out, void *ws, size_t ws_bytes,

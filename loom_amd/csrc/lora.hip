@@ -2,12 +2,25 @@
 // out_t = base_t + s_e * B_e (A_e x_t), e the adapter of vector t (none: base_t).
 // Everything is f32: the adapters' values widened exactly, products and sums
 // in f32, as the projection's own activations and outputs are.
+//
+// Two launches: y = A_e x for every vector into the workspace, then out.  In
+// decode (most vectors name adapters of their own, so the adapters' bytes are
+// the work) a wave takes a few rows of A_e or B_e for one vector with plain
+// multiply-adds.  In prefill (a request's tokens share an adapter) 16 vectors
+// of one adapter are the columns of f32 matrix-core tiles
+// (v_mfma_f32_16x16x4_f32), found among 128 vectors at a time.  What an
+// adapter holds reaches its own vectors only.
 #include "runtime.hpp"
+
+#include <type_traits>
 
 namespace lh {
 
+typedef float lora_f4 __attribute__((ext_vector_type(4)));
+
 constexpr int LORA_THREADS = 256;
 constexpr int LORA_MAX_RANK = 256;
+constexpr double LORA_FEW = 160e6; // bytes
 
 struct LoraParams {
     const void *a, *b; // [n_adapters][rank][cols], [n_adapters][rows][rank]
@@ -18,7 +31,11 @@ struct LoraParams {
     const int32_t *ids;
     float *out;
     size_t n, x_stride, base_stride, out_stride;
+    float *y;   // [ks][n][rp]: scale * A_e x over each split
+    int rp, ks; // rank rounded up to 16, splits of the columns
 };
+
+constexpr size_t LORA_MAX_N = 65535 * 64; // vectors, and rows: the launches' work groups
 
 // Whether two device ranges [p, p + elements) share a byte.
 static bool overlap(const void *p, size_t pn, const void *q, size_t qn) {
@@ -37,6 +54,8 @@ static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, co
     if (l->n_adapters == 0 || l->rows == 0 || l->cols == 0 || l->n_adapters > 0x7fffffff || l->rows > 0x7fffffff ||
         l->cols > 0x7fffffff || n > 0x7fffffff)
         return fail(LOOMHIP_ERR_ARG, "lora: %zu vectors, %zu adapters of %zu x %zu", n, l->n_adapters, l->rows, l->cols);
+    if (n > LORA_MAX_N || l->rows > LORA_MAX_N)
+        return fail(LOOMHIP_DECLINED, "lora: %zu vectors, %zu rows not served", n, l->rows);
     if (n && (!l->a || !l->b || !l->scale || !x || !ids || !out))
         return fail(LOOMHIP_ERR_ARG, "lora: null argument");
     if (x_stride < l->cols || out_stride < l->rows || (base && base_stride < l->rows))
@@ -51,53 +70,519 @@ static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, co
     if (n && base && !(base == out && base_stride == out_stride) && overlap(out, on, base, (n - 1) * base_stride + l->rows))
         return fail(LOOMHIP_ERR_ARG, "lora: out overlaps base without being it");
     P = {l->a, l->b, l->scale, l->n_adapters, l->rows, l->cols, (int)l->rank, x, base, ids, out, n, x_stride,
-         base_stride, out_stride};
+         base_stride, out_stride, nullptr, 0, 1};
     return LOOMHIP_OK;
 }
 
 
+// Four consecutive elements as f32, and one.
 template <typename T>
-__device__ __forceinline__ float lora_widen(T v);
-template <>
-__device__ __forceinline__ float lora_widen(float v) { return v; }
-template <>
-__device__ __forceinline__ float lora_widen(_Float16 v) { return (float)v; }
-template <>
-__device__ __forceinline__ float lora_widen(uint16_t v) { return __uint_as_float((uint32_t)v << 16); } // bf16
+__device__ __forceinline__ float lora_one(const T *p) {
+    if constexpr (std::is_same_v<T, uint16_t>) // bf16
+        return __uint_as_float((uint32_t)*p << 16);
+    else
+        return (float)*p;
+}
+template <typename T>
+__device__ __forceinline__ lora_f4 lora_four(const T *p) {
+    if constexpr (std::is_same_v<T, float>) {
+        return *(const lora_f4 *)p;
+    } else {
+        const uint2 v = *(const uint2 *)p;
+        if constexpr (std::is_same_v<T, uint16_t>)
+            return lora_f4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                           __uint_as_float(v.y & 0xffff0000u)};
+        else
+            return lora_f4{half_bits_to_float(v.x), half_bits_to_float(v.x >> 16), half_bits_to_float(v.y),
+                           half_bits_to_float(v.y >> 16)};
+    }
+}
+// Elements k .. k + 3 of a row of `len`, zero past its end.  VEC: the row starts at a multiple of four elements' bytes
+// and so does every k.
+template <bool VEC, typename T>
+__device__ __forceinline__ lora_f4 lora_at(const T *row, size_t k, size_t len) {
+    lora_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (VEC) {
+        if (k < len) // len a multiple of 4
+            v = lora_four(row + k);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (k + i < len)
+                v[i] = lora_one(row + k + i);
+    }
+    return v;
+}
+// Eight from a 16-byte aligned place of a 16-bit row (two times four of a wider one).
+template <typename T>
+__device__ __forceinline__ void lora_eight(const T *p, float *v) {
+    if constexpr (std::is_same_v<T, float>) {
+        const lora_f4 a = *(const lora_f4 *)p, b = *(const lora_f4 *)(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            v[i] = a[i], v[4 + i] = b[i];
+    } else {
+        const uint4 w = *(const uint4 *)p;
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = std::is_same_v<T, uint16_t> ? __uint_as_float(u[i] << 16) : half_bits_to_float(u[i]);
+            v[2 * i + 1] = std::is_same_v<T, uint16_t> ? __uint_as_float(u[i] & 0xffff0000u) : half_bits_to_float(u[i] >> 16);
+        }
+    }
+}
+// The sum over aligned groups of L lanes, in all of them.
+template <int L>
+__device__ __forceinline__ float lora_sum(float v) {
+    if constexpr (L >= 2)
+        v += dpp_f<0xB1>(v, v);
+    if constexpr (L >= 4)
+        v += dpp_f<0x4E>(v, v);
+    if constexpr (L >= 8)
+        v += dpp_f<0x141>(v, v);
+    if constexpr (L >= 16)
+        v += dpp_f<0x140>(v, v);
+    if constexpr (L >= 32)
+        v += __shfl_xor(v, 16);
+    if constexpr (L >= 64)
+        v += __shfl_xor(v, 32);
+    return v;
+}
+__device__ __forceinline__ bool lora_names(const LoraParams &P, int e) { return e >= 0 && (size_t)e < P.n_adapters; }
 
-// One work group per vector: its `rank` values A_e x, a wave each in turn, then its output rows.
-template <typename T>
-__global__ __launch_bounds__(LORA_THREADS) void lora_kernel(LoraParams P) {
-    __shared__ float y[LORA_MAX_RANK];
-    const size_t t = blockIdx.x;
-    const int e = P.ids[t];
+// ---- few vectors ------------------------------------------------------------------
+// y[t][r .. r + RPW): a wave per RPW rows of A_e, a lane every 64th group of eight columns (of four, one by one, where
+// rows are not 16-byte aligned).
+template <typename T, bool VEC, int RPW>
+__global__ __launch_bounds__(LORA_THREADS) void lora_few_y_kernel(LoraParams P) {
+    const size_t t = blockIdx.y;
+    const int e = P.ids[t], lane = threadIdx.x & 63;
+    const int r0 = (blockIdx.x * (LORA_THREADS / 64) + (threadIdx.x >> 6)) * RPW;
+    if (!lora_names(P, e) || r0 >= P.rank)
+        return;
     const float *x = P.x + t * P.x_stride;
+    const T *a[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; i++)
+        a[i] = (const T *)P.a + ((size_t)e * P.rank + (r0 + i < P.rank ? r0 + i : P.rank - 1)) * P.cols;
+    float s[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; i++)
+        s[i] = 0.0f;
+    if constexpr (VEC) {
+#pragma unroll 2
+        for (size_t k = lane * 8; k < P.cols; k += 512) {
+            float xv[8], av[RPW][8];
+            lora_eight(x + k, xv);
+#pragma unroll
+            for (int i = 0; i < RPW; i++)
+                lora_eight(a[i] + k, av[i]);
+#pragma unroll
+            for (int i = 0; i < RPW; i++)
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    s[i] = __builtin_fmaf(av[i][c], xv[c], s[i]);
+        }
+    } else {
+#pragma unroll 8
+        for (size_t k = lane; k < P.cols; k += 64)
+#pragma unroll
+            for (int i = 0; i < RPW; i++)
+                s[i] = __builtin_fmaf(lora_one(a[i] + k), x[k], s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < RPW; i++) {
+        s[i] = lora_sum<64>(s[i]);
+        if (lane == 0 && r0 + i < P.rank)
+            P.y[t * P.rp + r0 + i] = s[i] * P.scale[e];
+    }
+}
+
+// out[t][..]: LPR lanes per row of B_e, each with the same ranks of every row (its part of y stays in registers): Q times
+// eight in a row (VEC), else Q times eight that lie LPR apart.  LORA_PASSES passes of 64 / LPR rows a wave.
+constexpr int LORA_PASSES = 4;
+template <typename T, bool VEC, int LPR, int Q>
+__global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P) {
+    constexpr int RPI = 64 / LPR, W = LORA_THREADS / 64;
+    const size_t t = blockIdx.y;
+    const int e = P.ids[t], lane = threadIdx.x & 63, sub = lane % LPR;
+    const size_t w0 = ((size_t)blockIdx.x * W + (threadIdx.x >> 6)) * (LORA_PASSES * RPI);
     const float *base = P.base ? P.base + t * P.base_stride : nullptr;
     float *out = P.out + t * P.out_stride;
-    const int tid = threadIdx.x, lane = tid & 63;
-    if (e < 0 || e >= (int)P.n_adapters) {
-        for (size_t r = tid; r < P.rows; r += LORA_THREADS)
-            out[r] = base ? base[r] : 0.0f;
-        return;
+    const bool named = lora_names(P, e);
+    const T *b = (const T *)P.b + (named ? (size_t)e * P.rows * P.rank : 0);
+    const int rank = P.rank;
+    float y[Q][8], v[LORA_PASSES][Q][8], o[LORA_PASSES];
+    const auto k_of = [&](int q, int c) { return VEC ? (q * LPR + sub) * 8 + c : (q * 8 + c) * LPR + sub; };
+#pragma unroll
+    for (int p = 0; p < LORA_PASSES; p++) {
+        const size_t r = w0 + p * RPI + lane / LPR, at = r < P.rows ? r : P.rows - 1;
+        o[p] = base ? base[at] : 0.0f;
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            if constexpr (VEC) {
+                // ranks past the last are the first ones again, against a y of zero
+                lora_eight(b + at * rank + (k_of(q, 0) < rank ? k_of(q, 0) : 0), v[p][q]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    v[p][q][c] = k_of(q, c) < rank ? lora_one(b + at * rank + k_of(q, c)) : 0.0f;
+            }
+        }
     }
-    const T *a = (const T *)P.a + (size_t)e * P.rank * P.cols;
-    const T *b = (const T *)P.b + (size_t)e * P.rows * P.rank;
-    for (int k = tid >> 6; k < P.rank; k += LORA_THREADS / 64) {
+#pragma unroll
+    for (int q = 0; q < Q; q++)
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            y[q][c] = k_of(q, c) < rank ? P.y[t * P.rp + k_of(q, c)] : 0.0f;
+#pragma unroll
+    for (int p = 0; p < LORA_PASSES; p++) {
+        const size_t r = w0 + p * RPI + lane / LPR;
         float s = 0.0f;
-        for (size_t c = lane; c < P.cols; c += 64)
-            s = __builtin_fmaf(lora_widen(a[k * P.cols + c]), x[c], s);
-        for (int o = 1; o < 64; o *= 2)
-            s += __shfl_xor(s, o);
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                s = k_of(q, c) < rank ? __builtin_fmaf(v[p][q][c], y[q][c], s) : s;
+        s = lora_sum<LPR>(s);
+        if (sub == 0 && r < P.rows)
+            out[r] = named ? o[p] + s : o[p];
+    }
+}
+
+// ---- many vectors -----------------------------------------------------------------
+// Tiles of v_mfma_f32_16x16x4_f32 with 16 vectors as columns: lane l has column l % 16 and, of four contracted indices,
+// l / 16; four products take 16 indices, lane group g those 4 g .. 4 g + 3, which both operands read as one load.  The
+// result: column l % 16, rows 4 (l / 16) + i.
+
+// The vectors of a block of LORA_BLOCK, put together by adapter: tiles of up to 16 vectors that name one (or none).
+// Where a request's tokens follow one another the runs of one adapter are cut into tiles as they stand (a vector's place
+// follows from two ballots).  Where that gives more than half as many tiles again as 16 in each, every vector finds its
+// place by comparing its adapter with the block's others.
+constexpr int LORA_BLOCK = 128;
+struct LoraTiles {
+    int key[LORA_BLOCK], count[LORA_BLOCK]; // of each vector its adapter, -1: none; of an adapter's first one its tiles
+    int adapter[LORA_BLOCK];                // of each tile
+    short vec[LORA_BLOCK][16];              // of each tile its vectors, -1 past the last
+    unsigned long long starts[2];           // of runs, then of tiles
+};
+__device__ __forceinline__ int lora_tiles(const LoraParams &P, size_t t0, LoraTiles &L) {
+    static_assert(LORA_BLOCK == 128, "two waves");
+    const int i = threadIdx.x, wave = i >> 6, lane = i & 63;
+    const int here = P.n - t0 < LORA_BLOCK ? (int)(P.n - t0) : LORA_BLOCK;
+    int key = -2; // past the last vector: nobody's
+    if (i < LORA_BLOCK) {
+        if (i < here) {
+            key = P.ids[t0 + i];
+            key = lora_names(P, key) ? key : -1;
+        }
+        L.key[i] = key;
+    }
+    for (int c = i; c < LORA_BLOCK * 8; c += blockDim.x)
+        ((int *)&L.vec[0][0])[c] = -1;
+    __syncthreads();
+    const bool in = i < here;
+    // The newest set bit at or before vector i, and how many there are up to it.
+    const unsigned long long upto = ~0ull >> (63 - lane);
+    if (wave < 2) {
+        const unsigned long long s = __ballot(in && (i == 0 || L.key[i - 1] != key));
         if (lane == 0)
-            y[k] = s * P.scale[e];
+            L.starts[wave] = s;
     }
     __syncthreads();
-    for (size_t r = tid; r < P.rows; r += LORA_THREADS) {
-        float s = 0.0f;
-        for (int k = 0; k < P.rank; k++)
-            s = __builtin_fmaf(lora_widen(b[r * P.rank + k]), y[k], s);
-        out[r] = base ? base[r] + s : s;
+    int at = 0;
+    if (wave < 2) {
+        const unsigned long long mine = L.starts[wave] & upto;
+        at = i - (mine ? wave * 64 + 63 - __builtin_clzll(mine) : 63 - __builtin_clzll(L.starts[0]));
     }
+    __syncthreads();
+    if (wave < 2) {
+        const unsigned long long s = __ballot(in && at % 16 == 0);
+        if (lane == 0)
+            L.starts[wave] = s;
+    }
+    __syncthreads();
+    int n = __popcll(L.starts[0]) + __popcll(L.starts[1]);
+    int tile = 0;
+    if (wave < 2)
+        tile = __popcll(L.starts[wave] & upto) - 1 + (wave ? __popcll(L.starts[0]) : 0);
+    if (n > (here + 15) / 16 + LORA_BLOCK / 32) {
+        const int4 *keys = (const int4 *)L.key, *counts = (const int4 *)L.count;
+        int before = 0, same = 0; // vectors of the same adapter in front, and all
+        if (i < LORA_BLOCK) {
+#pragma unroll 4
+            for (int j = 0; j < LORA_BLOCK / 4; j++) {
+                const int4 k = keys[j];
+                const int m = (k.x == key) | (k.y == key) << 1 | (k.z == key) << 2 | (k.w == key) << 3;
+                same += __popc(m);
+                before += __popc(4 * j + 4 <= i ? m : 4 * j < i ? m & ((1 << (i - 4 * j)) - 1) : 0);
+            }
+            L.count[i] = in && before == 0 ? (same + 15) / 16 : 0;
+        }
+        __syncthreads();
+        tile = n = 0;
+        at = before;
+#pragma unroll 4
+        for (int j = 0; j < LORA_BLOCK / 4; j++) {
+            const int4 k = keys[j], c = counts[j];
+            tile += (k.x < key ? c.x : 0) + (k.y < key ? c.y : 0) + (k.z < key ? c.z : 0) + (k.w < key ? c.w : 0);
+            n += c.x + c.y + c.z + c.w;
+        }
+        tile += before / 16;
+    }
+    if (in) {
+        L.vec[tile][at % 16] = (short)i;
+        L.adapter[tile] = key;
+    }
+    __syncthreads();
+    return n;
+}
+
+// y for every LORA_Z-th tile of a block and one of ks splits of the columns: W waves take an equal part each, their sums
+// meet in LDS.  The second launch adds the splits, once for every 64 rows, so there are as few as fill the chip.  RT: tiles
+// of 16 ranks.
+constexpr int LORA_Z = LORA_BLOCK / 16;
+__host__ __device__ constexpr int lora_y_waves(int rt) { return rt <= 8 ? 8 : 4; }
+template <typename T, bool VEC, int RT>
+__global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(LoraParams P) {
+    constexpr int W = lora_y_waves(RT);
+    __shared__ lora_f4 part[W][RT][64];
+    __shared__ LoraTiles L;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const size_t t0 = (size_t)blockIdx.x * LORA_BLOCK;
+    const int tiles = lora_tiles(P, t0, L);
+    const size_t share = (P.cols + 16 * W * P.ks - 1) / (16 * W * P.ks) * 16; // columns a wave
+    const size_t k0 = (blockIdx.z * W + wave) * share, k1 = k0 + share < P.cols ? k0 + share : P.cols;
+    for (int tile = blockIdx.y; tile < tiles; tile += LORA_Z) {
+        const int e = L.adapter[tile], v = L.vec[tile][col];
+        if (e < 0)
+            continue;
+        const size_t t = t0 + (v < 0 ? L.vec[tile][0] : v);
+        const float *x = P.x + t * P.x_stride;
+        const T *a = (const T *)P.a + (size_t)e * P.rank * P.cols;
+        lora_f4 acc[RT];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+            acc[r] = lora_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int KB = RT <= 2 ? 8 : RT == 4 ? 4 : 2; // groups of 16 columns loaded together, a row's lines at a time
+        for (size_t k = k0 + g * 4; k - g * 4 < k1; k += 16 * KB) {
+            lora_f4 xv[KB], av[KB][RT];
+#pragma unroll
+            for (int q = 0; q < KB; q++)
+                xv[q] = lora_at<VEC>(x, k + q * 16, k1);
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                // ranks past the last: the last one's, dropped with the rows of y
+                const int row = r * 16 + col < P.rank ? r * 16 + col : P.rank - 1;
+#pragma unroll
+                for (int q = 0; q < KB; q++)
+                    av[q][r] = lora_at<VEC>(a + (size_t)row * P.cols, k + q * 16, k1);
+            }
+#pragma unroll
+            for (int q = 0; q < KB; q++)
+#pragma unroll
+                for (int r = 0; r < RT; r++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(av[q][r][c], xv[q][c], acc[r], 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+            part[wave][r][lane] = acc[r];
+        __syncthreads();
+        for (int r = wave; r < RT; r += W) {
+            lora_f4 y = part[0][r][lane];
+#pragma unroll
+            for (int w = 1; w < W; w++)
+                y += part[w][r][lane];
+            if (v >= 0 && r * 16 < P.rp)
+                *(lora_f4 *)(P.y + ((size_t)blockIdx.z * P.n + t) * P.rp + r * 16 + g * 4) = y * P.scale[e];
+        }
+        __syncthreads();
+    }
+}
+
+// out for a block's vectors and 64 rows: a wave every LORA_OW-th tile, M-tile m the rows 16 m + .. of B_e.  The products leave
+// a lane 16 bytes of 16 vectors' rows; through LDS the wave reads base and writes out as 256 bytes of a row at a time.
+constexpr int LORA_OW = 8, LORA_OUT = 64, LORA_OUT_PAD = LORA_OUT + 4;
+template <typename T, bool VEC, bool OVEC>
+__global__ __launch_bounds__(64 * LORA_OW) void lora_many_out_kernel(LoraParams P) {
+    constexpr int MT = LORA_OUT / 16;
+    __shared__ LoraTiles L;
+    __shared__ lora_f4 turn[LORA_OW][16 * LORA_OUT_PAD / 4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const size_t t0 = (size_t)blockIdx.y * LORA_BLOCK, r0 = (size_t)blockIdx.x * LORA_OUT;
+    const int tiles = lora_tiles(P, t0, L);
+    float *const mine = (float *)turn[wave]; // [vector][row], rows padded against bank conflicts
+    for (int tile = wave; tile < tiles; tile += LORA_OW) {
+        const int e = L.adapter[tile];
+        // four rows of 16 lanes' four values each (OVEC), or one of 64 lanes' one, a pass
+        constexpr int PASS = OVEC ? 4 : 16, PER = 16 / PASS;
+        int v[PASS];
+        lora_f4 o[PASS];
+        const size_t row = r0 + (OVEC ? (lane & 15) * 4 : lane);
+#pragma unroll
+        for (int p = 0; p < PASS; p++) {
+            v[p] = L.vec[tile][p * PER + (OVEC ? lane >> 4 : 0)];
+            o[p] = lora_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (P.base && v[p] >= 0 && row < P.rows) {
+                const float *b = P.base + (t0 + v[p]) * P.base_stride + row;
+                if constexpr (OVEC)
+                    o[p] = *(const lora_f4 *)b;
+                else
+                    o[p][0] = *b;
+            }
+        }
+        if (e >= 0) {
+            const int c0 = L.vec[tile][col];
+            const size_t t = t0 + (c0 < 0 ? L.vec[tile][0] : c0);
+            const T *b = (const T *)P.b + (size_t)e * P.rows * P.rank;
+            lora_f4 acc[MT];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+                acc[m] = lora_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+            for (int k = g * 4; k - g * 4 < P.rank; k += 16) {
+                lora_f4 y = *(const lora_f4 *)(P.y + t * P.rp + k);
+                for (int s = 1; s < P.ks; s++)
+                    y += *(const lora_f4 *)(P.y + ((size_t)s * P.n + t) * P.rp + k);
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const size_t r = r0 + m * 16 + col;
+                    const lora_f4 bv = lora_at<VEC>(b + (r < P.rows ? r : P.rows - 1) * P.rank, k, P.rank);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        // ranks past the last are zero in b; y there may be anything
+                        acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[c], k + c < P.rank ? y[c] : 0.0f, acc[m], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+                *(lora_f4 *)(mine + col * LORA_OUT_PAD + m * 16 + g * 4) = acc[m];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int p = 0; p < PASS; p++) {
+                if constexpr (OVEC)
+                    o[p] += *(const lora_f4 *)(mine + (p * PER + (lane >> 4)) * LORA_OUT_PAD + (lane & 15) * 4);
+                else
+                    o[p][0] += mine[p * LORA_OUT_PAD + lane];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int p = 0; p < PASS; p++)
+            if (v[p] >= 0 && row < P.rows) {
+                float *out = P.out + (t0 + v[p]) * P.out_stride + row;
+                if constexpr (OVEC)
+                    *(lora_f4 *)out = o[p];
+                else
+                    *out = o[p][0];
+            }
+    }
+}
+
+template <typename T, bool VB, int LPR, int Q>
+static void lora_few_out(const LoraParams &P, hipStream_t st) {
+    const size_t rows = (LORA_THREADS / 64) * LORA_PASSES * (64 / LPR);
+    hipLaunchKernelGGL((lora_few_out_kernel<T, VB, LPR, Q>), dim3((P.rows + rows - 1) / rows, P.n), dim3(LORA_THREADS), 0,
+                       st, P);
+}
+template <typename T, bool VA, bool VB>
+static void lora_few(const LoraParams &P, hipStream_t st) {
+    constexpr int W = LORA_THREADS / 64;
+    // rows of A_e a wave: one while that leaves the chip few waves, else two (a vector is read once for both)
+    const int rpw = P.n * P.rank <= 2048 ? 1 : 2;
+    const dim3 gy((P.rank + W * rpw - 1) / (W * rpw), P.n);
+    if (rpw == 1)
+        hipLaunchKernelGGL((lora_few_y_kernel<T, VA, 1>), gy, dim3(LORA_THREADS), 0, st, P);
+    else
+        hipLaunchKernelGGL((lora_few_y_kernel<T, VA, 2>), gy, dim3(LORA_THREADS), 0, st, P);
+    if (P.rank <= 8)
+        lora_few_out<T, VB, 1, 1>(P, st);
+    else if (P.rank <= 16)
+        lora_few_out<T, VB, 2, 1>(P, st);
+    else if (P.rank <= 32)
+        lora_few_out<T, VB, 4, 1>(P, st);
+    else if (P.rank <= 64)
+        lora_few_out<T, VB, 8, 1>(P, st);
+    else if (P.rank <= 128)
+        lora_few_out<T, VB, 16, 1>(P, st);
+    else
+        lora_few_out<T, VB, 16, 2>(P, st);
+}
+
+template <typename T, bool VA, int RT>
+static void lora_many_y(const LoraParams &P, hipStream_t st) {
+    hipLaunchKernelGGL((lora_many_y_kernel<T, VA, RT>), dim3((P.n + LORA_BLOCK - 1) / LORA_BLOCK, LORA_Z, P.ks),
+                       dim3(64 * lora_y_waves(RT)), 0, st, P);
+}
+template <typename T, bool VA>
+static void lora_many_y(const LoraParams &P, hipStream_t st) {
+    if (P.rp <= 16)
+        lora_many_y<T, VA, 1>(P, st);
+    else if (P.rp <= 32)
+        lora_many_y<T, VA, 2>(P, st);
+    else if (P.rp <= 64)
+        lora_many_y<T, VA, 4>(P, st);
+    else if (P.rp <= 128)
+        lora_many_y<T, VA, 8>(P, st);
+    else
+        lora_many_y<T, VA, 16>(P, st);
+}
+template <typename T, bool VB>
+static void lora_many_out(const LoraParams &P, bool ovec, hipStream_t st) {
+    const dim3 g((P.rows + LORA_OUT - 1) / LORA_OUT, (P.n + LORA_BLOCK - 1) / LORA_BLOCK);
+    if (ovec)
+        hipLaunchKernelGGL((lora_many_out_kernel<T, VB, true>), g, dim3(64 * LORA_OW), 0, st, P);
+    else
+        hipLaunchKernelGGL((lora_many_out_kernel<T, VB, false>), g, dim3(64 * LORA_OW), 0, st, P);
+}
+
+// Whether the vectors are taken one by one: while all their reads of A_e and B_e, mostly from L2, stay under LORA_FEW
+// bytes.  Measured at 4096 x 2048, rank 64, fp16: 101 MB (128 vectors) 17 us one by one, 21 as tiles, 41 as tiles of
+// mixed requests; 201 MB 29, 21, 42; 403 MB 52, 22, 45.
+static bool lora_is_few(const LoraParams &P, size_t es) {
+    return P.n <= 65535 && (double)P.n * P.rank * (P.rows + P.cols) * es <= LORA_FEW;
+}
+// Loads of four elements where rows and pointers allow them: A_e's rows and x for the first launch, B_e's for the
+// second (base and out beside them where many vectors are tiles).
+template <typename T>
+static void lora_run(const LoraParams &P, hipStream_t st) {
+    const size_t q = 4 * sizeof(T);
+    const bool va = P.cols % 4 == 0 && (uintptr_t)P.a % q == 0 && (uintptr_t)P.x % 16 == 0 && P.x_stride % 4 == 0;
+    const bool vb = P.rank % 4 == 0 && (uintptr_t)P.b % q == 0;
+    const bool ovec = P.rows % 4 == 0 && (uintptr_t)P.out % 16 == 0 && P.out_stride % 4 == 0 &&
+                      (!P.base || ((uintptr_t)P.base % 16 == 0 && P.base_stride % 4 == 0));
+    if (lora_is_few(P, sizeof(T))) {
+        const bool va8 = va && P.cols % 8 == 0 && (uintptr_t)P.a % 16 == 0;
+        const bool vb8 = P.rank % 8 == 0 && (uintptr_t)P.b % 16 == 0;
+        if (va8 && vb8)
+            lora_few<T, true, true>(P, st);
+        else if (va8)
+            lora_few<T, true, false>(P, st);
+        else if (vb8)
+            lora_few<T, false, true>(P, st);
+        else
+            lora_few<T, false, false>(P, st);
+        return;
+    }
+    if (va)
+        lora_many_y<T, true>(P, st);
+    else
+        lora_many_y<T, false>(P, st);
+    if (vb)
+        lora_many_out<T, true>(P, ovec, st);
+    else
+        lora_many_out<T, false>(P, ovec, st);
+}
+
+// Splits of the columns: a work group for every CU, none under 512 columns.
+static int lora_splits(size_t cols, size_t n) {
+    const size_t tiles = (n + 15) / 16, s = (256 + tiles - 1) / tiles, most = (cols + 511) / 512;
+    return (int)(s > most ? most : s > 4 ? 4 : s);
+}
+static size_t lora_ws_bytes(const loomhip_lora *l, size_t n) {
+    return lora_splits(l->cols, n) * n * ((l->rank + 15) / 16 * 16) * 4;
 }
 
 } // namespace lh
@@ -106,7 +591,9 @@ using namespace lh;
 
 extern "C" {
 
-size_t loomhip_lora_ws(const loomhip_lora *l, size_t n) { return 0; }
+size_t loomhip_lora_ws(const loomhip_lora *l, size_t n) {
+    return l && l->rank && l->rank <= LORA_MAX_RANK && l->cols && l->rows && n <= LORA_MAX_N ? lora_ws_bytes(l, n) : 0;
+}
 
 int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, const int32_t *ids, const float *base,
                      size_t base_stride, size_t n, float *out, size_t out_stride, void *ws, size_t ws_bytes,
@@ -116,15 +603,22 @@ int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, con
         return rc;
     if (n == 0)
         return LOOMHIP_OK;
+    const size_t need = lora_ws_bytes(l, n);
+    if (!ws || ws_bytes < need || (uintptr_t)ws % 16)
+        return fail(LOOMHIP_ERR_ARG, "lora: the workspace takes %zu bytes at a multiple of 16, got %zu", need, ws_bytes);
     if (int rc = require_device())
         return rc;
+    P.y = (float *)ws;
+    P.rp = (int)((l->rank + 15) / 16 * 16);
+    P.ks = lora_splits(l->cols, n);
     hipStream_t st = stream_of(stream);
     if (l->type == LH_F32)
-        hipLaunchKernelGGL(lora_kernel<float>, dim3(n), dim3(LORA_THREADS), 0, st, P);
+        lora_run<float>(P, st);
     else if (l->type == LH_F16)
-        hipLaunchKernelGGL(lora_kernel<_Float16>, dim3(n), dim3(LORA_THREADS), 0, st, P);
+        lora_run<_Float16>(P, st);
     else
-        hipLaunchKernelGGL(lora_kernel<uint16_t>, dim3(n), dim3(LORA_THREADS), 0, st, P);
+        lora_run<uint16_t>(P, st);
+    note_launch();
     note_launch();
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "lora launch");

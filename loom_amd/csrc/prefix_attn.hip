@@ -861,6 +861,7 @@ static void pa_launch(const PaPlan &p, const PrefixAttnParams &P, size_t items, 
 using namespace lh;
 
 constexpr size_t PA_MAX_ROWS = 0x3fffffff;
+constexpr size_t PA_MAX_STRIDE = (size_t)1 << 23; // the rows of a tile (128) at 32-bit byte offsets from its first
 // The sizes the kernels index in 32 bits.
 static bool pa_served(size_t n, size_t n_q, size_t n_heads, size_t n_kv, size_t hd) {
     return n && n <= 65535 && n_q && n_q <= 4096 && n_heads && n_heads <= 65535 && n_kv && n_heads % n_kv == 0 && hd &&
@@ -876,6 +877,8 @@ static int kv_rows_check(const loomhip_kv_rows *r, size_t n_kv, size_t hd, bool 
         return fail(LOOMHIP_DECLINED, "prefix_attn: %zu %s rows not served", r->rows, what);
     if (r->row_stride < hd && r->rows > 1)
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: %s row stride %zu below a head", what, r->row_stride);
+    if (r->row_stride > PA_MAX_STRIDE)
+        return fail(LOOMHIP_DECLINED, "prefix_attn: %s rows %zu elements apart not served", what, r->row_stride);
     if ((uintptr_t)r->k % 16 || (uintptr_t)r->v % 16 || r->row_stride % 8 || r->head_stride % 8 ||
         (lanes && r->lane_stride % 8))
         return fail(LOOMHIP_DECLINED, "prefix_attn: %s rows not at multiples of 16 bytes", what);

@@ -17,62 +17,71 @@ library refuses or does not serve ``LoomHipError``.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+
+import torch
 
 from . import BF16, F16, F32, KvRowsDesc, LoomHipError, LoraDesc, OK, last_error, lib
-from .backend import _stream
 
-_LORA_TYPES = {}
+_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
+_LORA_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_HALF = (torch.float16, torch.int16)
 
-
-def _torch():
-    import torch
-
-    return torch
+# A serving step makes hundreds of these calls, each a few microseconds of device work: the checks below are plain
+# comparisons, messages are formed only when one fails, and workspace sizes are remembered by the sizes they follow from.
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _place(first, *others) -> tuple:
+    """(device, stream handle) for tensors that have to be on the current device; raises ValueError otherwise."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    if dev < 0:
+        raise ValueError(f"tensors on {first.device}, not on the GPU")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on {first.device}, the current device is {torch.cuda.current_device()}")
+    return first.device, torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _on_device(**tensors) -> None:
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} is on {t.device}, not on the GPU")
-        if dev is None:
-            dev = _torch().cuda.current_device()
-        if t.get_device() != dev:
-            raise ValueError(f"{name} is on {t.device}, the current device is {dev}")
-
-
-def _run(rc: int, what: str) -> None:
+def _fail(what: str, rc: int):
     """These calls have no path of the caller's to fall back to: a decline is an error too."""
-    if rc != OK:
-        raise LoomHipError(f"{what}: {last_error()} (rc={rc})")
+    raise LoomHipError(f"{what}: {last_error()} (rc={rc})")
 
 
-def _ws(n: int, like):
-    """A workspace of n bytes from torch's allocator, or None."""
-    return _torch().empty(n, dtype=_torch().uint8, device=like.device) if n else None
+@functools.lru_cache(maxsize=4096)
+def _attn_ws(*sizes) -> int:
+    return lib().loomhip_prefix_attn_ws(*sizes)
 
 
-def _p(t):
-    return None if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=4096)
+def _lora_ws(n: int, t: int, *sizes) -> int:
+    return lib().loomhip_lora_ws(C.byref(LoraDesc(t, *sizes)), n)
+
+
+@functools.lru_cache(maxsize=4096)
+def _probs_ws(n: int, vocab: int) -> int:
+    return lib().loomhip_token_probs_ws(n, vocab)
+
+
+@functools.lru_cache(maxsize=4096)
+def _verify_ws(n: int, vocab: int) -> int:
+    return lib().loomhip_verify_drafts_ws(n, vocab)
+
+
+_NO_ROWS = KvRowsDesc()
 
 
 def _kv_desc(k, v, lanes: bool, name: str):
-    torch = _torch()
-    want = 4 if lanes else 3
-    _need(k.dim() == want and k.shape == v.shape and (k.stride() == v.stride() or k.numel() == 0),
-          f"{name}: keys and values of one shape and layout, [{'n, ' if lanes else ''}rows, n_kv_heads, head_dim]")
-    _need(k.dtype == v.dtype and k.dtype in (torch.float16, torch.int16), f"{name}: fp16 rows (or their bits as int16)")
-    if k.numel() == 0:
-        return KvRowsDesc()
-    _need(k.stride(-1) == 1 or k.shape[-1] == 1, f"{name}: the values of a head one after the other")
-    return KvRowsDesc(k.data_ptr(), v.data_ptr(), k.shape[-3], k.stride(0) if lanes else 0, k.stride(-3), k.stride(-2))
+    shape, stride = k.shape, k.stride()
+    if (len(shape) != 3 + lanes or v.shape != shape or k.dtype not in _HALF or v.dtype != k.dtype):
+        raise ValueError(f"{name}: keys and values of one shape, [{'n, ' if lanes else ''}rows, n_kv_heads, head_dim], fp16 "
+                         "(or its bits as int16)")
+    if 0 in shape:
+        return _NO_ROWS
+    if v.stride() != stride or (stride[-1] != 1 and shape[-1] != 1):
+        raise ValueError(f"{name}: keys and values of one layout, the values of a head one after the other")
+    return KvRowsDesc(k.data_ptr(), v.data_ptr(), shape[-3], stride[0] if lanes else 0, stride[-3], stride[-2])
 
 
 def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, q_len=None, out=None):
@@ -84,34 +93,49 @@ def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, 
     multiples of 8, a ``Decoder``'s at one layer among them.  Returns out f32 as q; rows past q_len[i] keep what an
     ``out`` given holds, and are zero in one made here.
     """
-    torch = _torch()
-    _need(q.dim() == 4 and q.dtype == torch.float32 and q.is_contiguous(), "q: contiguous f32 [n, n_q, n_heads, head_dim]")
-    n, n_q, heads, hd = q.shape
-    pre, own = KvRowsDesc(), KvRowsDesc()
+    shape = q.shape
+    if len(shape) != 4 or q.dtype is not _F32 or not q.is_contiguous():
+        raise ValueError("q: contiguous f32 [n, n_q, n_heads, head_dim]")
+    n, n_q, heads, hd = shape
+    pre = own = _NO_ROWS
     kv = None
     if k_prefix is not None:
         pre = _kv_desc(k_prefix, v_prefix, False, "prefix")
-        kv = k_prefix.shape[-2]
-        _need(k_prefix.shape[-1] == hd, "prefix: another head size than q's")
+        kv = k_prefix.shape[1]
+        if k_prefix.shape[2] != hd:
+            raise ValueError("prefix: another head size than q's")
     if k_own is not None:
         own = _kv_desc(k_own, v_own, True, "own")
-        _need(k_own.shape[0] == n and k_own.shape[-1] == hd and kv in (None, k_own.shape[-2]),
-              "own: lanes and head size as q's, key heads as the prefix's")
-        _need(own_len is not None, "own rows without own_len")
-        kv = k_own.shape[-2]
-    _need(kv is not None, "neither a prefix nor own rows")
-    for name, t in (("own_len", own_len), ("q_len", q_len)):
-        _need(t is None or (t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous()), f"{name}: int32 [n]")
+        s = k_own.shape
+        if s[0] != n or s[3] != hd or (kv is not None and s[2] != kv):
+            raise ValueError("own: lanes and head size as q's, key heads as the prefix's")
+        kv = s[2]
+        if own_len is None:
+            raise ValueError("own rows without own_len")
+    elif k_prefix is None:
+        raise ValueError("neither a prefix nor own rows")
+    for t in (own_len, q_len):
+        if t is not None and (t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError("own_len, q_len: int32 [n]")
+    dev, stream = _place(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, out)
     if out is None:
         out = torch.empty_like(q) if q_len is None else torch.zeros_like(q)
-    _need(out.shape == q.shape and out.dtype == torch.float32 and out.is_contiguous(), "out: as q")
-    _on_device(q=q, k_prefix=k_prefix, v_prefix=v_prefix, k_own=k_own, v_own=v_own, own_len=own_len, q_len=q_len, out=out)
-    L = lib()
-    ws = L.loomhip_prefix_attn_ws(pre.rows, own.rows, n, n_q, heads, kv, hd)
-    w = _ws(ws, q)
-    _run(L.loomhip_prefix_attn_dev(C.byref(pre), C.byref(own), _p(q), _p(own_len), _p(q_len), n, n_q, heads, kv, hd,
-                                   scale, _p(out), _p(w), ws, _stream()), "prefix_attn_dev")
+    elif out.shape != shape or out.dtype is not _F32 or not out.is_contiguous():
+        raise ValueError("out: as q")
+    nb = _attn_ws(pre.rows, own.rows, n, n_q, heads, kv, hd)
+    ws = torch.empty(nb, dtype=_U8, device=dev)
+    rc = lib().loomhip_prefix_attn_dev(
+        C.byref(pre), C.byref(own), q.data_ptr(), None if own_len is None else own_len.data_ptr(),
+        None if q_len is None else q_len.data_ptr(), n, n_q, heads, kv, hd, scale, out.data_ptr(), ws.data_ptr(), nb, stream)
+    if rc != OK:
+        _fail("prefix_attn_dev", rc)
     return out
+
+
+def _rows_ok(t, n: int, width: int) -> bool:
+    """f32 [n, width] whose rows are consecutive values and do not overlap."""
+    return (t.shape == (n, width) and t.dtype is _F32 and (t.is_contiguous() or (
+        (width == 1 or t.stride(1) == 1) and (n == 1 or t.stride(0) >= width))))
 
 
 def lora_dev(x, a, b, scale, ids, base=None, out=None):
@@ -121,54 +145,65 @@ def lora_dev(x, a, b, scale, ids, base=None, out=None):
     [adapters], ids int32 [n], base f32 [n, rows] or None (zeros).  ``out=base`` adds in place, as beside
     ``matvec_dev``'s output.  Rows of x, base and out may be strided.  Returns out.
     """
-    torch = _torch()
-    if not _LORA_TYPES:
-        _LORA_TYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
-    _need(x.dim() == 2 and x.dtype == torch.float32, "x: f32 [n, cols]")
-    _need(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.dtype in _LORA_TYPES and a.is_contiguous()
-          and b.is_contiguous(), "a, b: contiguous, of one type (f32, fp16 or bf16)")
+    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
+        raise ValueError("x [n, cols], a [adapters, rank, cols], b [adapters, rows, rank]")
     n, cols = x.shape
-    adapters, rank = a.shape[:2]
+    adapters, rank, ac = a.shape
     rows = b.shape[1]
-    _need(a.shape[2] == cols and b.shape[0] == adapters and b.shape[2] == rank,
-          "a [adapters, rank, cols], b [adapters, rows, rank]")
-    _need(scale.shape == (adapters,) and scale.dtype == torch.float32 and scale.is_contiguous(), "scale: f32 [adapters]")
-    _need(ids.shape == (n,) and ids.dtype == torch.int32 and ids.is_contiguous(), "ids: int32 [n]")
+    kind = _LORA_TYPES.get(a.dtype)
+    if kind is None or b.dtype != a.dtype or not a.is_contiguous() or not b.is_contiguous():
+        raise ValueError("a, b: contiguous, of one type (f32, fp16 or bf16)")
+    if ac != cols or b.shape[0] != adapters or b.shape[2] != rank:
+        raise ValueError("a [adapters, rank, cols], b [adapters, rows, rank]")
+    if scale.shape != (adapters,) or scale.dtype is not _F32 or not scale.is_contiguous():
+        raise ValueError("scale: f32 [adapters]")
+    if ids.shape != (n,) or ids.dtype is not _I32 or not ids.is_contiguous():
+        raise ValueError("ids: int32 [n]")
+    dev, stream = _place(x, a, b, scale, ids, base, out)
     if out is None:
-        out = torch.empty((n, rows), dtype=torch.float32, device=x.device)
-    for name, t, w in (("x", x, cols), ("base", base, rows), ("out", out, rows)):
-        _need(t is None or (t.shape == (n, w) and t.dtype == torch.float32 and (w == 1 or t.stride(1) == 1)
-                            and (n == 1 or t.stride(0) >= w)), f"{name}: f32 [{n}, {w}], rows of consecutive values")
-    _on_device(x=x, a=a, b=b, scale=scale, ids=ids, base=base, out=out)
-    L = lib()
-    d = LoraDesc(_LORA_TYPES[a.dtype], adapters, rank, rows, cols, a.data_ptr(), b.data_ptr(), scale.data_ptr())
-    ws = L.loomhip_lora_ws(C.byref(d), n)
-    w = _ws(ws, x)
-    _run(L.loomhip_lora_dev(C.byref(d), _p(x), max(x.stride(0), cols), _p(ids), _p(base),
-                            max(base.stride(0), rows) if base is not None else rows, n, _p(out),
-                            max(out.stride(0), rows), _p(w), ws, _stream()), "lora_dev")
+        out = torch.empty((n, rows), dtype=_F32, device=dev)
+    if not _rows_ok(x, n, cols) or not _rows_ok(out, n, rows) or not (base is None or _rows_ok(base, n, rows)):
+        raise ValueError("x [n, cols], base and out [n, rows]: f32, rows of consecutive values")
+    nb = _lora_ws(n, kind, adapters, rank, rows, cols)
+    ws = torch.empty(nb, dtype=_U8, device=dev)
+    d = LoraDesc(kind, adapters, rank, rows, cols, a.data_ptr(), b.data_ptr(), scale.data_ptr())
+    rc = lib().loomhip_lora_dev(
+        C.byref(d), x.data_ptr(), x.stride(0) if n > 1 else cols, ids.data_ptr(), None if base is None else base.data_ptr(),
+        base.stride(0) if base is not None and n > 1 else rows, n, out.data_ptr(), out.stride(0) if n > 1 else rows,
+        ws.data_ptr(), nb, stream)
+    if rc != OK:
+        _fail("lora_dev", rc)
     return out
 
 
 def token_probs_dev(logits, temperature=None, out=None):
     """softmax(logits / temperature) of every row: logits f32 [..., vocab] contiguous, temperature f32 of the leading
     shape (None: 1; not positive: 1 at the first maximum).  ``out=logits`` works in place.  Returns out."""
-    torch = _torch()
-    _need(logits.dim() >= 1 and logits.dtype == torch.float32 and logits.is_contiguous(), "logits: contiguous f32")
-    vocab = logits.shape[-1]
+    shape = logits.shape
+    if not shape or logits.dtype is not _F32 or not logits.is_contiguous():
+        raise ValueError("logits: contiguous f32")
+    vocab = shape[-1]
     n = logits.numel() // vocab if vocab else 0
-    _need(temperature is None or (temperature.dtype == torch.float32 and temperature.shape == logits.shape[:-1]
-                                  and temperature.is_contiguous()), "temperature: f32, one a row")
+    if temperature is not None and (temperature.dtype is not _F32 or temperature.shape != shape[:-1]
+                                    or not temperature.is_contiguous()):
+        raise ValueError("temperature: f32, one a row")
+    dev, stream = _place(logits, temperature, out)
     if out is None:
         out = torch.empty_like(logits)
-    _need(out.shape == logits.shape and out.dtype == torch.float32 and out.is_contiguous(), "out: as logits")
-    _on_device(logits=logits, temperature=temperature, out=out)
-    L = lib()
-    ws = L.loomhip_token_probs_ws(n, vocab)
-    w = _ws(ws, logits)
-    _run(L.loomhip_token_probs_dev(_p(logits), n, vocab, vocab, _p(temperature), _p(out), vocab, _p(w), ws, _stream()),
-         "token_probs_dev")
+    elif out.shape != shape or out.dtype is not _F32 or not out.is_contiguous():
+        raise ValueError("out: as logits")
+    nb = _probs_ws(n, vocab)
+    ws = torch.empty(nb, dtype=_U8, device=dev)
+    rc = lib().loomhip_token_probs_dev(logits.data_ptr(), n, vocab, vocab,
+                                       None if temperature is None else temperature.data_ptr(), out.data_ptr(), vocab,
+                                       ws.data_ptr(), nb, stream)
+    if rc != OK:
+        _fail("token_probs_dev", rc)
     return out
+
+
+def _is(t, dtype, *shape) -> bool:
+    return t.shape == shape and t.dtype is dtype and t.is_contiguous()
 
 
 def verify_drafts_dev(target_probs, draft_tokens, u_accept, u_sample, draft_probs=None, n_draft=None):
@@ -178,27 +213,26 @@ def verify_drafts_dev(target_probs, draft_tokens, u_accept, u_sample, draft_prob
     f32 [n, k, vocab] (None: a drafter that names one token), n_draft int32 [n] (None: k each).  Returns (tokens int32
     [n, k + 1]: the accepted ones, the next one, then -1; accepted int32 [n]).
     """
-    torch = _torch()
-    _need(target_probs.dim() == 3 and target_probs.shape[1] >= 1, "target_probs: f32 [n, k + 1, vocab]")
+    if target_probs.dim() != 3 or target_probs.shape[1] < 1:
+        raise ValueError("target_probs: f32 [n, k + 1, vocab]")
     n, k1, vocab = target_probs.shape
     k = k1 - 1
-    for name, t, shape, dt in (("target_probs", target_probs, (n, k1, vocab), torch.float32),
-                               ("draft_tokens", draft_tokens, (n, k), torch.int32),
-                               ("u_accept", u_accept, (n, k), torch.float32), ("u_sample", u_sample, (n,), torch.float32),
-                               ("draft_probs", draft_probs, (n, k, vocab), torch.float32),
-                               ("n_draft", n_draft, (n,), torch.int32)):
-        _need(t is None or (t.shape == shape and t.dtype == dt and t.is_contiguous()),
-              f"{name}: contiguous {str(dt)[6:]} {list(shape)}")
-    _on_device(target_probs=target_probs, draft_tokens=draft_tokens, u_accept=u_accept, u_sample=u_sample,
-               draft_probs=draft_probs, n_draft=n_draft)
-    tokens = torch.empty((n, k1), dtype=torch.int32, device=target_probs.device)
-    accepted = torch.empty((n,), dtype=torch.int32, device=target_probs.device)
-    L = lib()
-    ws = L.loomhip_verify_drafts_ws(n, vocab)
-    w = _ws(ws, target_probs)
-    _run(L.loomhip_verify_drafts_dev(_p(target_probs), _p(draft_probs), _p(draft_tokens), _p(n_draft), _p(u_accept),
-                                     _p(u_sample), n, k, vocab, _p(tokens), _p(accepted), _p(w), ws, _stream()),
-         "verify_drafts_dev")
+    if not (_is(target_probs, _F32, n, k1, vocab) and _is(draft_tokens, _I32, n, k) and _is(u_accept, _F32, n, k)
+            and _is(u_sample, _F32, n) and (draft_probs is None or _is(draft_probs, _F32, n, k, vocab))
+            and (n_draft is None or _is(n_draft, _I32, n))):
+        raise ValueError(f"contiguous target_probs f32 [{n}, {k1}, {vocab}], draft_tokens int32 [{n}, {k}], u_accept f32 "
+                         f"[{n}, {k}], u_sample f32 [{n}], draft_probs f32 [{n}, {k}, {vocab}], n_draft int32 [{n}]")
+    dev, stream = _place(target_probs, draft_tokens, u_accept, u_sample, draft_probs, n_draft)
+    tokens = torch.empty((n, k1), dtype=_I32, device=dev)
+    accepted = torch.empty((n,), dtype=_I32, device=dev)
+    nb = _verify_ws(n, vocab)
+    ws = torch.empty(nb, dtype=_U8, device=dev)
+    rc = lib().loomhip_verify_drafts_dev(
+        target_probs.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), draft_tokens.data_ptr(),
+        None if n_draft is None else n_draft.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), n, k, vocab,
+        tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nb, stream)
+    if rc != OK:
+        _fail("verify_drafts_dev", rc)
     return tokens, accepted
 
 

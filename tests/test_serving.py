@@ -41,6 +41,11 @@ def _attn(prefix=None, own=None, q=FAKE, own_len=FAKE, q_len=None, n=2, n_q=1, h
     (loom_amd.DECLINED, dict(prefix=(FAKE, FAKE, 1 << 40, 0, 128, 64))),
     (loom_amd.DECLINED, dict(n=1 << 20)),
     (loom_amd.DECLINED, dict(n_q=1 << 20)),
+    (loom_amd.ERR_ARG, dict(ws=None)),
+    (loom_amd.ERR_ARG, dict(ws=FAKE + 8)),
+    (loom_amd.ERR_ARG, dict(ws_bytes=2 * 4 * (64 * 4 + 8))),
+    (loom_amd.DECLINED, dict(prefix=(FAKE, FAKE, 16, 0, 1 << 24, 64))),
+    (loom_amd.DECLINED, dict(own=(FAKE, FAKE, 8, 1 << 30, 1 << 24, 64))),
 ])
 def test_prefix_attn_refuses(rc, args):
     assert _attn(**args) == rc
@@ -57,9 +62,9 @@ def test_nothing_to_do_is_ok():
 
 
 def _lora(type=loom_amd.F16, adapters=2, rank=8, rows=64, cols=32, a=FAKE, b=FAKE, scale=FAKE, x=0x100000, xs=32, ids=FAKE,
-          base=None, bs=64, n=4, out=0x200000, os=64):
+          base=None, bs=64, n=4, out=0x200000, os=64, ws=FAKE, ws_bytes=1 << 40):
     d = loom_amd.LoraDesc(type, adapters, rank, rows, cols, a, b, scale)
-    return loom_amd.lib().loomhip_lora_dev(C.byref(d), x, xs, ids, base, bs, n, out, os, FAKE, 1 << 40, None)
+    return loom_amd.lib().loomhip_lora_dev(C.byref(d), x, xs, ids, base, bs, n, out, os, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("rc,args", [
@@ -79,6 +84,10 @@ def _lora(type=loom_amd.F16, adapters=2, rank=8, rows=64, cols=32, a=FAKE, b=FAK
     (loom_amd.ERR_ARG, dict(base=0x300000, bs=63)),
     (loom_amd.ERR_ARG, dict(a=FAKE + 1)),
     (loom_amd.ERR_ARG, dict(x=0x100002)),
+    (loom_amd.ERR_ARG, dict(ws=None)),
+    (loom_amd.ERR_ARG, dict(ws=FAKE + 8)),
+    (loom_amd.ERR_ARG, dict(ws_bytes=255)),
+    (loom_amd.DECLINED, dict(n=65535 * 64 + 1)),
     (loom_amd.ERR_ARG, dict(out=0x100000)),               # over x
     (loom_amd.ERR_ARG, dict(out=0x100000 - 4)),           # into x
     (loom_amd.ERR_ARG, dict(base=0x200004)),              # over base, shifted
