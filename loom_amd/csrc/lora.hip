@@ -592,7 +592,7 @@ using namespace lh;
 extern "C" {
 
 size_t loomhip_lora_ws(const loomhip_lora *l, size_t n) {
-    return l && l->rank && l->rank <= LORA_MAX_RANK && l->cols && l->rows && n <= LORA_MAX_N ? lora_ws_bytes(l, n) : 0;
+    return l && n && n <= LORA_MAX_N && l->rank && l->rank <= LORA_MAX_RANK && l->cols && l->rows ? lora_ws_bytes(l, n) : 0;
 }
 
 int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, const int32_t *ids, const float *base,

@@ -152,6 +152,18 @@ def test_without_a_device_the_calls_say_so():
 def test_workspaces_grow_with_the_call():
     L = loom_amd.lib()
     assert L.loomhip_token_probs_ws(0, 100) == 0 and L.loomhip_verify_drafts_ws(0, 100) == 0
+    assert L.loomhip_token_probs_ws(5, 0) == 0 and L.loomhip_verify_drafts_ws(5, 0) == 0
+    d = loom_amd.LoraDesc(loom_amd.F16, 1, 8, 64, 64, FAKE, FAKE, FAKE)
+    assert L.loomhip_lora_ws(C.byref(d), 0) == 0 and L.loomhip_lora_ws(None, 4) == 0
+    assert 0 < L.loomhip_lora_ws(C.byref(d), 1) <= L.loomhip_lora_ws(C.byref(d), 1000)
+    for bad in (loom_amd.LoraDesc(loom_amd.F16, 1, 0, 64, 64), loom_amd.LoraDesc(loom_amd.F16, 1, 8, 0, 64),
+                loom_amd.LoraDesc(loom_amd.F16, 1, 8, 64, 0), loom_amd.LoraDesc(loom_amd.F16, 1, 257, 64, 64)):
+        assert L.loomhip_lora_ws(C.byref(bad), 4) == 0
+    assert L.loomhip_prefix_attn_ws(100, 10, 0, 1, 8, 2, 64) == 0
+    assert L.loomhip_prefix_attn_ws(100, 10, 2, 0, 8, 2, 64) == 0
+    assert L.loomhip_prefix_attn_ws(100, 10, 2, 1, 8, 0, 64) == 0
+    assert L.loomhip_prefix_attn_ws(0, 0, 2, 1, 8, 2, 64) == 0
+    assert L.loomhip_prefix_attn_ws(100, 10, 2, 1, 8, 2, 64) >= 2 * 8 * 64 * 4 * 2
     for n, vocab in ((1, 1), (1, 32000), (64, 151936), (65535, 7)):
         assert L.loomhip_token_probs_ws(n, vocab) >= 16 * n
         assert L.loomhip_verify_drafts_ws(n, vocab) >= 16 * n
