@@ -3,24 +3,43 @@
 // against the target's probabilities from given random numbers.
 #include "runtime.hpp"
 
+#include <type_traits>
+
 namespace lh {
 
-// The work groups a row of `vocab` values is split over: enough that the
-// whole launch fills the chip, no more than SPLIT_MAX, none with less than
-// SPLIT_MIN values.
 constexpr int SMP_THREADS = 256;
-constexpr int SPLIT_MAX = 64;
-constexpr size_t SPLIT_MIN = 2048;
-constexpr size_t SPLIT_GROUPS = 1024;
+typedef float smp_f4 __attribute__((ext_vector_type(4)));
 
-static int row_splits(size_t rows, size_t vocab) {
-    size_t s = (SPLIT_GROUPS + rows - 1) / rows;
-    const size_t most = (vocab + SPLIT_MIN - 1) / SPLIT_MIN;
-    s = s > most ? most : s;
-    return (int)(s > SPLIT_MAX ? SPLIT_MAX : s < 1 ? 1 : s);
+// How a row of `vocab` values is cut: work groups of NV * 1024 values, a thread NV times four, all of them loaded before
+// the first is used.  Enough work groups to fill the chip four times over, none with fewer than 2048 values; up to
+// 16384 (64 registers a thread).
+struct RowCut {
+    int splits, nv; // nv 2, 4, 8 or 16
+};
+static RowCut row_cut(size_t rows, size_t vocab, size_t groups = 1024) {
+    const size_t want = (groups + rows - 1) / rows;
+    int nv = 2;
+    while (nv < 16 && (vocab + nv * 1024 - 1) / (nv * 1024) > want)
+        nv *= 2;
+    return {(int)((vocab + nv * 1024 - 1) / (nv * 1024)), nv};
 }
-// Values per split, a multiple of 4 so that splits of aligned rows start aligned.
-static size_t split_len(size_t vocab, int splits) { return ((vocab + splits - 1) / splits + 3) / 4 * 4; }
+
+// The values of a work group's part of a row that its thread holds: four at (i * 256 + tid) * 4 of the part, `fill` past
+// the row's end.  VEC: rows at multiples of 16 bytes, their lengths a multiple of 4.
+template <int NV, bool VEC>
+__device__ __forceinline__ void row_part(const float *x, size_t v0, size_t vocab, float fill, smp_f4 (&v)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const size_t at = v0 + ((size_t)i * SMP_THREADS + threadIdx.x) * 4;
+        if constexpr (VEC) {
+            v[i] = at < vocab ? *(const smp_f4 *)(x + at) : smp_f4{fill, fill, fill, fill};
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                v[i][c] = at + c < vocab ? x[at + c] : fill;
+        }
+    }
+}
 
 // ---- token probabilities -------------------------------------------------------
 // p_v = exp((x_v - m) / T) / sum_w exp((x_w - m) / T), m = max x.  Two launches:
@@ -62,20 +81,26 @@ __device__ __forceinline__ void max_first(float &m, int &at, float m2, int at2) 
     at = take ? at2 : at;
 }
 
+template <int NV, bool VEC>
 __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *__restrict__ logits, size_t vocab,
                                                                    size_t stride, const float *__restrict__ temperature,
-                                                                   size_t len, ProbRec *__restrict__ rec) {
+                                                                   int splits, ProbRec *__restrict__ rec) {
     __shared__ float sm[SMP_THREADS / 64], sl[SMP_THREADS / 64];
     __shared__ int sa[SMP_THREADS / 64];
-    const size_t row = blockIdx.y;
-    const float *x = logits + row * stride;
-    const size_t v0 = blockIdx.x * len, v1 = v0 + len < vocab ? v0 + len : vocab;
-    const ProbScale sc = prob_scale(temperature, row);
+    const size_t row = blockIdx.x / splits;
+    const int split = blockIdx.x % splits;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t v0 = (size_t)split * (NV * SMP_THREADS * 4);
+    smp_f4 v[NV];
+    row_part<NV, VEC>(logits + row * stride, v0, vocab, -__builtin_inff(), v);
+    const ProbScale sc = prob_scale(temperature, row);
     float m = -__builtin_inff();
     int at = 0x7fffffff;
-    for (size_t v = v0 + tid; v < v1; v += SMP_THREADS)
-        max_first(m, at, x[v], (int)v);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            max_first(m, at, v[i][c], (int)(v0 + ((size_t)i * SMP_THREADS + tid) * 4 + c));
     for (int o = 1; o < 64; o *= 2)
         max_first(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
     if (lane == 0)
@@ -86,8 +111,11 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *
         max_first(m, at, sm[w], sa[w]);
     float l = 0.0f;
     if (m != -__builtin_inff())
-        for (size_t v = v0 + tid; v < v1; v += SMP_THREADS)
-            l += exp_scaled(x[v] - m, sc.hi, sc.lo);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                l += exp_scaled(v[i][c] - m, sc.hi, sc.lo);
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
     if (lane == 0)
@@ -96,39 +124,59 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *
     if (tid == 0) {
         for (int w = 1; w < SMP_THREADS / 64; w++)
             l += sl[w];
-        rec[row * gridDim.x + blockIdx.x] = {m, l, at, 0};
+        rec[blockIdx.x] = {m, l, at, 0};
     }
 }
 
+template <int NV, bool VEC>
 __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *__restrict__ logits, size_t vocab,
                                                                   size_t stride, const float *__restrict__ temperature,
-                                                                  size_t len, const ProbRec *__restrict__ rec,
+                                                                  int splits, const ProbRec *__restrict__ rec,
                                                                   float *__restrict__ probs, size_t out_stride) {
-    const size_t row = blockIdx.y;
-    const float *x = logits + row * stride;
+    // The parts in the reduction's order backwards, eight at a time: a part stays with its XCD, and those read last
+    // may still be in its L2.
+    const int item = (int)((gridDim.x - 1 - blockIdx.x) & ~7u) + (int)(blockIdx.x & 7);
+    const int b = gridDim.x % 8 ? (int)(gridDim.x - 1 - blockIdx.x) : item;
+    const size_t row = b / splits;
+    const int split = b % splits, tid = threadIdx.x, lane = tid & 63;
+    const size_t v0 = (size_t)split * (NV * SMP_THREADS * 4);
+    smp_f4 v[NV];
+    row_part<NV, VEC>(logits + row * stride, v0, vocab, -__builtin_inff(), v);
     float *p = probs + row * out_stride;
-    const size_t v0 = blockIdx.x * len, v1 = v0 + len < vocab ? v0 + len : vocab;
     const ProbScale sc = prob_scale(temperature, row);
-    const int tid = threadIdx.x, lane = tid & 63, splits = gridDim.x;
-    ProbRec r = {-__builtin_inff(), 0.0f, 0x7fffffff, 0};
-    if (lane < splits)
-        r = rec[row * splits + lane];
-    float m = r.m;
-    int at = r.at;
+    float m = -__builtin_inff();
+    int at = 0x7fffffff;
+    for (int s = lane; s < splits; s += 64)
+        max_first(m, at, rec[row * splits + s].m, rec[row * splits + s].at);
     for (int o = 1; o < 64; o *= 2)
         max_first(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
-    if (sc.greedy) {
-        for (size_t v = v0 + tid; v < v1; v += SMP_THREADS)
-            p[v] = v == (size_t)at ? 1.0f : 0.0f;
-        return;
+    float l = 0.0f;
+    for (int s = lane; s < splits; s += 64) {
+        const ProbRec r = rec[row * splits + s];
+        l += r.m == -__builtin_inff() ? 0.0f : r.l * exp_scaled(r.m - m, sc.hi, sc.lo);
     }
-    float l = r.m == -__builtin_inff() ? 0.0f : r.l * exp_scaled(r.m - m, sc.hi, sc.lo);
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
     const float inv = 1.0f / l;
     const bool none = m == -__builtin_inff(); // every logit is -inf: no token has a probability
-    for (size_t v = v0 + tid; v < v1; v += SMP_THREADS)
-        p[v] = none ? 0.0f : exp_scaled(x[v] - m, sc.hi, sc.lo) * inv;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const size_t k = v0 + ((size_t)i * SMP_THREADS + tid) * 4;
+        smp_f4 e;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            e[c] = sc.greedy ? (k + c == (size_t)at ? 1.0f : 0.0f)
+                             : none ? 0.0f : exp_scaled(v[i][c] - m, sc.hi, sc.lo) * inv;
+        if constexpr (VEC) {
+            if (k < vocab)
+                __builtin_nontemporal_store(e, (smp_f4 *)(p + k));
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (k + c < vocab)
+                    p[k + c] = e[c];
+        }
+    }
 }
 
 // ---- verification of drafted tokens ----------------------------------------------
@@ -137,15 +185,14 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *_
 // max(p_r - q_r, 0), after none from p_nd, by the inverse of the running sum
 // at a given number u: the lowest v with c_v > u * c_last.  The products and
 // the sums are in 64 bits: they decide a whole number.  Two launches: each
-// (lane, split) finds r and sums its values; then one work group per lane
-// scans the split sums and the one split that holds the token.
+// (lane, part of the row) finds r and sums its values; then one work group per
+// lane scans the parts' sums and the one part that holds the token.
 struct VerifyParams {
     const float *target, *draft; // [n][k+1][vocab], [n][k][vocab] or null
     const int32_t *tok, *n_draft;
     const float *u_accept, *u_sample;
     size_t n, k, vocab;
-    size_t len;
-    int splits;
+    int splits;   // parts of a row
     double *sums; // [n][splits][2]: of max(p - q, 0) and of p
     int32_t *out; // [n][k+1]
     int32_t *accepted;
@@ -199,9 +246,10 @@ __device__ __forceinline__ VerifyRow verify_row(const VerifyParams &P, size_t i,
     }
     return r;
 }
-__device__ __forceinline__ double residual(const VerifyRow &r, size_t v, float p) {
+// What is left of p (as_prob) at v, q the drafter's value there.
+__device__ __forceinline__ double residual(const VerifyRow &r, size_t v, float p, float q) {
     if (r.q) {
-        const double d = (double)p - (double)as_prob(r.q[v]);
+        const double d = (double)p - (double)as_prob(q);
         return d > 0.0 ? d : 0.0;
     }
     return (int64_t)v == r.out ? 0.0 : (double)p;
@@ -213,18 +261,34 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return v;
 }
 
+// Two rows are in registers here and the last step goes through one part alone: parts of 2048 or 4096 values, larger
+// ones only where a row would have over 1024 of them.
+static RowCut verify_cut(size_t n, size_t vocab) {
+    const RowCut c = row_cut(n, vocab, 2048);
+    const int nv = c.nv > 4 && (vocab + 4095) / 4096 <= 1024 ? 4 : c.nv;
+    return {(int)((vocab + nv * 1024 - 1) / (nv * 1024)), nv};
+}
+
+template <int NV, bool VEC>
 __global__ __launch_bounds__(SMP_THREADS) void verify_sum_kernel(VerifyParams P) {
     __shared__ double sd[SMP_THREADS / 64], sp[SMP_THREADS / 64];
     const size_t i = blockIdx.y;
     const int nd = verify_nd(P, i), acc = verify_accepted(P, i, nd);
     const VerifyRow r = verify_row(P, i, nd, acc);
-    const size_t v0 = blockIdx.x * P.len, v1 = v0 + P.len < P.vocab ? v0 + P.len : P.vocab;
+    const size_t v0 = (size_t)blockIdx.x * (NV * SMP_THREADS * 4);
+    smp_f4 p[NV], q[NV];
+    row_part<NV, VEC>(r.p, v0, P.vocab, 0.0f, p);
+    if (r.q)
+        row_part<NV, VEC>(r.q, v0, P.vocab, 0.0f, q);
     double d = 0.0, all = 0.0;
-    for (size_t v = v0 + threadIdx.x; v < v1; v += SMP_THREADS) {
-        const float p = as_prob(r.p[v]);
-        d += residual(r, v, p);
-        all += (double)p;
-    }
+#pragma unroll
+    for (int x = 0; x < NV; x++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float pv = as_prob(p[x][c]);
+            d += residual(r, v0 + ((size_t)x * SMP_THREADS + threadIdx.x) * 4 + c, pv, r.q ? q[x][c] : 0.0f);
+            all += (double)pv;
+        }
     d = wave_sum_f64(d);
     all = wave_sum_f64(all);
     if ((threadIdx.x & 63) == 0)
@@ -235,35 +299,51 @@ __global__ __launch_bounds__(SMP_THREADS) void verify_sum_kernel(VerifyParams P)
             d += sd[w], all += sp[w];
         double *o = P.sums + (i * P.splits + blockIdx.x) * 2;
         o[0] = d, o[1] = all;
+        if (blockIdx.x == 0)
+            P.accepted[i] = acc;
     }
 }
 
-__global__ __launch_bounds__(SMP_THREADS) void verify_pick_kernel(VerifyParams P) {
-    constexpr int W = SMP_THREADS / 64;
-    __shared__ double sw[W];
-    __shared__ int s_found[W], s_last[W];
-    const size_t i = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int nd = verify_nd(P, i), acc = verify_accepted(P, i, nd);
-    VerifyRow r = verify_row(P, i, nd, acc);
-    // the running sum at each split's end (splits <= 64: a lane each)
-    const double *s = P.sums + i * P.splits * 2;
-    double d = lane < P.splits ? s[2 * lane] : 0.0;
-    if (!(wave_sum_f64(d) > 0.0)) { // p nowhere above q: the target's own row
-        d = lane < P.splits ? s[2 * lane + 1] : 0.0;
-        r.q = nullptr;
-        r.out = -1;
-    }
+// A lane's running sums of d over the wave, and the wave's sum.
+__device__ __forceinline__ double wave_scan_f64(double d, double *sum) {
+    const int lane = threadIdx.x & 63;
     double c = d;
     for (int o = 1; o < 64; o *= 2) {
         const double up = __shfl_up(c, o);
         c += lane >= o ? up : 0.0;
     }
-    const double total = __shfl(c, 63);
+    *sum = __shfl(c, 63);
+    return c;
+}
+
+// The part that holds the token, then of its 256 threads' runs of NV * 4 values (one after the other here) the one that
+// does, then the value.  At each step the first whose running sum passes `at` and that has anything in it, else the last
+// that has.
+template <int NV, bool VEC>
+__global__ __launch_bounds__(SMP_THREADS) void verify_pick_kernel(VerifyParams P) {
+    constexpr int W = SMP_THREADS / 64, E = NV * 4;
+    __shared__ double sw[W], before[SMP_THREADS];
+    __shared__ int s_hit[W], s_last[W];
+    const size_t i = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nd = verify_nd(P, i), acc = P.accepted[i];
+    VerifyRow r = verify_row(P, i, nd, acc);
+    const double *s = P.sums + i * P.splits * 2;
+    double left = 0.0, total = 0.0;
+    for (int b = lane; b < P.splits; b += 64)
+        left += s[2 * b], total += s[2 * b + 1];
+    left = wave_sum_f64(left);
+    int which = 0;
+    if (left > 0.0) {
+        total = left;
+    } else { // p nowhere above q: the target's own row
+        total = wave_sum_f64(total);
+        which = 1;
+        r.q = nullptr;
+        r.out = -1;
+    }
     const double at = fmax((double)P.u_sample[i] * total, 0.0); // NaN: 0
     int32_t *out = P.out + i * (P.k + 1);
-    if (tid == 0)
-        P.accepted[i] = acc;
     for (int j = tid; j <= (int)P.k; j += SMP_THREADS)
         if (j != acc)
             out[j] = j < acc ? P.tok[i * P.k + j] : -1;
@@ -272,54 +352,92 @@ __global__ __launch_bounds__(SMP_THREADS) void verify_pick_kernel(VerifyParams P
             out[acc] = -1;
         return;
     }
-    // the split that holds the token: the first whose end passes `at`, else the last with anything in it
-    const unsigned long long past = __ballot(c > at && d > 0.0), some = __ballot(d > 0.0);
-    const int sp = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-    double run = __shfl(c, sp) - __shfl(d, sp); // what comes before the split
-    if (sp > 0) // the same sum that the split before it ends with
-        run = __shfl(c, sp - 1);
-    else
-        run = 0.0;
-    const size_t v0 = sp * P.len, v1 = v0 + P.len < P.vocab ? v0 + P.len : P.vocab;
-    int last = -1; // the last value so far with a probability, for a number that no sum passes
-    for (size_t b = v0; b < v1; b += SMP_THREADS) {
-        const size_t v = b + tid;
-        const double e = v < v1 ? residual(r, v, as_prob(r.p[v])) : 0.0;
-        double sum = e;
-        for (int o = 1; o < 64; o *= 2) {
-            const double up = __shfl_up(sum, o);
-            sum += lane >= o ? up : 0.0;
+    int part = 0;
+    double run = 0.0, base = 0.0; // the sums before the chunk of 64 parts, and before the part
+    for (int b0 = 0; b0 < P.splits; b0 += 64) {
+        const double d = b0 + lane < P.splits ? s[2 * (b0 + lane) + which] : 0.0;
+        double sum;
+        const double c = wave_scan_f64(d, &sum) + run;
+        const unsigned long long some = __ballot(d > 0.0), past = __ballot(d > 0.0 && c > at);
+        const int x = past ? __builtin_ctzll(past) : some ? 63 - __builtin_clzll(some) : -1;
+        if (x >= 0) {
+            part = b0 + x;
+            base = x ? __shfl(c, x - 1) : run;
         }
-        if (lane == 63)
-            sw[wave] = sum;
-        __syncthreads();
-        double before = run;
-        for (int w = 0; w < W; w++) {
-            if (w == wave)
-                sum += before;
-            before += sw[w];
-        }
-        run = before;
-        const unsigned long long hit = __ballot(e > 0.0 && sum > at), any = __ballot(e > 0.0);
-        if (lane == 0) {
-            s_found[wave] = hit ? __builtin_ctzll(hit) : -1;
-            s_last[wave] = any ? 63 - __builtin_clzll(any) : -1;
-        }
-        __syncthreads();
-        int found = -1;
-        for (int w = W - 1; w >= 0; w--)
-            found = s_found[w] >= 0 ? w * 64 + s_found[w] : found;
-        for (int w = 0; w < W; w++)
-            last = s_last[w] >= 0 ? (int)(b + w * 64 + s_last[w]) : last;
-        if (found >= 0) {
-            if (tid == 0)
-                out[acc] = (int32_t)(b + found);
-            return;
-        }
-        __syncthreads();
+        if (past)
+            break;
+        run += sum;
     }
-    if (tid == 0)
-        out[acc] = last;
+    // the threads' runs
+    const size_t v0 = (size_t)part * (NV * SMP_THREADS * 4) + (size_t)tid * E;
+    double d = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        smp_f4 p = {0.0f, 0.0f, 0.0f, 0.0f}, q = p;
+        if constexpr (VEC) {
+            if (v0 + e < P.vocab) {
+                p = *(const smp_f4 *)(r.p + v0 + e);
+                if (r.q)
+                    q = *(const smp_f4 *)(r.q + v0 + e);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (v0 + e + c < P.vocab) {
+                    p[c] = r.p[v0 + e + c];
+                    q[c] = r.q ? r.q[v0 + e + c] : 0.0f;
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            d += residual(r, v0 + e + c, as_prob(p[c]), q[c]);
+    }
+    double sum;
+    double c = wave_scan_f64(d, &sum);
+    if (lane == 63)
+        sw[wave] = c;
+    __syncthreads();
+    double start = base;
+    for (int w = 0; w < wave; w++)
+        start += sw[w];
+    const double up = __shfl_up(c, 1);
+    before[tid] = lane ? start + up : start;
+    c += start;
+    const unsigned long long some = __ballot(d > 0.0), past = __ballot(d > 0.0 && c > at);
+    if (lane == 0) {
+        s_hit[wave] = past ? wave * 64 + __builtin_ctzll(past) : -1;
+        s_last[wave] = some ? wave * 64 + 63 - __builtin_clzll(some) : -1;
+    }
+    __syncthreads();
+    if (wave)
+        return;
+    int t = -1;
+    for (int w = W - 1; w >= 0; w--)
+        t = s_hit[w] >= 0 ? s_hit[w] : t;
+    for (int w = W - 1; w >= 0 && t < 0; w--)
+        t = s_last[w];
+    if (t < 0) // the part held nothing after all: not with sums above zero
+        t = 0;
+    // the run's values, a lane each
+    const size_t v = (size_t)part * (NV * SMP_THREADS * 4) + (size_t)t * E + lane;
+    const double e = lane < E && v < P.vocab ? residual(r, v, as_prob(r.p[v]), r.q ? r.q[v] : 0.0f) : 0.0;
+    const double ce = wave_scan_f64(e, &sum) + before[t];
+    const unsigned long long any = __ballot(e > 0.0), hit = __ballot(e > 0.0 && ce > at);
+    const int x = hit ? __builtin_ctzll(hit) : any ? 63 - __builtin_clzll(any) : 0;
+    if (lane == x)
+        out[acc] = any ? (int32_t)v : -1;
+}
+
+template <class F>
+static void by_values(int nv, F f) {
+    if (nv == 2)
+        f(std::integral_constant<int, 2>{});
+    else if (nv == 4)
+        f(std::integral_constant<int, 4>{});
+    else if (nv == 8)
+        f(std::integral_constant<int, 8>{});
+    else
+        f(std::integral_constant<int, 16>{});
 }
 
 } // namespace lh
@@ -329,7 +447,7 @@ using namespace lh;
 extern "C" {
 
 size_t loomhip_token_probs_ws(size_t n, size_t vocab) {
-    return n && vocab ? n * row_splits(n, vocab) * sizeof(ProbRec) : 0;
+    return n && vocab ? n * row_cut(n, vocab).splits * sizeof(ProbRec) : 0;
 }
 
 int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const float *temperature,
@@ -348,13 +466,28 @@ int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t 
     if (int rc = require_device())
         return rc;
     hipStream_t st = stream_of(stream);
-    const int splits = row_splits(n, vocab);
-    const size_t len = split_len(vocab, splits);
+    const RowCut cut = row_cut(n, vocab);
+    if (n * cut.splits > 0xffffff)
+        return fail(LOOMHIP_DECLINED, "token_probs: %zu rows of %zu not served", n, vocab);
     ProbRec *rec = (ProbRec *)ws;
-    hipLaunchKernelGGL(probs_reduce_kernel, dim3(splits, n), dim3(SMP_THREADS), 0, st, logits, vocab, stride,
-                       temperature, len, rec);
-    hipLaunchKernelGGL(probs_write_kernel, dim3(splits, n), dim3(SMP_THREADS), 0, st, logits, vocab, stride,
-                       temperature, len, rec, probs, out_stride);
+    const dim3 g(n * cut.splits);
+    const bool in = vocab % 4 == 0 && (uintptr_t)logits % 16 == 0 && stride % 4 == 0;
+    const bool both = in && (uintptr_t)probs % 16 == 0 && out_stride % 4 == 0;
+    by_values(cut.nv, [&](auto nv) {
+        constexpr int NV = decltype(nv)::value;
+        if (in)
+            hipLaunchKernelGGL((probs_reduce_kernel<NV, true>), g, dim3(SMP_THREADS), 0, st, logits, vocab, stride,
+                               temperature, cut.splits, rec);
+        else
+            hipLaunchKernelGGL((probs_reduce_kernel<NV, false>), g, dim3(SMP_THREADS), 0, st, logits, vocab, stride,
+                               temperature, cut.splits, rec);
+        if (both)
+            hipLaunchKernelGGL((probs_write_kernel<NV, true>), g, dim3(SMP_THREADS), 0, st, logits, vocab, stride,
+                               temperature, cut.splits, rec, probs, out_stride);
+        else
+            hipLaunchKernelGGL((probs_write_kernel<NV, false>), g, dim3(SMP_THREADS), 0, st, logits, vocab, stride,
+                               temperature, cut.splits, rec, probs, out_stride);
+    });
     note_launch();
     note_launch();
     const hipError_t e = hipGetLastError();
@@ -362,7 +495,7 @@ int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t 
 }
 
 size_t loomhip_verify_drafts_ws(size_t n, size_t vocab) {
-    return n && vocab ? n * row_splits(n, vocab) * 2 * sizeof(double) : 0;
+    return n && vocab ? n * verify_cut(n, vocab).splits * 2 * sizeof(double) : 0;
 }
 
 int loomhip_verify_drafts_dev(const float *target_probs, const float *draft_probs, const int32_t *draft_tokens,
@@ -392,13 +525,23 @@ int loomhip_verify_drafts_dev(const float *target_probs, const float *draft_prob
     P.n = n;
     P.k = k;
     P.vocab = vocab;
-    P.splits = row_splits(n, vocab);
-    P.len = split_len(vocab, P.splits);
+    const RowCut cut = verify_cut(n, vocab);
+    P.splits = cut.splits;
     P.sums = (double *)ws;
     P.out = tokens_out;
     P.accepted = n_accepted;
-    hipLaunchKernelGGL(verify_sum_kernel, dim3(P.splits, n), dim3(SMP_THREADS), 0, st, P);
-    hipLaunchKernelGGL(verify_pick_kernel, dim3(n), dim3(SMP_THREADS), 0, st, P);
+    const bool vec = vocab % 4 == 0 && (uintptr_t)target_probs % 16 == 0 && (uintptr_t)draft_probs % 16 == 0;
+    by_values(cut.nv, [&](auto nv) {
+        constexpr int NV = decltype(nv)::value;
+        if (vec)
+            hipLaunchKernelGGL((verify_sum_kernel<NV, true>), dim3(P.splits, n), dim3(SMP_THREADS), 0, st, P);
+        else
+            hipLaunchKernelGGL((verify_sum_kernel<NV, false>), dim3(P.splits, n), dim3(SMP_THREADS), 0, st, P);
+        if (vec)
+            hipLaunchKernelGGL((verify_pick_kernel<NV, true>), dim3(n), dim3(SMP_THREADS), 0, st, P);
+        else
+            hipLaunchKernelGGL((verify_pick_kernel<NV, false>), dim3(n), dim3(SMP_THREADS), 0, st, P);
+    });
     note_launch();
     note_launch();
     const hipError_t e = hipGetLastError();
