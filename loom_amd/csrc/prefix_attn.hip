@@ -237,6 +237,7 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
         const int k = e > 0 && e < 255 ? pa_clamp(13 + 127 - e, -120, 120) : 0;
         const float f = __uint_as_float((uint32_t)(127 + k) << 23) * (P.scale < 0.0f ? -1.0f : 1.0f);
         cs = fabsf(P.scale) * 0x1.715476p+0f * __uint_as_float((uint32_t)(127 - k) << 23);
+        cs = cs < 0x1p-126f ? 0x1p-126f : cs; // not 0: it multiplies a masked key's -inf (scores stay far below 1)
 #pragma unroll
         for (int s = 0; s < STEPS; s++)
 #pragma unroll

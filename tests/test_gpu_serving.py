@@ -95,6 +95,15 @@ def test_prefix_attn_matches_its_definition(sv, shape):
     assert (got[np.isnan(want)] == 0).all()
 
 
+@pytest.mark.parametrize("scale", [-0.25, 0.0, -3e4])
+def test_prefix_attn_scales(sv, scale):
+    """A negative scale turns the order around, zero weighs every row alike."""
+    c = _attn_case(8, 2, 64, 150, 3, 2, 40)
+    c["scale"] = scale
+    want, bound = _attn_ref(c)
+    _within(_attn(sv, c).cpu().numpy(), want, bound)
+
+
 def test_prefix_attn_leaves_rows_past_q_len(sv):
     import torch
 
