@@ -784,7 +784,7 @@ int loomhip_mla_layer_cached_dev(const loomhip_mla_attn *a, const float *const *
  * the same time on several streams or from several threads, each with a
  * workspace of its own: `ws` (device, at a multiple of 16 bytes, contents
  * undefined before and after) of at least the bytes the call's _ws function
- * gives for the same sizes.  Calls that can run at the same time, captured
+ * gives for the same sizes (0: none, NULL will do).  Calls that can run at the same time, captured
  * graphs among them, must not share it.  Outputs must not overlap inputs
  * except where said.  n == 0 is OK and does nothing. */
 

@@ -6,10 +6,10 @@
 // Two launches: y = A_e x for every vector into the workspace, then out.  In
 // decode (most vectors name adapters of their own, so the adapters' bytes are
 // the work) a wave takes a few rows of A_e or B_e for one vector with plain
-// multiply-adds.  In prefill (a request's tokens share an adapter) 16 vectors
-// of one adapter are the columns of f32 matrix-core tiles
-// (v_mfma_f32_16x16x4_f32), found among 128 vectors at a time.  What an
-// adapter holds reaches its own vectors only.
+// multiply-adds; small adapters take both steps in one launch.  In prefill (a
+// request's tokens share an adapter) 16 vectors of one adapter are the columns
+// of f32 matrix-core tiles (v_mfma_f32_16x16x4_f32), found among 128 vectors
+// at a time.  What an adapter holds reaches its own vectors only.
 #include "runtime.hpp"
 
 #include <type_traits>
@@ -20,7 +20,8 @@ typedef float lora_f4 __attribute__((ext_vector_type(4)));
 
 constexpr int LORA_THREADS = 256;
 constexpr int LORA_MAX_RANK = 256;
-constexpr double LORA_FEW = 160e6; // bytes
+constexpr double LORA_FEW = 160e6;    // bytes
+constexpr size_t LORA_SMALL = 131072; // bytes of one A_e
 
 struct LoraParams {
     const void *a, *b; // [n_adapters][rank][cols], [n_adapters][rows][rank]
@@ -247,6 +248,89 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P
         s = lora_sum<LPR>(s);
         if (sub == 0 && r < P.rows)
             out[r] = named ? o[p] + s : o[p];
+    }
+}
+
+// Both steps in one launch, where A_e is small: a work group forms the vector's whole y for itself, LPR * 8 / 16 rows of
+// A_e a wave, then its rows of B_e; the first of those are loaded before y is formed.
+constexpr int LORA_ONE = 1024;
+template <typename T, bool VEC, int LPR>
+__global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
+    constexpr int W = LORA_ONE / 64, RPI = 64 / LPR, R = LPR > 2 ? LPR / 2 : 1;
+    __shared__ float ys[W * R];
+    const size_t t = blockIdx.y, step = (size_t)gridDim.x * W * RPI;
+    const int e = P.ids[t], lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane % LPR, rank = P.rank;
+    const float *x = P.x + t * P.x_stride, *base = P.base ? P.base + t * P.base_stride : nullptr;
+    float *out = P.out + t * P.out_stride;
+    const bool named = lora_names(P, e);
+    const T *a = (const T *)P.a + (named ? (size_t)e * rank * P.cols : 0);
+    const T *b = (const T *)P.b + (named ? (size_t)e * P.rows * rank : 0);
+    const auto k_of = [&](int c) { return VEC ? sub * 8 + c : c * LPR + sub; };
+    float v[8], o;
+    const auto load = [&](size_t r0) {
+        const size_t r = r0 + lane / LPR, at = r < P.rows ? r : P.rows - 1;
+        o = base ? base[at] : 0.0f;
+        if constexpr (VEC) {
+            lora_eight(b + at * rank + (k_of(0) < rank ? k_of(0) : 0), v);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; c++)
+                v[c] = k_of(c) < rank ? lora_one(b + at * rank + k_of(c)) : 0.0f;
+        }
+    };
+    size_t r0 = ((size_t)blockIdx.x * W + wave) * RPI;
+    load(r0);
+    if (named && wave * R < rank) {
+        const T *ar[R];
+        float s[R] = {};
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            ar[i] = a + (size_t)(wave * R + i < rank ? wave * R + i : 0) * P.cols;
+        if constexpr (VEC) {
+#pragma unroll 4
+            for (size_t c = lane * 8; c < P.cols; c += 512) {
+                float xv[8], av[8];
+                lora_eight(x + c, xv);
+#pragma unroll
+                for (int i = 0; i < R; i++) {
+                    lora_eight(ar[i] + c, av);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        s[i] = __builtin_fmaf(av[j], xv[j], s[i]);
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (size_t c = lane; c < P.cols; c += 64)
+#pragma unroll
+                for (int i = 0; i < R; i++)
+                    s[i] = __builtin_fmaf(lora_one(ar[i] + c), x[c], s[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const float y = lora_sum<64>(s[i]) * P.scale[e];
+            if (lane == 0)
+                ys[wave * R + i] = y;
+        }
+    }
+    __syncthreads();
+    float y[8];
+#pragma unroll
+    for (int c = 0; c < 8; c++)
+        y[c] = named && k_of(c) < rank ? ys[k_of(c)] : 0.0f;
+    while (r0 < P.rows) {
+        float s = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            s = k_of(c) < rank ? __builtin_fmaf(v[c], y[c], s) : s;
+        s = lora_sum<LPR>(s);
+        const size_t r = r0 + lane / LPR;
+        const float sum = named ? o + s : o;
+        r0 += step;
+        if (r0 < P.rows)
+            load(r0);
+        if (sub == 0 && r < P.rows)
+            out[r] = sum;
     }
 }
 
@@ -487,6 +571,21 @@ static void lora_few_out(const LoraParams &P, hipStream_t st) {
     hipLaunchKernelGGL((lora_few_out_kernel<T, VB, LPR, Q>), dim3((P.rows + rows - 1) / rows, P.n), dim3(LORA_THREADS), 0,
                        st, P);
 }
+template <typename T, bool VEC>
+static void lora_one(const LoraParams &P, hipStream_t st) {
+    // work groups for half the chip, no more: each reads A_e again
+    const int lpr = P.rank <= 8 ? 1 : P.rank <= 16 ? 2 : P.rank <= 32 ? 4 : 8;
+    const size_t most = (P.rows * lpr + LORA_ONE - 1) / LORA_ONE, want = (128 + P.n - 1) / P.n;
+    const dim3 g(want < most ? want : most, P.n);
+    if (lpr == 1)
+        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 1>), g, dim3(LORA_ONE), 0, st, P);
+    else if (lpr == 2)
+        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 2>), g, dim3(LORA_ONE), 0, st, P);
+    else if (lpr == 4)
+        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 4>), g, dim3(LORA_ONE), 0, st, P);
+    else
+        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 8>), g, dim3(LORA_ONE), 0, st, P);
+}
 template <typename T, bool VA, bool VB>
 static void lora_few(const LoraParams &P, hipStream_t st) {
     constexpr int W = LORA_THREADS / 64;
@@ -541,21 +640,36 @@ static void lora_many_out(const LoraParams &P, bool ovec, hipStream_t st) {
 // Whether the vectors are taken one by one: while all their reads of A_e and B_e, mostly from L2, stay under LORA_FEW
 // bytes.  Measured at 4096 x 2048, rank 64, fp16: 101 MB (128 vectors) 17 us one by one, 21 as tiles, 41 as tiles of
 // mixed requests; 201 MB 29, 21, 42; 403 MB 52, 22, 45.
-static bool lora_is_few(const LoraParams &P, size_t es) {
-    return P.n <= 65535 && (double)P.n * P.rank * (P.rows + P.cols) * es <= LORA_FEW;
+template <class L>
+static bool lora_is_few(const L &l, size_t n, size_t es) {
+    return n <= 65535 && (double)n * l.rank * (l.rows + l.cols) * es <= LORA_FEW;
+}
+// Of those, whether one launch does both steps: the second costs the host 3.5 us, and each work group reads A_e again.
+// Measured, in a graph, against two launches, fp16: A_e of 64 KB, rank 8, 1 vector 4.2 us for 5.1, 256 6.2 for 7.2; of
+// 128 KB, rank 16, 1 vector 5.5 for 5.3, 32 6.2 for 5.5, 256 9.3 for 10.1; rank 64, 1 vector 5.0 for 5.1, 32 8.1 for 7.3.
+template <class L>
+static bool lora_is_one(const L &l, size_t n, size_t es) {
+    return lora_is_few(l, n, es) && l.rank <= 64 && l.rank * l.cols * es <= LORA_SMALL;
 }
 // Loads of four elements where rows and pointers allow them: A_e's rows and x for the first launch, B_e's for the
-// second (base and out beside them where many vectors are tiles).
+// second (base and out beside them where many vectors are tiles).  Returns the launches.
 template <typename T>
-static void lora_run(const LoraParams &P, hipStream_t st) {
+static int lora_run(const LoraParams &P, hipStream_t st) {
     const size_t q = 4 * sizeof(T);
     const bool va = P.cols % 4 == 0 && (uintptr_t)P.a % q == 0 && (uintptr_t)P.x % 16 == 0 && P.x_stride % 4 == 0;
     const bool vb = P.rank % 4 == 0 && (uintptr_t)P.b % q == 0;
     const bool ovec = P.rows % 4 == 0 && (uintptr_t)P.out % 16 == 0 && P.out_stride % 4 == 0 &&
                       (!P.base || ((uintptr_t)P.base % 16 == 0 && P.base_stride % 4 == 0));
-    if (lora_is_few(P, sizeof(T))) {
+    if (lora_is_few(P, P.n, sizeof(T))) {
         const bool va8 = va && P.cols % 8 == 0 && (uintptr_t)P.a % 16 == 0;
         const bool vb8 = P.rank % 8 == 0 && (uintptr_t)P.b % 16 == 0;
+        if (lora_is_one(P, P.n, sizeof(T))) {
+            if (va8 && vb8)
+                lora_one<T, true>(P, st);
+            else
+                lora_one<T, false>(P, st);
+            return 1;
+        }
         if (va8 && vb8)
             lora_few<T, true, true>(P, st);
         else if (va8)
@@ -564,7 +678,7 @@ static void lora_run(const LoraParams &P, hipStream_t st) {
             lora_few<T, false, true>(P, st);
         else
             lora_few<T, false, false>(P, st);
-        return;
+        return 2;
     }
     if (va)
         lora_many_y<T, true>(P, st);
@@ -574,6 +688,7 @@ static void lora_run(const LoraParams &P, hipStream_t st) {
         lora_many_out<T, true>(P, ovec, st);
     else
         lora_many_out<T, false>(P, ovec, st);
+    return 2;
 }
 
 // Splits of the columns: a work group for every CU, none under 512 columns.
@@ -582,6 +697,8 @@ static int lora_splits(size_t cols, size_t n) {
     return (int)(s > most ? most : s > 4 ? 4 : s);
 }
 static size_t lora_ws_bytes(const loomhip_lora *l, size_t n) {
+    if (lora_is_one(*l, n, l->type == LH_F32 ? 4 : 2))
+        return 0;
     return lora_splits(l->cols, n) * n * ((l->rank + 15) / 16 * 16) * 4;
 }
 
@@ -604,7 +721,7 @@ int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, con
     if (n == 0)
         return LOOMHIP_OK;
     const size_t need = lora_ws_bytes(l, n);
-    if (!ws || ws_bytes < need || (uintptr_t)ws % 16)
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
         return fail(LOOMHIP_ERR_ARG, "lora: the workspace takes %zu bytes at a multiple of 16, got %zu", need, ws_bytes);
     if (int rc = require_device())
         return rc;
@@ -612,14 +729,11 @@ int loomhip_lora_dev(const loomhip_lora *l, const float *x, size_t x_stride, con
     P.rp = (int)((l->rank + 15) / 16 * 16);
     P.ks = lora_splits(l->cols, n);
     hipStream_t st = stream_of(stream);
-    if (l->type == LH_F32)
-        lora_run<float>(P, st);
-    else if (l->type == LH_F16)
-        lora_run<_Float16>(P, st);
-    else
-        lora_run<uint16_t>(P, st);
-    note_launch();
-    note_launch();
+    const int launches = l->type == LH_F32   ? lora_run<float>(P, st)
+                         : l->type == LH_F16 ? lora_run<_Float16>(P, st)
+                                             : lora_run<uint16_t>(P, st);
+    for (int i = 0; i < launches; i++)
+        note_launch();
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "lora launch");
 }

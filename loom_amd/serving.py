@@ -39,7 +39,7 @@ def _place(first, *others) -> tuple:
             raise ValueError(f"tensors on {first.device} and {t.device}")
     if dev < 0:
         raise ValueError(f"tensors on {first.device}, not on the GPU")
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         raise ValueError(f"tensors on {first.device}, the current device is {torch.cuda.current_device()}")
     return first.device, torch._C._cuda_getCurrentRawStream(dev)
 
@@ -123,10 +123,10 @@ def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, 
     elif out.shape != shape or out.dtype is not _F32 or not out.is_contiguous():
         raise ValueError("out: as q")
     nb = _attn_ws(pre.rows, own.rows, n, n_q, heads, kv, hd)
-    ws = torch.empty(nb, dtype=_U8, device=dev)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     rc = lib().loomhip_prefix_attn_dev(
         C.byref(pre), C.byref(own), q.data_ptr(), None if own_len is None else own_len.data_ptr(),
-        None if q_len is None else q_len.data_ptr(), n, n_q, heads, kv, hd, scale, out.data_ptr(), ws.data_ptr(), nb, stream)
+        None if q_len is None else q_len.data_ptr(), n, n_q, heads, kv, hd, scale, out.data_ptr(), ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
         _fail("prefix_attn_dev", rc)
     return out
@@ -165,12 +165,12 @@ def lora_dev(x, a, b, scale, ids, base=None, out=None):
     if not _rows_ok(x, n, cols) or not _rows_ok(out, n, rows) or not (base is None or _rows_ok(base, n, rows)):
         raise ValueError("x [n, cols], base and out [n, rows]: f32, rows of consecutive values")
     nb = _lora_ws(n, kind, adapters, rank, rows, cols)
-    ws = torch.empty(nb, dtype=_U8, device=dev)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     d = LoraDesc(kind, adapters, rank, rows, cols, a.data_ptr(), b.data_ptr(), scale.data_ptr())
     rc = lib().loomhip_lora_dev(
         C.byref(d), x.data_ptr(), x.stride(0) if n > 1 else cols, ids.data_ptr(), None if base is None else base.data_ptr(),
         base.stride(0) if base is not None and n > 1 else rows, n, out.data_ptr(), out.stride(0) if n > 1 else rows,
-        ws.data_ptr(), nb, stream)
+        ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
         _fail("lora_dev", rc)
     return out
@@ -193,10 +193,10 @@ def token_probs_dev(logits, temperature=None, out=None):
     elif out.shape != shape or out.dtype is not _F32 or not out.is_contiguous():
         raise ValueError("out: as logits")
     nb = _probs_ws(n, vocab)
-    ws = torch.empty(nb, dtype=_U8, device=dev)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     rc = lib().loomhip_token_probs_dev(logits.data_ptr(), n, vocab, vocab,
                                        None if temperature is None else temperature.data_ptr(), out.data_ptr(), vocab,
-                                       ws.data_ptr(), nb, stream)
+                                       ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
         _fail("token_probs_dev", rc)
     return out
@@ -226,11 +226,11 @@ def verify_drafts_dev(target_probs, draft_tokens, u_accept, u_sample, draft_prob
     tokens = torch.empty((n, k1), dtype=_I32, device=dev)
     accepted = torch.empty((n,), dtype=_I32, device=dev)
     nb = _verify_ws(n, vocab)
-    ws = torch.empty(nb, dtype=_U8, device=dev)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     rc = lib().loomhip_verify_drafts_dev(
         target_probs.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(), draft_tokens.data_ptr(),
         None if n_draft is None else n_draft.data_ptr(), u_accept.data_ptr(), u_sample.data_ptr(), n, k, vocab,
-        tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nb, stream)
+        tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
         _fail("verify_drafts_dev", rc)
     return tokens, accepted

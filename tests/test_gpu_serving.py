@@ -95,6 +95,19 @@ def test_prefix_attn_matches_its_definition(sv, shape):
     assert (got[np.isnan(want)] == 0).all()
 
 
+@pytest.mark.parametrize("shape", [(2, 1, 8, 20, 300, 2, 9), (2, 2, 16, 0, 1030, 3, 4), (1, 1, 16, 70, 1, 1500, 1500),
+                                   (4, 2, 32, 200, 600, 1, 5)], ids=lambda s: "x".join(map(str, s)))
+def test_prefix_attn_many_lanes_and_queries(sv, shape):
+    c = _attn_case(*shape)
+    want, bound = _attn_ref(c)
+    got = _attn(sv, c).cpu().numpy()
+    _within(got, want, bound, "ragged")
+    assert (got[np.isnan(want)] == 0).all()
+    c["q_len"][:-1] = 0  # one lane alone has query tokens
+    want, bound = _attn_ref(c)
+    _within(_attn(sv, c).cpu().numpy(), want, bound, "one lane")
+
+
 @pytest.mark.parametrize("scale", [-0.25, 0.0, -3e4])
 def test_prefix_attn_scales(sv, scale):
     """A negative scale turns the order around, zero weighs every row alike."""
@@ -324,6 +337,78 @@ def test_lora_matches_its_definition(sv, shape, dtype):
     assert bool((out == got).all())  # in place: the same kernels, the same bits
 
 
+LORA_LONG = [
+    # two launches, a vector at a time
+    (3, 70, 16400, 16, 2),
+    (2, 65, 32801, 8, 2),
+    (9, 130, 4099, 40, 3),
+    (4, 1001, 3000, 64, 3),
+    # tiles of vectors that share an adapter
+    (700, 131, 321, 256, 5),
+    (6001, 333, 517, 16, 7),
+    (9001, 500, 700, 8, 3),
+    (3001, 400, 500, 33, 40),
+    (1203, 301, 402, 100, 4),
+    (70000, 3, 5, 1, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("spans", [False, True])
+@pytest.mark.parametrize("shape", LORA_LONG, ids=lambda s: "x".join(map(str, s)))
+def test_lora_many_vectors_and_long_rows(sv, shape, spans, dtype):
+    """Adapters named in any order, and by runs of vectors (the last run none)."""
+    import torch
+
+    n, adapters = shape[0], shape[4]
+    t = _lora_case(*shape, dtype)
+    if spans:
+        t["ids"] = (torch.arange(n, device="cuda") * (adapters + 1) // n).to(torch.int32)
+    want, bound = _lora_ref(t)
+    got = sv.lora_dev(t["x"], t["a"], t["b"], t["scale"], t["ids"], base=t["base"])
+    _within(got.cpu().numpy(), want, bound)
+    none = (t["ids"] < 0) | (t["ids"] >= adapters)
+    assert bool((got[none] == t["base"][none]).all())
+    out = t["base"].clone()
+    sv.lora_dev(t["x"], t["a"], t["b"], t["scale"], t["ids"], base=out, out=out)
+    assert bool((out == got).all())
+    got = sv.lora_dev(t["x"], t["a"], t["b"], t["scale"], t["ids"])
+    _within(got.cpu().numpy(), *_lora_ref(t, base=False), "no base")
+
+
+def test_lora_many_vectors_strided(sv):
+    """Rows shifted by an odd number of values and by four; what lies beside them stays."""
+    import torch
+
+    t = _lora_case(901, 200, 256, 250, 5, "f16")
+    want, bound = _lora_ref(t)
+    for shift in (1, 4):
+        x = torch.full((901, 300), float("nan"), device="cuda")
+        x[:, shift:shift + 256] = t["x"]
+        wide = torch.full((901, 404), 3.25, device="cuda")
+        wide[:, shift:shift + 200] = t["base"]
+        view = wide[:, shift:shift + 200]
+        sv.lora_dev(x[:, shift:shift + 256], t["a"], t["b"], t["scale"], t["ids"], base=view, out=view)
+        _within(view.cpu().numpy(), want, bound, f"shift {shift}")
+        assert bool((wide[:, :shift] == 3.25).all()) and bool((wide[:, shift + 200:] == 3.25).all())
+
+
+def test_lora_many_vectors_bad_values_stay_alone(sv):
+    import torch
+
+    t = _lora_case(1500, 220, 240, 128, 4, "bf16")
+    t["ids"] = (torch.arange(1500, device="cuda") % 4).to(torch.int32)
+    want, bound = _lora_ref(t)
+    t["a"][2] = float("nan")
+    t["b"][1] = float("inf")
+    t["x"][[3, 800]] = float("nan")
+    got = sv.lora_dev(t["x"], t["a"], t["b"], t["scale"], t["ids"], base=t["base"]).cpu().numpy()
+    i = np.arange(1500)
+    fine = np.isin(i % 4, (0, 3)) & ~np.isin(i, (3, 800))
+    _within(got[fine], want[fine], bound[fine])
+    assert not np.isfinite(got[i % 4 == 2]).any() and not np.isfinite(got[[3, 800]]).any()
+
+
 @pytest.mark.parametrize("n", [1, 40, 300])
 def test_lora_spans_and_one_adapter(sv, n):
     """Tokens of a request one after the other; every token the same adapter; no token an adapter."""
@@ -388,7 +473,9 @@ def test_lora_large_values(sv):
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 5), (3, 257), (1, 2048), (2, 2049), (1, 32000), (5, 49999), (70, 1000),
-                                        (2, 151936), (1500, 33), (7, 151937)])
+                                        (2, 151936), (1500, 33), (7, 151937), (3, 1024), (2, 1025), (2, 4096), (1, 4097),
+                                        (3, 16384), (2, 16385), (1, 32768), (2, 32769), (70, 50257), (200, 40001),
+                                        (300, 40003)])
 def test_token_probs_matches_its_definition(sv, rows, vocab):
     r = _rng(rows, vocab)
     x = (r.standard_normal((rows, vocab)) * 4).astype(np.float32)
@@ -403,53 +490,57 @@ def test_token_probs_matches_its_definition(sv, rows, vocab):
     assert bool((logits == got).all())  # in place: the same bits
 
 
-def test_token_probs_special_rows(sv):
+@pytest.mark.parametrize("vocab", [5000, 4900, 1001, 40001])
+def test_token_probs_special_rows(sv, vocab):
     """Masked values (-inf and the type's lowest), a row of them alone, temperatures of zero, below, NaN, tiny, huge."""
     r = _rng(5)
-    vocab = 5000
     x = (r.standard_normal((12, vocab)) * 2).astype(np.float32)
-    x[0, 100:4900] = -np.inf
+    x[0, 100:vocab - 100] = -np.inf
     x[1, 100:] = np.finfo(np.float32).min
     x[2] = -np.inf
-    x[2, 4321] = -3.0
+    x[2, vocab - 679] = -3.0
     x[3] = -np.inf
     x[4] = np.finfo(np.float32).min
     x[5] = 1e30
-    x[6, [50, 4000, 4500]] = 99.0  # the maximum three times
-    x[7, [50, 4000, 4500]] = 99.0
-    x[8, 4999] = 99.0
+    x[6, [50, vocab - 500, vocab - 100]] = 99.0  # the maximum three times
+    x[7, [50, vocab - 500, vocab - 100]] = 99.0
+    x[8, vocab - 1] = 99.0
+    x[11] = -np.inf
     t = np.ones(12, np.float32)
-    t[6], t[7], t[8], t[9], t[10] = 0.0, -1.0, np.nan, 1e-3, 1e6
+    t[6], t[7], t[8], t[9], t[10], t[11] = 0.0, -1.0, np.nan, 1e-3, 1e6, 0.0
     want, bound = ref.token_probs(x, t)
     got = sv.token_probs_dev(_dev(x), _dev(t)).cpu().numpy()
     _within(got, want, bound)
-    assert (got[3] == 0).all() and got[2, 4321] == 1
-    for row, at in ((6, 50), (7, 50), (8, 4999)):
+    assert (got[3] == 0).all() and got[2, vocab - 679] == 1 and (got[11] == 0).all()
+    for row, at in ((6, 50), (7, 50), (8, vocab - 1)):
         assert got[row, at] == 1 and got[row].sum() == 1
-    x[0, 7], x[1, 7] = np.nan, np.inf
+    x[0, 7], x[1, 7], x[3] = np.nan, np.inf, np.nan
     got = sv.token_probs_dev(_dev(x), _dev(t)).cpu().numpy()
-    assert np.isnan(got[0]).all() and np.isnan(got[1]).all()
-    _within(got[2:], want[2:], bound[2:])
+    assert np.isnan(got[[0, 1, 3]]).all()
+    fine = [2, 4, 5, 6, 7, 8, 9, 10, 11]
+    _within(got[fine], want[fine], bound[fine])
 
 
-def test_token_probs_strided_rows(sv):
+@pytest.mark.parametrize("vocab", [700, 33000])
+def test_token_probs_strided_rows(sv, vocab):
     import torch
 
     import loom_amd
     from loom_amd.backend import _ptr, _stream
 
-    x = (_rng(9).standard_normal((6, 700)) * 3).astype(np.float32)
-    wide = torch.full((6, 901), float("nan"), device="cuda")
-    wide[:, 3:703] = _dev(x)
-    out = torch.full((6, 811), 5.0, device="cuda")
+    x = (_rng(9).standard_normal((6, vocab)) * 3).astype(np.float32)
+    wide = torch.full((6, vocab + 201), float("nan"), device="cuda")
+    wide[:, 3:vocab + 3] = _dev(x)
+    out = torch.full((6, vocab + 111), 5.0, device="cuda")
     L = loom_amd.lib()
-    nb = L.loomhip_token_probs_ws(6, 700)
-    ws = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    nb = L.loomhip_token_probs_ws(6, vocab)
+    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device="cuda")
     src, dst = wide[:, 3:], out[:, 1:]
-    assert L.loomhip_token_probs_dev(_ptr(src), 6, 700, 901, None, _ptr(dst), 811, _ptr(ws), nb, _stream()) == 0
+    assert L.loomhip_token_probs_dev(_ptr(src), 6, vocab, vocab + 201, None, _ptr(dst), vocab + 111, _ptr(ws), nb,
+                                     _stream()) == 0
     want, bound = ref.token_probs(x, None)
-    _within(out[:, 1:701].cpu().numpy(), want, bound)
-    assert bool((out[:, 0] == 5).all()) and bool((out[:, 701:] == 5).all())
+    _within(out[:, 1:vocab + 1].cpu().numpy(), want, bound)
+    assert bool((out[:, 0] == 5).all()) and bool((out[:, vocab + 1:] == 5).all())
 
 
 # ---- verification of drafts ---------------------------------------------------------
@@ -485,7 +576,8 @@ def _verify(sv, c, draft=True, n_draft=True):
 
 
 @pytest.mark.parametrize("n,k,vocab", [(1, 0, 1), (1, 1, 1), (1, 3, 7), (4, 4, 300), (9, 2, 2049), (2, 5, 32000),
-                                       (40, 3, 1000), (3, 4, 151936), (1, 130, 50), (300, 1, 64), (1, 2, 151937)])
+                                       (40, 3, 1000), (3, 4, 151936), (1, 130, 50), (300, 1, 64), (1, 2, 151937), (2, 2, 8192),
+                                       (1, 2, 8193), (2, 2, 32768), (2, 2, 32769), (90, 1, 33001)])
 def test_verify_drafts_matches_its_definition(sv, n, k, vocab):
     c = _verify_case(n, k, vocab)
     for draft in (True, False):
@@ -504,42 +596,45 @@ def test_verify_drafts_all_and_none_accepted(sv):
     assert (acc == 0).all()
 
 
-def test_verify_drafts_nothing_left_to_draw(sv):
+@pytest.mark.parametrize("vocab", [3000, 9000, 33003])
+def test_verify_drafts_nothing_left_to_draw(sv, vocab):
     """p equal to q (nothing above it: the target's own row), p nowhere positive, a single positive value."""
-    c = _verify_case(6, 2, 3000)
+    c = _verify_case(6, 2, vocab)
     c["ua"][:] = 1.0
     c["draft"][0] = c["target"][0, :2]
     c["draft"][1] = np.maximum(c["target"][1, :2], c["draft"][1])
     c["target"][2] = 0.0
     c["target"][3] = 0.0
-    c["target"][3, :, 2999] = 0.25
+    c["target"][3, :, vocab - 1] = 0.25
     c["target"][4] = 0.0
     c["target"][4, :, 0] = 1.0
     t, a = _verify(sv, c, n_draft=False)
-    assert t[2, 0] == -1 and t[3, 0] == 2999 and a[0] == 0
+    assert t[2, 0] == -1 and t[3, 0] == vocab - 1 and a[0] == 0
     _verify(sv, c, draft=False)
 
 
-def test_verify_drafts_numbers_at_the_ends(sv):
-    c = _verify_case(8, 1, 4097)
+@pytest.mark.parametrize("vocab", [4097, 9000, 33003])
+def test_verify_drafts_numbers_at_the_ends(sv, vocab):
+    c = _verify_case(8, 1, vocab)
     c["us"][:] = [0.0, -1.0, np.nan, 1.0, 2.0, np.inf, 1.0 - 2.0 ** -24, -np.inf]
     c["target"][:, :, :100] = 0.0
     c["target"][:, :, -100:] = 0.0
     t, a = _verify(sv, c)
     _verify(sv, c, draft=False)
     drawn = t[np.arange(8), a]
-    assert (drawn[[0, 1, 2, 7]] >= 100).all() and (drawn[[3, 4, 5]] < 4097 - 100).all()
+    assert (drawn[[0, 1, 2, 7]] >= 100).all() and (drawn[[3, 4, 5]] < vocab - 100).all()
 
 
-def test_verify_drafts_strange_values(sv):
+@pytest.mark.parametrize("vocab", [777, 9000, 33003])
+def test_verify_drafts_strange_values(sv, vocab):
     """NaN, infinite and negative entries count as nothing; drafted tokens outside the vocabulary are refused; counts
     out of range are clamped."""
-    c = _verify_case(12, 3, 777)
+    c = _verify_case(12, 3, vocab)
     r = _rng(3)
     for bad in (np.nan, np.inf, -np.inf, -1.0):
         for name in ("target", "draft"):
             c[name][r.random(c[name].shape) < 0.05] = bad
-    c["tok"][0, 0], c["tok"][1, 1], c["tok"][2, 0] = 777, -1, 1 << 30
+    c["tok"][0, 0], c["tok"][1, 1], c["tok"][2, 0] = vocab, -1, 1 << 30
     c["ua"][3:5] = np.nan
     c["n_draft"][:] = [3, 3, 3, 3, 3, 99, -4, 0, 1, 2, 3, 3]
     for draft in (True, False):

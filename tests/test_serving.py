@@ -84,9 +84,9 @@ def _lora(type=loom_amd.F16, adapters=2, rank=8, rows=64, cols=32, a=FAKE, b=FAK
     (loom_amd.ERR_ARG, dict(base=0x300000, bs=63)),
     (loom_amd.ERR_ARG, dict(a=FAKE + 1)),
     (loom_amd.ERR_ARG, dict(x=0x100002)),
-    (loom_amd.ERR_ARG, dict(ws=None)),
-    (loom_amd.ERR_ARG, dict(ws=FAKE + 8)),
-    (loom_amd.ERR_ARG, dict(ws_bytes=255)),
+    (loom_amd.ERR_ARG, dict(rank=128, ws=None)),
+    (loom_amd.ERR_ARG, dict(rank=128, ws=FAKE + 8)),
+    (loom_amd.ERR_ARG, dict(rank=128, ws_bytes=255)),
     (loom_amd.DECLINED, dict(n=65535 * 64 + 1)),
     (loom_amd.ERR_ARG, dict(out=0x100000)),               # over x
     (loom_amd.ERR_ARG, dict(out=0x100000 - 4)),           # into x
@@ -104,9 +104,12 @@ def test_lora_refuses(rc, args):
     (loom_amd.ERR_ARG, dict(vocab=0)),
     (loom_amd.ERR_ARG, dict(stride=99)),
     (loom_amd.ERR_ARG, dict(os=99)),
-    (loom_amd.ERR_ARG, dict(ws=None)),
-    (loom_amd.ERR_ARG, dict(ws=FAKE + 8)),
-    (loom_amd.ERR_ARG, dict(ws_bytes=15)),
+    (loom_amd.ERR_ARG, dict(logits=FAKE + 2)),
+    (loom_amd.ERR_ARG, dict(t=FAKE + 1)),
+    (loom_amd.ERR_ARG, dict(probs=0x100002)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, stride=40000, os=40000, ws=None)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, stride=40000, os=40000, ws=FAKE + 8)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, stride=40000, os=40000, ws_bytes=15)),
     (loom_amd.DECLINED, dict(n=65536)),
     (loom_amd.DECLINED, dict(vocab=1 << 31, stride=1 << 31, os=1 << 31)),
 ])
@@ -125,10 +128,13 @@ def test_token_probs_refuses(rc, args):
     (loom_amd.ERR_ARG, dict(us=None)),
     (loom_amd.ERR_ARG, dict(out=None)),
     (loom_amd.ERR_ARG, dict(acc=None)),
+    (loom_amd.ERR_ARG, dict(target=FAKE + 2)),
+    (loom_amd.ERR_ARG, dict(us=FAKE + 1)),
+    (loom_amd.ERR_ARG, dict(out=FAKE + 2)),
     (loom_amd.ERR_ARG, dict(vocab=0)),
-    (loom_amd.ERR_ARG, dict(ws=None)),
-    (loom_amd.ERR_ARG, dict(ws=FAKE + 4)),
-    (loom_amd.ERR_ARG, dict(ws_bytes=8)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, ws=None)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, ws=FAKE + 4)),
+    (loom_amd.ERR_ARG, dict(vocab=40000, ws_bytes=8)),
     (loom_amd.DECLINED, dict(n=65536)),
     (loom_amd.DECLINED, dict(k=4097)),
     (loom_amd.DECLINED, dict(vocab=1 << 31)),
@@ -155,6 +161,8 @@ def test_workspaces_grow_with_the_call():
     assert L.loomhip_token_probs_ws(5, 0) == 0 and L.loomhip_verify_drafts_ws(5, 0) == 0
     d = loom_amd.LoraDesc(loom_amd.F16, 1, 8, 64, 64, FAKE, FAKE, FAKE)
     assert L.loomhip_lora_ws(C.byref(d), 0) == 0 and L.loomhip_lora_ws(None, 4) == 0
+    assert L.loomhip_lora_ws(C.byref(d), 1) == 0  # one launch
+    d = loom_amd.LoraDesc(loom_amd.F16, 1, 128, 64, 64, FAKE, FAKE, FAKE)
     assert 0 < L.loomhip_lora_ws(C.byref(d), 1) <= L.loomhip_lora_ws(C.byref(d), 1000)
     for bad in (loom_amd.LoraDesc(loom_amd.F16, 1, 0, 64, 64), loom_amd.LoraDesc(loom_amd.F16, 1, 8, 0, 64),
                 loom_amd.LoraDesc(loom_amd.F16, 1, 8, 64, 0), loom_amd.LoraDesc(loom_amd.F16, 1, 257, 64, 64)):
@@ -164,7 +172,10 @@ def test_workspaces_grow_with_the_call():
     assert L.loomhip_prefix_attn_ws(100, 10, 2, 1, 8, 0, 64) == 0
     assert L.loomhip_prefix_attn_ws(0, 0, 2, 1, 8, 2, 64) == 0
     assert L.loomhip_prefix_attn_ws(100, 10, 2, 1, 8, 2, 64) >= 2 * 8 * 64 * 4 * 2
-    for n, vocab in ((1, 1), (1, 32000), (64, 151936), (65535, 7)):
+    for n, vocab in ((1, 1), (1, 8192), (65535, 7)):  # one launch
+        assert L.loomhip_token_probs_ws(n, vocab) == 0
+        assert L.loomhip_verify_drafts_ws(n, vocab) == 0
+    for n, vocab in ((1, 32769), (64, 151936), (65535, 50257)):
         assert L.loomhip_token_probs_ws(n, vocab) >= 16 * n
         assert L.loomhip_verify_drafts_ws(n, vocab) >= 16 * n
 
