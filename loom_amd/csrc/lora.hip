@@ -17,6 +17,10 @@
 namespace lh {
 
 typedef float lora_f4 __attribute__((ext_vector_type(4)));
+// The same at any element: rows of odd lengths start anywhere.
+typedef lora_f4 lora_f4u __attribute__((aligned(4)));
+typedef uint32_t lora_u2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t lora_u4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int LORA_THREADS = 256;
 constexpr int LORA_MAX_RANK = 256;
@@ -87,9 +91,9 @@ __device__ __forceinline__ float lora_one(const T *p) {
 template <typename T>
 __device__ __forceinline__ lora_f4 lora_four(const T *p) {
     if constexpr (std::is_same_v<T, float>) {
-        return *(const lora_f4 *)p;
+        return *(const lora_f4u *)p;
     } else {
-        const uint2 v = *(const uint2 *)p;
+        const lora_u2u v = *(const lora_u2u *)p;
         if constexpr (std::is_same_v<T, uint16_t>)
             return lora_f4{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
                            __uint_as_float(v.y & 0xffff0000u)};
@@ -98,38 +102,46 @@ __device__ __forceinline__ lora_f4 lora_four(const T *p) {
                            half_bits_to_float(v.y >> 16)};
     }
 }
-// Elements k .. k + 3 of a row of `len`, zero past its end.  VEC: the row starts at a multiple of four elements' bytes
-// and so does every k.
-template <bool VEC, typename T>
+// Elements k .. k + 3 of a row of `len`, zero past its end.
+template <typename T>
 __device__ __forceinline__ lora_f4 lora_at(const T *row, size_t k, size_t len) {
     lora_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (VEC) {
-        if (k < len) // len a multiple of 4
-            v = lora_four(row + k);
+    if (k + 4 <= len) {
+        v = lora_four(row + k);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 3; i++)
             if (k + i < len)
                 v[i] = lora_one(row + k + i);
     }
     return v;
 }
-// Eight from a 16-byte aligned place of a 16-bit row (two times four of a wider one).
+// Eight.
 template <typename T>
 __device__ __forceinline__ void lora_eight(const T *p, float *v) {
     if constexpr (std::is_same_v<T, float>) {
-        const lora_f4 a = *(const lora_f4 *)p, b = *(const lora_f4 *)(p + 4);
+        const lora_f4 a = *(const lora_f4u *)p, b = *(const lora_f4u *)(p + 4);
 #pragma unroll
         for (int i = 0; i < 4; i++)
             v[i] = a[i], v[4 + i] = b[i];
     } else {
-        const uint4 w = *(const uint4 *)p;
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        const lora_u4u u = *(const lora_u4u *)p;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             v[2 * i] = std::is_same_v<T, uint16_t> ? __uint_as_float(u[i] << 16) : half_bits_to_float(u[i]);
             v[2 * i + 1] = std::is_same_v<T, uint16_t> ? __uint_as_float(u[i] & 0xffff0000u) : half_bits_to_float(u[i] >> 16);
         }
+    }
+}
+// The eight from k on of a row of `len`, zero past its end.
+template <typename T>
+__device__ __forceinline__ void lora_eight_at(const T *row, int k, int len, float (&v)[8]) {
+    if (k + 8 <= len) {
+        lora_eight(row + k, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            v[i] = k + i < len ? lora_one(row + k + i) : 0.0f;
     }
 }
 // The sum over aligned groups of L lanes, in all of them.
@@ -152,9 +164,8 @@ __device__ __forceinline__ float lora_sum(float v) {
 __device__ __forceinline__ bool lora_names(const LoraParams &P, int e) { return e >= 0 && (size_t)e < P.n_adapters; }
 
 // ---- few vectors ------------------------------------------------------------------
-// y[t][r .. r + RPW): a wave per RPW rows of A_e, a lane every 64th group of eight columns (of four, one by one, where
-// rows are not 16-byte aligned).
-template <typename T, bool VEC, int RPW>
+// y[t][r .. r + RPW): a wave per RPW rows of A_e, a lane every 64th group of eight columns.
+template <typename T, int RPW>
 __global__ __launch_bounds__(LORA_THREADS) void lora_few_y_kernel(LoraParams P) {
     const size_t t = blockIdx.y;
     const int e = P.ids[t], lane = threadIdx.x & 63;
@@ -170,27 +181,25 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_y_kernel(LoraParams P) 
 #pragma unroll
     for (int i = 0; i < RPW; i++)
         s[i] = 0.0f;
-    if constexpr (VEC) {
+    const size_t eights = P.cols / 8 * 8;
 #pragma unroll 2
-        for (size_t k = lane * 8; k < P.cols; k += 512) {
-            float xv[8], av[RPW][8];
-            lora_eight(x + k, xv);
+    for (size_t k = lane * 8; k < eights; k += 512) {
+        float xv[8], av[RPW][8];
+        lora_eight(x + k, xv);
 #pragma unroll
-            for (int i = 0; i < RPW; i++)
-                lora_eight(a[i] + k, av[i]);
+        for (int i = 0; i < RPW; i++)
+            lora_eight(a[i] + k, av[i]);
 #pragma unroll
-            for (int i = 0; i < RPW; i++)
+        for (int i = 0; i < RPW; i++)
 #pragma unroll
-                for (int c = 0; c < 8; c++)
-                    s[i] = __builtin_fmaf(av[i][c], xv[c], s[i]);
-        }
-    } else {
-#pragma unroll 8
-        for (size_t k = lane; k < P.cols; k += 64)
-#pragma unroll
-            for (int i = 0; i < RPW; i++)
-                s[i] = __builtin_fmaf(lora_one(a[i] + k), x[k], s[i]);
+            for (int c = 0; c < 8; c++)
+                s[i] = __builtin_fmaf(av[i][c], xv[c], s[i]);
     }
+    const size_t k = eights + lane;
+    if (k < P.cols)
+#pragma unroll
+        for (int i = 0; i < RPW; i++)
+            s[i] = __builtin_fmaf(lora_one(a[i] + k), x[k], s[i]);
 #pragma unroll
     for (int i = 0; i < RPW; i++) {
         s[i] = lora_sum<64>(s[i]);
@@ -200,9 +209,9 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_y_kernel(LoraParams P) 
 }
 
 // out[t][..]: LPR lanes per row of B_e, each with the same ranks of every row (its part of y stays in registers): Q times
-// eight in a row (VEC), else Q times eight that lie LPR apart.  LORA_PASSES passes of 64 / LPR rows a wave.
+// eight in a row.  LORA_PASSES passes of 64 / LPR rows a wave.
 constexpr int LORA_PASSES = 4;
-template <typename T, bool VEC, int LPR, int Q>
+template <typename T, int LPR, int Q>
 __global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P) {
     constexpr int RPI = 64 / LPR, W = LORA_THREADS / 64;
     const size_t t = blockIdx.y;
@@ -214,23 +223,22 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P
     const T *b = (const T *)P.b + (named ? (size_t)e * P.rows * P.rank : 0);
     const int rank = P.rank;
     float y[Q][8], v[LORA_PASSES][Q][8], o[LORA_PASSES];
-    const auto k_of = [&](int q, int c) { return VEC ? (q * LPR + sub) * 8 + c : (q * 8 + c) * LPR + sub; };
+    const auto k_of = [&](int q, int c) { return (q * LPR + sub) * 8 + c; };
+    const auto row = [&](int p) { return w0 + p * RPI + lane / LPR; };
+    const auto load = [&](auto eight) {
 #pragma unroll
-    for (int p = 0; p < LORA_PASSES; p++) {
-        const size_t r = w0 + p * RPI + lane / LPR, at = r < P.rows ? r : P.rows - 1;
-        o[p] = base ? base[at] : 0.0f;
+        for (int p = 0; p < LORA_PASSES; p++) {
+            const size_t at = row(p) < P.rows ? row(p) : P.rows - 1;
+            o[p] = base ? base[at] : 0.0f;
 #pragma unroll
-        for (int q = 0; q < Q; q++) {
-            if constexpr (VEC) {
-                // ranks past the last are the first ones again, against a y of zero
-                lora_eight(b + at * rank + (k_of(q, 0) < rank ? k_of(q, 0) : 0), v[p][q]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    v[p][q][c] = k_of(q, c) < rank ? lora_one(b + at * rank + k_of(q, c)) : 0.0f;
-            }
+            for (int q = 0; q < Q; q++)
+                eight(b + at * rank, k_of(q, 0), v[p][q]);
         }
-    }
+    };
+    if (rank % 8 == 0) // ranks past the last are the first ones again, and left out of the sum
+        load([&](const T *r, int k, float (&v)[8]) { lora_eight(r + (k < rank ? k : 0), v); });
+    else
+        load([&](const T *r, int k, float (&v)[8]) { lora_eight_at(r, k, rank, v); });
 #pragma unroll
     for (int q = 0; q < Q; q++)
 #pragma unroll
@@ -238,13 +246,13 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P
             y[q][c] = k_of(q, c) < rank ? P.y[t * P.rp + k_of(q, c)] : 0.0f;
 #pragma unroll
     for (int p = 0; p < LORA_PASSES; p++) {
-        const size_t r = w0 + p * RPI + lane / LPR;
+        const size_t r = row(p);
         float s = 0.0f;
 #pragma unroll
         for (int q = 0; q < Q; q++)
 #pragma unroll
             for (int c = 0; c < 8; c++)
-                s = k_of(q, c) < rank ? __builtin_fmaf(v[p][q][c], y[q][c], s) : s;
+                s = k_of(q, 0) < rank ? __builtin_fmaf(v[p][q][c], y[q][c], s) : s;
         s = lora_sum<LPR>(s);
         if (sub == 0 && r < P.rows)
             out[r] = named ? o[p] + s : o[p];
@@ -254,7 +262,7 @@ __global__ __launch_bounds__(LORA_THREADS) void lora_few_out_kernel(LoraParams P
 // Both steps in one launch, where A_e is small: a work group forms the vector's whole y for itself, LPR * 8 / 16 rows of
 // A_e a wave, then its rows of B_e; the first of those are loaded before y is formed.
 constexpr int LORA_ONE = 1024;
-template <typename T, bool VEC, int LPR>
+template <typename T, int LPR>
 __global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
     constexpr int W = LORA_ONE / 64, RPI = 64 / LPR, R = LPR > 2 ? LPR / 2 : 1;
     __shared__ float ys[W * R];
@@ -265,18 +273,11 @@ __global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
     const bool named = lora_names(P, e);
     const T *a = (const T *)P.a + (named ? (size_t)e * rank * P.cols : 0);
     const T *b = (const T *)P.b + (named ? (size_t)e * P.rows * rank : 0);
-    const auto k_of = [&](int c) { return VEC ? sub * 8 + c : c * LPR + sub; };
     float v[8], o;
     const auto load = [&](size_t r0) {
         const size_t r = r0 + lane / LPR, at = r < P.rows ? r : P.rows - 1;
         o = base ? base[at] : 0.0f;
-        if constexpr (VEC) {
-            lora_eight(b + at * rank + (k_of(0) < rank ? k_of(0) : 0), v);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 8; c++)
-                v[c] = k_of(c) < rank ? lora_one(b + at * rank + k_of(c)) : 0.0f;
-        }
+        lora_eight_at(b + at * rank, sub * 8, rank, v);
     };
     size_t r0 = ((size_t)blockIdx.x * W + wave) * RPI;
     load(r0);
@@ -286,26 +287,24 @@ __global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
 #pragma unroll
         for (int i = 0; i < R; i++)
             ar[i] = a + (size_t)(wave * R + i < rank ? wave * R + i : 0) * P.cols;
-        if constexpr (VEC) {
+        const size_t eights = P.cols / 8 * 8;
 #pragma unroll 4
-            for (size_t c = lane * 8; c < P.cols; c += 512) {
-                float xv[8], av[8];
-                lora_eight(x + c, xv);
+        for (size_t c = lane * 8; c < eights; c += 512) {
+            float xv[8], av[8];
+            lora_eight(x + c, xv);
 #pragma unroll
-                for (int i = 0; i < R; i++) {
-                    lora_eight(ar[i] + c, av);
+            for (int i = 0; i < R; i++) {
+                lora_eight(ar[i] + c, av);
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        s[i] = __builtin_fmaf(av[j], xv[j], s[i]);
-                }
+                for (int j = 0; j < 8; j++)
+                    s[i] = __builtin_fmaf(av[j], xv[j], s[i]);
             }
-        } else {
-#pragma unroll 4
-            for (size_t c = lane; c < P.cols; c += 64)
-#pragma unroll
-                for (int i = 0; i < R; i++)
-                    s[i] = __builtin_fmaf(lora_one(ar[i] + c), x[c], s[i]);
         }
+        const size_t c = eights + lane;
+        if (c < P.cols)
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                s[i] = __builtin_fmaf(lora_one(ar[i] + c), x[c], s[i]);
 #pragma unroll
         for (int i = 0; i < R; i++) {
             const float y = lora_sum<64>(s[i]) * P.scale[e];
@@ -317,12 +316,12 @@ __global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
     float y[8];
 #pragma unroll
     for (int c = 0; c < 8; c++)
-        y[c] = named && k_of(c) < rank ? ys[k_of(c)] : 0.0f;
+        y[c] = named && sub * 8 + c < rank ? ys[sub * 8 + c] : 0.0f;
     while (r0 < P.rows) {
         float s = 0.0f;
 #pragma unroll
         for (int c = 0; c < 8; c++)
-            s = k_of(c) < rank ? __builtin_fmaf(v[c], y[c], s) : s;
+            s = __builtin_fmaf(v[c], y[c], s);
         s = lora_sum<LPR>(s);
         const size_t r = r0 + lane / LPR;
         const float sum = named ? o + s : o;
@@ -427,7 +426,7 @@ __device__ __forceinline__ int lora_tiles(const LoraParams &P, size_t t0, LoraTi
 // of 16 ranks.
 constexpr int LORA_Z = LORA_BLOCK / 16;
 __host__ __device__ constexpr int lora_y_waves(int rt) { return rt <= 8 ? 8 : 4; }
-template <typename T, bool VEC, int RT>
+template <typename T, int RT>
 __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(LoraParams P) {
     constexpr int W = lora_y_waves(RT);
     __shared__ lora_f4 part[W][RT][64];
@@ -453,14 +452,14 @@ __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(Lora
             lora_f4 xv[KB], av[KB][RT];
 #pragma unroll
             for (int q = 0; q < KB; q++)
-                xv[q] = lora_at<VEC>(x, k + q * 16, k1);
+                xv[q] = lora_at(x, k + q * 16, k1);
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 // ranks past the last: the last one's, dropped with the rows of y
                 const int row = r * 16 + col < P.rank ? r * 16 + col : P.rank - 1;
 #pragma unroll
                 for (int q = 0; q < KB; q++)
-                    av[q][r] = lora_at<VEC>(a + (size_t)row * P.cols, k + q * 16, k1);
+                    av[q][r] = lora_at(a + (size_t)row * P.cols, k + q * 16, k1);
             }
 #pragma unroll
             for (int q = 0; q < KB; q++)
@@ -489,7 +488,7 @@ __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(Lora
 // out for a block's vectors and 64 rows: a wave every LORA_OW-th tile, M-tile m the rows 16 m + .. of B_e.  The products leave
 // a lane 16 bytes of 16 vectors' rows; through LDS the wave reads base and writes out as 256 bytes of a row at a time.
 constexpr int LORA_OW = 8, LORA_OUT = 64, LORA_OUT_PAD = LORA_OUT + 4;
-template <typename T, bool VEC, bool OVEC>
+template <typename T>
 __global__ __launch_bounds__(64 * LORA_OW) void lora_many_out_kernel(LoraParams P) {
     constexpr int MT = LORA_OUT / 16;
     __shared__ LoraTiles L;
@@ -500,22 +499,16 @@ __global__ __launch_bounds__(64 * LORA_OW) void lora_many_out_kernel(LoraParams 
     float *const mine = (float *)turn[wave]; // [vector][row], rows padded against bank conflicts
     for (int tile = wave; tile < tiles; tile += LORA_OW) {
         const int e = L.adapter[tile];
-        // four rows of 16 lanes' four values each (OVEC), or one of 64 lanes' one, a pass
-        constexpr int PASS = OVEC ? 4 : 16, PER = 16 / PASS;
-        int v[PASS];
-        lora_f4 o[PASS];
-        const size_t row = r0 + (OVEC ? (lane & 15) * 4 : lane);
+        // four vectors' 16 lanes of four values each, a pass
+        int v[4];
+        lora_f4 o[4];
+        const size_t row = r0 + (lane & 15) * 4;
 #pragma unroll
-        for (int p = 0; p < PASS; p++) {
-            v[p] = L.vec[tile][p * PER + (OVEC ? lane >> 4 : 0)];
+        for (int p = 0; p < 4; p++) {
+            v[p] = L.vec[tile][p * 4 + (lane >> 4)];
             o[p] = lora_f4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (P.base && v[p] >= 0 && row < P.rows) {
-                const float *b = P.base + (t0 + v[p]) * P.base_stride + row;
-                if constexpr (OVEC)
-                    o[p] = *(const lora_f4 *)b;
-                else
-                    o[p][0] = *b;
-            }
+            if (P.base && v[p] >= 0)
+                o[p] = lora_at(P.base + (t0 + v[p]) * P.base_stride, row, P.rows);
         }
         if (e >= 0) {
             const int c0 = L.vec[tile][col];
@@ -533,7 +526,7 @@ __global__ __launch_bounds__(64 * LORA_OW) void lora_many_out_kernel(LoraParams 
 #pragma unroll
                 for (int m = 0; m < MT; m++) {
                     const size_t r = r0 + m * 16 + col;
-                    const lora_f4 bv = lora_at<VEC>(b + (r < P.rows ? r : P.rows - 1) * P.rank, k, P.rank);
+                    const lora_f4 bv = lora_at(b + (r < P.rows ? r : P.rows - 1) * P.rank, k, P.rank);
 #pragma unroll
                     for (int c = 0; c < 4; c++)
                         // ranks past the last are zero in b; y there may be anything
@@ -545,96 +538,91 @@ __global__ __launch_bounds__(64 * LORA_OW) void lora_many_out_kernel(LoraParams 
                 *(lora_f4 *)(mine + col * LORA_OUT_PAD + m * 16 + g * 4) = acc[m];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int p = 0; p < PASS; p++) {
-                if constexpr (OVEC)
-                    o[p] += *(const lora_f4 *)(mine + (p * PER + (lane >> 4)) * LORA_OUT_PAD + (lane & 15) * 4);
-                else
-                    o[p][0] += mine[p * LORA_OUT_PAD + lane];
-            }
+            for (int p = 0; p < 4; p++)
+                o[p] += *(const lora_f4 *)(mine + (p * 4 + (lane >> 4)) * LORA_OUT_PAD + (lane & 15) * 4);
             __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
-        for (int p = 0; p < PASS; p++)
-            if (v[p] >= 0 && row < P.rows) {
-                float *out = P.out + (t0 + v[p]) * P.out_stride + row;
-                if constexpr (OVEC)
-                    *(lora_f4 *)out = o[p];
-                else
-                    *out = o[p][0];
+        for (int p = 0; p < 4; p++) {
+            float *out = P.out + (t0 + v[p]) * P.out_stride + row;
+            if (v[p] < 0)
+                continue;
+            if (row + 4 <= P.rows) {
+                *(lora_f4u *)out = o[p];
+            } else {
+#pragma unroll
+                for (int c = 0; c < 3; c++)
+                    if (row + c < P.rows)
+                        out[c] = o[p][c];
             }
+        }
     }
 }
 
-template <typename T, bool VB, int LPR, int Q>
+template <typename T, int LPR, int Q>
 static void lora_few_out(const LoraParams &P, hipStream_t st) {
     const size_t rows = (LORA_THREADS / 64) * LORA_PASSES * (64 / LPR);
-    hipLaunchKernelGGL((lora_few_out_kernel<T, VB, LPR, Q>), dim3((P.rows + rows - 1) / rows, P.n), dim3(LORA_THREADS), 0,
-                       st, P);
+    hipLaunchKernelGGL((lora_few_out_kernel<T, LPR, Q>), dim3((P.rows + rows - 1) / rows, P.n), dim3(LORA_THREADS), 0, st,
+                       P);
 }
-template <typename T, bool VEC>
-static void lora_one(const LoraParams &P, hipStream_t st) {
+template <typename T>
+static void lora_both(const LoraParams &P, hipStream_t st) {
     // work groups for half the chip, no more: each reads A_e again
     const int lpr = P.rank <= 8 ? 1 : P.rank <= 16 ? 2 : P.rank <= 32 ? 4 : 8;
     const size_t most = (P.rows * lpr + LORA_ONE - 1) / LORA_ONE, want = (128 + P.n - 1) / P.n;
     const dim3 g(want < most ? want : most, P.n);
     if (lpr == 1)
-        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 1>), g, dim3(LORA_ONE), 0, st, P);
+        hipLaunchKernelGGL((lora_one_kernel<T, 1>), g, dim3(LORA_ONE), 0, st, P);
     else if (lpr == 2)
-        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 2>), g, dim3(LORA_ONE), 0, st, P);
+        hipLaunchKernelGGL((lora_one_kernel<T, 2>), g, dim3(LORA_ONE), 0, st, P);
     else if (lpr == 4)
-        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 4>), g, dim3(LORA_ONE), 0, st, P);
+        hipLaunchKernelGGL((lora_one_kernel<T, 4>), g, dim3(LORA_ONE), 0, st, P);
     else
-        hipLaunchKernelGGL((lora_one_kernel<T, VEC, 8>), g, dim3(LORA_ONE), 0, st, P);
+        hipLaunchKernelGGL((lora_one_kernel<T, 8>), g, dim3(LORA_ONE), 0, st, P);
 }
-template <typename T, bool VA, bool VB>
+template <typename T>
 static void lora_few(const LoraParams &P, hipStream_t st) {
     constexpr int W = LORA_THREADS / 64;
     // rows of A_e a wave: one while that leaves the chip few waves, else two (a vector is read once for both)
     const int rpw = P.n * P.rank <= 2048 ? 1 : 2;
     const dim3 gy((P.rank + W * rpw - 1) / (W * rpw), P.n);
     if (rpw == 1)
-        hipLaunchKernelGGL((lora_few_y_kernel<T, VA, 1>), gy, dim3(LORA_THREADS), 0, st, P);
+        hipLaunchKernelGGL((lora_few_y_kernel<T, 1>), gy, dim3(LORA_THREADS), 0, st, P);
     else
-        hipLaunchKernelGGL((lora_few_y_kernel<T, VA, 2>), gy, dim3(LORA_THREADS), 0, st, P);
+        hipLaunchKernelGGL((lora_few_y_kernel<T, 2>), gy, dim3(LORA_THREADS), 0, st, P);
     if (P.rank <= 8)
-        lora_few_out<T, VB, 1, 1>(P, st);
+        lora_few_out<T, 1, 1>(P, st);
     else if (P.rank <= 16)
-        lora_few_out<T, VB, 2, 1>(P, st);
+        lora_few_out<T, 2, 1>(P, st);
     else if (P.rank <= 32)
-        lora_few_out<T, VB, 4, 1>(P, st);
+        lora_few_out<T, 4, 1>(P, st);
     else if (P.rank <= 64)
-        lora_few_out<T, VB, 8, 1>(P, st);
+        lora_few_out<T, 8, 1>(P, st);
     else if (P.rank <= 128)
-        lora_few_out<T, VB, 16, 1>(P, st);
+        lora_few_out<T, 16, 1>(P, st);
     else
-        lora_few_out<T, VB, 16, 2>(P, st);
+        lora_few_out<T, 16, 2>(P, st);
 }
 
-template <typename T, bool VA, int RT>
+template <typename T, int RT>
 static void lora_many_y(const LoraParams &P, hipStream_t st) {
-    hipLaunchKernelGGL((lora_many_y_kernel<T, VA, RT>), dim3((P.n + LORA_BLOCK - 1) / LORA_BLOCK, LORA_Z, P.ks),
+    hipLaunchKernelGGL((lora_many_y_kernel<T, RT>), dim3((P.n + LORA_BLOCK - 1) / LORA_BLOCK, LORA_Z, P.ks),
                        dim3(64 * lora_y_waves(RT)), 0, st, P);
 }
-template <typename T, bool VA>
-static void lora_many_y(const LoraParams &P, hipStream_t st) {
+template <typename T>
+static void lora_many(const LoraParams &P, hipStream_t st) {
     if (P.rp <= 16)
-        lora_many_y<T, VA, 1>(P, st);
+        lora_many_y<T, 1>(P, st);
     else if (P.rp <= 32)
-        lora_many_y<T, VA, 2>(P, st);
+        lora_many_y<T, 2>(P, st);
     else if (P.rp <= 64)
-        lora_many_y<T, VA, 4>(P, st);
+        lora_many_y<T, 4>(P, st);
     else if (P.rp <= 128)
-        lora_many_y<T, VA, 8>(P, st);
+        lora_many_y<T, 8>(P, st);
     else
-        lora_many_y<T, VA, 16>(P, st);
-}
-template <typename T, bool VB>
-static void lora_many_out(const LoraParams &P, bool ovec, hipStream_t st) {
+        lora_many_y<T, 16>(P, st);
     const dim3 g((P.rows + LORA_OUT - 1) / LORA_OUT, (P.n + LORA_BLOCK - 1) / LORA_BLOCK);
-    if (ovec)
-        hipLaunchKernelGGL((lora_many_out_kernel<T, VB, true>), g, dim3(64 * LORA_OW), 0, st, P);
-    else
-        hipLaunchKernelGGL((lora_many_out_kernel<T, VB, false>), g, dim3(64 * LORA_OW), 0, st, P);
+    hipLaunchKernelGGL((lora_many_out_kernel<T>), g, dim3(64 * LORA_OW), 0, st, P);
 }
 
 // Whether the vectors are taken one by one: while all their reads of A_e and B_e, mostly from L2, stay under LORA_FEW
@@ -651,43 +639,17 @@ template <class L>
 static bool lora_is_one(const L &l, size_t n, size_t es) {
     return lora_is_few(l, n, es) && l.rank <= 64 && l.rank * l.cols * es <= LORA_SMALL;
 }
-// Loads of four elements where rows and pointers allow them: A_e's rows and x for the first launch, B_e's for the
-// second (base and out beside them where many vectors are tiles).  Returns the launches.
+// Returns the launches.
 template <typename T>
 static int lora_run(const LoraParams &P, hipStream_t st) {
-    const size_t q = 4 * sizeof(T);
-    const bool va = P.cols % 4 == 0 && (uintptr_t)P.a % q == 0 && (uintptr_t)P.x % 16 == 0 && P.x_stride % 4 == 0;
-    const bool vb = P.rank % 4 == 0 && (uintptr_t)P.b % q == 0;
-    const bool ovec = P.rows % 4 == 0 && (uintptr_t)P.out % 16 == 0 && P.out_stride % 4 == 0 &&
-                      (!P.base || ((uintptr_t)P.base % 16 == 0 && P.base_stride % 4 == 0));
-    if (lora_is_few(P, P.n, sizeof(T))) {
-        const bool va8 = va && P.cols % 8 == 0 && (uintptr_t)P.a % 16 == 0;
-        const bool vb8 = P.rank % 8 == 0 && (uintptr_t)P.b % 16 == 0;
-        if (lora_is_one(P, P.n, sizeof(T))) {
-            if (va8 && vb8)
-                lora_one<T, true>(P, st);
-            else
-                lora_one<T, false>(P, st);
-            return 1;
-        }
-        if (va8 && vb8)
-            lora_few<T, true, true>(P, st);
-        else if (va8)
-            lora_few<T, true, false>(P, st);
-        else if (vb8)
-            lora_few<T, false, true>(P, st);
-        else
-            lora_few<T, false, false>(P, st);
-        return 2;
+    if (lora_is_one(P, P.n, sizeof(T))) {
+        lora_both<T>(P, st);
+        return 1;
     }
-    if (va)
-        lora_many_y<T, true>(P, st);
+    if (lora_is_few(P, P.n, sizeof(T)))
+        lora_few<T>(P, st);
     else
-        lora_many_y<T, false>(P, st);
-    if (vb)
-        lora_many_out<T, true>(P, ovec, st);
-    else
-        lora_many_out<T, false>(P, ovec, st);
+        lora_many<T>(P, st);
     return 2;
 }
 
