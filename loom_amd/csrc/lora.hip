@@ -357,91 +357,63 @@ __global__ __launch_bounds__(LORA_ONE) void lora_one_kernel(LoraParams P) {
 }
 
 // ---- many vectors -----------------------------------------------------------------
-// Tiles of v_mfma_f32_16x16x4_f32 with 16 vectors as columns: lane l has column l % 16 and, of four contracted indices,
-// l / 16; four products take 16 indices, lane group g those 4 g .. 4 g + 3, which both operands read as one load.  The
-// result: column l % 16, rows 4 (l / 16) + i.
+// Tiles of v_mfma_f32_16x16x4_f32 with 16 vectors as columns: lane l has column l % 16 and one of four contracted
+// indices, l / 16.  Which four a product takes is free as long as both operands agree: lane group g has those of its 16
+// bytes.  The result: column l % 16, rows 4 (l / 16) + i.
 
-// The vectors of a block of LORA_BLOCK, put together by adapter: tiles of up to 16 vectors that name one (or none).
-// Where a request's tokens follow one another the runs of one adapter are cut into tiles as they stand (a vector's place
-// follows from two ballots).  Where that gives more than half as many tiles again as 16 in each, every vector finds its
-// place by comparing its adapter with the block's others.
+// The vectors of a block of LORA_BLOCK that name an adapter, put together by it: tiles of up to 16 vectors that name one.
+// Which vectors share an adapter follows from a ballot for each bit of its number, where its tiles begin from a scan.
 constexpr int LORA_BLOCK = 128;
 struct LoraTiles {
-    int key[LORA_BLOCK], count[LORA_BLOCK]; // of each vector its adapter, -1: none; of an adapter's first one its tiles
+    int key[LORA_BLOCK], first[LORA_BLOCK]; // of each vector its adapter (-1: none); of an adapter's first one its first tile
     int adapter[LORA_BLOCK];                // of each tile
     short vec[LORA_BLOCK][16];              // of each tile its vectors, -1 past the last
-    unsigned long long starts[2];           // of runs, then of tiles
+    int total[2];                           // tiles whose adapter's first vector is in each half
 };
 __device__ __forceinline__ int lora_tiles(const LoraParams &P, size_t t0, LoraTiles &L) {
     static_assert(LORA_BLOCK == 128, "two waves");
     const int i = threadIdx.x, wave = i >> 6, lane = i & 63;
     const int here = P.n - t0 < LORA_BLOCK ? (int)(P.n - t0) : LORA_BLOCK;
-    int key = -2; // past the last vector: nobody's
     if (i < LORA_BLOCK) {
-        if (i < here) {
-            key = P.ids[t0 + i];
-            key = lora_names(P, key) ? key : -1;
-        }
-        L.key[i] = key;
+        const int id = i < here ? P.ids[t0 + i] : -1;
+        L.key[i] = lora_names(P, id) ? id : -1;
     }
     for (int c = i; c < LORA_BLOCK * 8; c += blockDim.x)
         ((int *)&L.vec[0][0])[c] = -1;
     __syncthreads();
-    const bool in = i < here;
-    // The newest set bit at or before vector i, and how many there are up to it.
-    const unsigned long long upto = ~0ull >> (63 - lane);
+    int key = -1, before = 0, lead = 0;
     if (wave < 2) {
-        const unsigned long long s = __ballot(in && (i == 0 || L.key[i - 1] != key));
-        if (lane == 0)
-            L.starts[wave] = s;
-    }
-    __syncthreads();
-    int at = 0;
-    if (wave < 2) {
-        const unsigned long long mine = L.starts[wave] & upto;
-        at = i - (mine ? wave * 64 + 63 - __builtin_clzll(mine) : 63 - __builtin_clzll(L.starts[0]));
-    }
-    __syncthreads();
-    if (wave < 2) {
-        const unsigned long long s = __ballot(in && at % 16 == 0);
-        if (lane == 0)
-            L.starts[wave] = s;
-    }
-    __syncthreads();
-    int n = __popcll(L.starts[0]) + __popcll(L.starts[1]);
-    int tile = 0;
-    if (wave < 2)
-        tile = __popcll(L.starts[wave] & upto) - 1 + (wave ? __popcll(L.starts[0]) : 0);
-    if (n > (here + 15) / 16 + LORA_BLOCK / 32) {
-        const int4 *keys = (const int4 *)L.key, *counts = (const int4 *)L.count;
-        int before = 0, same = 0; // vectors of the same adapter in front, and all
-        if (i < LORA_BLOCK) {
-#pragma unroll 4
-            for (int j = 0; j < LORA_BLOCK / 4; j++) {
-                const int4 k = keys[j];
-                const int m = (k.x == key) | (k.y == key) << 1 | (k.z == key) << 2 | (k.w == key) << 3;
-                same += __popc(m);
-                before += __popc(4 * j + 4 <= i ? m : 4 * j < i ? m & ((1 << (i - 4 * j)) - 1) : 0);
-            }
-            L.count[i] = in && before == 0 ? (same + 15) / 16 : 0;
+        const int k0 = L.key[lane], k1 = L.key[64 + lane];
+        key = wave ? k1 : k0;
+        // the vectors of each half that name the same adapter, bit by bit of its number
+        unsigned long long m0 = __ballot(k0 >= 0), m1 = __ballot(k1 >= 0);
+        for (int bit = 0; (P.n_adapters - 1) >> bit; bit++) {
+            const unsigned long long b0 = __ballot(k0 >> bit & 1), b1 = __ballot(k1 >> bit & 1);
+            const unsigned long long flip = key >> bit & 1 ? 0 : ~0ull;
+            m0 &= b0 ^ flip;
+            m1 &= b1 ^ flip;
         }
-        __syncthreads();
-        tile = n = 0;
-        at = before;
-#pragma unroll 4
-        for (int j = 0; j < LORA_BLOCK / 4; j++) {
-            const int4 k = keys[j], c = counts[j];
-            tile += (k.x < key ? c.x : 0) + (k.y < key ? c.y : 0) + (k.z < key ? c.z : 0) + (k.w < key ? c.w : 0);
-            n += c.x + c.y + c.z + c.w;
+        const unsigned long long under = (1ull << lane) - 1;
+        before = wave ? __popcll(m0) + __popcll(m1 & under) : __popcll(m0 & under);
+        lead = m0 ? __builtin_ctzll(m0) : m1 ? 64 + __builtin_ctzll(m1) : 0;
+        const int mine = key >= 0 && before == 0 ? (__popcll(m0) + __popcll(m1) + 15) / 16 : 0;
+        int sum = mine; // up to and with this vector's
+        for (int o = 1; o < 64; o *= 2) {
+            const int up = __shfl_up(sum, o);
+            sum += lane >= o ? up : 0;
         }
-        tile += before / 16;
+        L.first[i] = sum - mine;
+        if (lane == 63)
+            L.total[wave] = sum;
     }
-    if (in) {
-        L.vec[tile][at % 16] = (short)i;
+    __syncthreads();
+    if (wave < 2 && key >= 0) {
+        const int tile = L.first[lead] + (lead < 64 ? 0 : L.total[0]) + before / 16;
+        L.vec[tile][before % 16] = (short)i;
         L.adapter[tile] = key;
     }
     __syncthreads();
-    return n;
+    return L.total[0] + L.total[1];
 }
 
 // y for every LORA_Z-th tile of a block and one of ks splits of the columns: W waves take an equal part each, their sums
@@ -470,8 +442,6 @@ __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(Lora
     const size_t k0 = (blockIdx.z * W + wave) * share, k1 = k0 + share < P.cols ? k0 + share : P.cols;
     for (int tile = blockIdx.y; tile < tiles; tile += LORA_Z) {
         const int e = L.adapter[tile];
-        if (e < 0)
-            continue;
         const T *a = (const T *)P.a + (size_t)e * P.rank * P.cols;
         const float *x[XL];
         const T *ar[RT][2];
@@ -609,8 +579,6 @@ __global__ __launch_bounds__(64 * LORA_OW, 4) void lora_many_out_kernel(LoraPara
             }
             for (int tile = wave; tile < tiles; tile += LORA_OW) {
                 const int e = L.adapter[tile], v = L.vec[tile][col];
-                if (e < 0)
-                    continue;
                 const T *b = (const T *)P.b + (size_t)e * P.rows * P.rank;
                 const float *y = ys + (v < 0 ? L.vec[tile][0] : v) * LORA_OUT_PAD;
                 lora_f4 acc[MT];
@@ -740,8 +708,8 @@ static void lora_many(const LoraParams &P, hipStream_t st) {
 }
 
 // Whether the vectors are taken one by one: while all their reads of A_e and B_e, mostly from L2, stay under LORA_FEW
-// bytes.  Measured at 4096 x 2048, rank 64, fp16: 101 MB (128 vectors) 17 us one by one, 21 as tiles, 41 as tiles of
-// mixed requests; 201 MB 29, 21, 42; 403 MB 52, 22, 45.
+// bytes.  Measured at 4096 x 2048, rank 64, fp16: 101 MB (128 vectors) 17 us one by one, 20 as tiles, 28 as tiles of
+// mixed requests; 201 MB 29, 21, 28; 403 MB 53, 23, 32.
 template <class L>
 static bool lora_is_few(const L &l, size_t n, size_t es) {
     return n <= 65535 && (double)n * l.rank * (l.rows + l.cols) * es <= LORA_FEW;
