@@ -23,6 +23,13 @@
 // operand's lane then needs 4 + 4 consecutive keys of one value column, which
 // the LDS transpose read (ds_read_b64_tr_b16) gives from row-major values.
 // The softmax of a query needs one exchange between the two half waves.
+//
+// Measured, heads of 128, 32 over 4 key heads: 190 query tokens of 64 lanes
+// against 16384 shared and up to 640 own rows 114 us (128 at the clock that
+// sustained matrix work leaves), bound by the matrix cores (104 GFLOP in
+// two-part products, 910 TFLOP/s of the 1001 a large library product reaches),
+// the merge 9; 32 lanes of one token against 4096 and 512 rows 19.5 us
+// (27 MB), one round of short ranges, the merge 6.
 #include "runtime.hpp"
 #include <cmath>
 #include <type_traits>
