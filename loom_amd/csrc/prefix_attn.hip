@@ -676,7 +676,7 @@ __host__ __device__ inline float pa_cost(int rows, int s, int x, int room, float
     const int len = pa_split_len(rows, s);
     if ((int64_t)(s - 1) * len >= rows)
         return __builtin_inff();
-    return (float)((x * s + room - 1) / room) * (PA_ITEM + (float)(len / 64)) + PA_RECORD * (float)s * records;
+    return (float)(((uint32_t)x * s + room - 1) / room) * (PA_ITEM + (float)(len / 64)) + PA_RECORD * (float)s * records;
 }
 __device__ __forceinline__ int pa_pre_cut(const PrefixAttnParams &P, int blocks, int block_rows) {
     const int s = (threadIdx.x & 63) + 1, x = P.n_kv * blocks;
