@@ -806,7 +806,7 @@ typedef struct {
  * reads key head h / (n_heads / n_kv_heads)):
  *   out = sum_t p_t v_t,  p = softmax over the row's t of scale * (q . k_t),
  * zero where a row sees nothing.  out rows j >= q_len[i] are left as they
- * were.  own_len and q_len are clamped into [0, own->rows] and [0, n_q]; rows
+ * were, or set to zero if zero_rest is not 0.  own_len and q_len are clamped into [0, own->rows] and [0, n_q]; rows
  * of the cache past a query's own are not part of its result, whatever they
  * hold (a cached NaN or infinity makes the rows that see it NaN).
  * prefix->rows or own->rows may be 0 (no rows; pointers unused).
@@ -815,8 +815,8 @@ typedef struct {
  * 4096; DECLINED otherwise. */
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
                             const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,
-                            size_t n_kv_heads, size_t head_dim, float scale, float *out, void *ws, size_t ws_bytes,
-                            void *stream);
+                            size_t n_kv_heads, size_t head_dim, float scale, float *out, int zero_rest, void *ws,
+                            size_t ws_bytes, void *stream);
 size_t loomhip_prefix_attn_ws(size_t prefix_rows, size_t own_rows, size_t n, size_t n_q, size_t n_heads,
                               size_t n_kv_heads, size_t head_dim);
 

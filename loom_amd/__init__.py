@@ -378,7 +378,7 @@ def lib() -> C.CDLL:
         "loomhip_mla_layer_cached_dev": (i, [C.POINTER(MlaAttnDesc), C.POINTER(vp), C.POINTER(vp), sz, sz, vp, vp, i,
                                              vp, vp, f, C.POINTER(MoeLayerEcDesc), vp, vp, vp, vp]),
         "loomhip_prefix_attn_dev": (i, [C.POINTER(KvRowsDesc), C.POINTER(KvRowsDesc), vp, vp, vp, sz, sz, sz, sz, sz,
-                                        f, vp, vp, sz, vp]),
+                                        f, vp, i, vp, sz, vp]),
         "loomhip_prefix_attn_ws": (sz, [sz, sz, sz, sz, sz, sz, sz]),
         "loomhip_lora_dev": (i, [C.POINTER(LoraDesc), vp, sz, vp, vp, sz, sz, vp, sz, vp, sz, vp]),
         "loomhip_lora_ws": (sz, [C.POINTER(LoraDesc), sz]),

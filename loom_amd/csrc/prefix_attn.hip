@@ -59,6 +59,7 @@ struct PrefixAttnParams {
     int n, n_q, n_heads, n_kv, hd;
     float scale;
     float *out;
+    bool zero_rest; // rows past q_len
     // Items: prefix [kv][split][row block], then own [lane][kv][split][row block].  The prefix's split count depends on
     // how many rows the lanes have (q_len is on the device): pa_pre_cut's, at most pre_splits, left in *cut.
     int pre_splits, pre_items, xcd_slots;
@@ -755,8 +756,11 @@ __global__ __launch_bounds__(PA_THREADS) void prefix_attn_merge_kernel(PrefixAtt
     if (row >= rows)
         return;
     const int token = row / P.n_heads, i = token / P.n_q, j = token % P.n_q;
-    if (j >= pa_q_len(P, i))
+    if (j >= pa_q_len(P, i)) {
+        if (P.zero_rest && lane * 4 < P.hd)
+            *(pa_f4 *)(P.out + (size_t)row * P.hd + lane * 4) = pa_f4{0.0f, 0.0f, 0.0f, 0.0f};
         return;
+    }
     const int len = pa_own_len(P, i);
     // the slots that were written: the own splits that start below the lane's length, and the prefix's
     const int own = P.own_splits ? (len + P.own_len_split - 1) / P.own_len_split : 0;
@@ -906,8 +910,8 @@ size_t loomhip_prefix_attn_ws(size_t prefix_rows, size_t own_rows, size_t n, siz
 
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
                             const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,
-                            size_t n_kv_heads, size_t head_dim, float scale, float *out, void *ws, size_t ws_bytes,
-                            void *stream) {
+                            size_t n_kv_heads, size_t head_dim, float scale, float *out, int zero_rest, void *ws,
+                            size_t ws_bytes, void *stream) {
     if (n == 0 || n_q == 0)
         return LOOMHIP_OK;
     if (!q || !out || n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads)
@@ -950,6 +954,7 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
     P.hd = (int)head_dim;
     P.scale = scale;
     P.out = out;
+    P.zero_rest = zero_rest != 0;
     P.pre_splits = p.pre_splits;
     P.pre_items = p.pre_items;
     P.xcd_slots = p.xcd_slots;

@@ -118,15 +118,17 @@ def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, 
         if t is not None and (t.dtype is not _I32 or t.shape != (n,) or not t.is_contiguous()):
             raise ValueError("own_len, q_len: int32 [n]")
     dev, stream = _place(q, k_prefix, v_prefix, k_own, v_own, own_len, q_len, out)
-    if out is None:
-        out = torch.empty_like(q) if q_len is None else torch.zeros_like(q)
+    fresh = out is None
+    if fresh:
+        out = torch.empty_like(q)
     elif out.shape != shape or out.dtype is not _F32 or not out.is_contiguous():
         raise ValueError("out: as q")
     nb = _attn_ws(pre.rows, own.rows, n, n_q, heads, kv, hd)
     ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
     rc = lib().loomhip_prefix_attn_dev(
         C.byref(pre), C.byref(own), q.data_ptr(), None if own_len is None else own_len.data_ptr(),
-        None if q_len is None else q_len.data_ptr(), n, n_q, heads, kv, hd, scale, out.data_ptr(), ws.data_ptr() if nb else None, nb, stream)
+        None if q_len is None else q_len.data_ptr(), n, n_q, heads, kv, hd, scale, out.data_ptr(), fresh,
+        ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
         _fail("prefix_attn_dev", rc)
     return out

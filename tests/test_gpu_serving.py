@@ -180,6 +180,21 @@ def test_prefix_attn_rows_behind_hold_anything(sv, bad, hd):
             assert np.isnan(got[i, L - 1]).all()
 
 
+@pytest.mark.parametrize("hd", [8, 48, 200, 256])
+def test_prefix_attn_zeroes_the_rest_of_its_own_output(sv, hd):
+    """Rows past q_len of an out made here, over memory that held something else."""
+    import torch
+
+    c = _attn_case(4, 2, hd, 33, 9, 3, 12)
+    c["q_len"] = np.array([0, 1, 2, 3, 0, 1, 2, 3, 1], np.int32)
+    want, bound = _attn_ref(c)
+    for _ in range(3):
+        torch.full((9, 3, 4, hd), float("nan"), device="cuda")  # freed: the next output's memory
+        got = _attn(sv, c).cpu().numpy()
+        _within(got, want, bound)
+        assert (got[np.isnan(want)] == 0).all() and np.isnan(want).any()
+
+
 def test_prefix_attn_one_bad_lane_stays_alone(sv):
     c = _attn_case(8, 2, 64, 90, 6, 2, 33)
     c["own_len"][:] = 33

@@ -16,7 +16,7 @@ def _attn(prefix=None, own=None, q=FAKE, own_len=FAKE, q_len=None, n=2, n_q=1, h
     L = loom_amd.lib()
     pre = loom_amd.KvRowsDesc(*(prefix or (FAKE, FAKE, 16, 0, 128, 64)))
     mine = loom_amd.KvRowsDesc(*(own or (FAKE, FAKE, 8, 1024, 128, 64)))
-    return L.loomhip_prefix_attn_dev(C.byref(pre), C.byref(mine), q, own_len, q_len, n, n_q, heads, kv, hd, 0.125, out, ws,
+    return L.loomhip_prefix_attn_dev(C.byref(pre), C.byref(mine), q, own_len, q_len, n, n_q, heads, kv, hd, 0.125, out, 0, ws,
                                      ws_bytes, None)
 
 
