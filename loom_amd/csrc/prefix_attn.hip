@@ -841,7 +841,7 @@ static PaPlan pa_plan(size_t prefix_rows, size_t own_rows, size_t n, size_t n_q,
             p.pre_splits = 2 * s + 2 < 64 ? 2 * s + 2 : 64;
             p.pre_splits = p.pre_splits > most ? most : p.pre_splits;
         }
-        const int64_t cap = (int64_t)pre_x * s > slots ? (int64_t)pre_x * s : slots;
+        const int64_t x = (int64_t)pre_x * s, cap = ragged && x < slots ? slots : x;
         p.pre_items = (int)((cap + 7) / 8 * 8);
     }
     p.slots = p.pre_splits + p.own_splits;
