@@ -28,8 +28,8 @@
 // against 16384 shared and up to 640 own rows 114 us (128 at the clock that
 // sustained matrix work leaves), bound by the matrix cores (104 GFLOP in
 // two-part products, 910 TFLOP/s of the 1001 a large library product reaches),
-// the merge 9; 32 lanes of one token against 4096 and 512 rows 19.5 us
-// (27 MB), one round of short ranges, the merge 6.
+// the merge 9; 32 lanes of one token against 4096 and 512 rows 20 us
+// (27 MB), one round of short ranges, the merge 4.5.
 #include "runtime.hpp"
 #include <cmath>
 #include <type_traits>
