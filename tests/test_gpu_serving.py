@@ -716,7 +716,7 @@ def _step(sv, s):
     return q, o, p, t, a
 
 
-def _step_inputs(n=6, nq=4, vocab=3001, seed=1):
+def _step_inputs(n=6, nq=4, vocab=3001, rank=16, seed=1):
     import torch
 
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -727,17 +727,21 @@ def _step_inputs(n=6, nq=4, vocab=3001, seed=1):
     def i(hi, *shape):
         return torch.randint(0, hi, shape, generator=g, device="cuda", dtype=torch.int32)
 
-    return {"n": n, "nq": nq, "x": f(n * nq, 256), "base": f(n * nq, 512), "a": (f(5, 16, 256) / 16).half(),
-            "b": (f(5, 512, 16) / 4).half(), "scale": torch.ones(5, device="cuda"), "ids": i(6, n * nq) - 1,
+    return {"n": n, "nq": nq, "x": f(n * nq, 256), "base": f(n * nq, 512), "a": (f(5, rank, 256) / 16).half(),
+            "b": (f(5, 512, rank) / rank ** 0.5).half(), "scale": torch.ones(5, device="cuda"), "ids": i(6, n * nq) - 1,
             "kp": f(300, 2, 64).half(), "vp": f(300, 2, 64).half(), "ko": f(n, 50, 2, 64).half(), "vo": f(n, 50, 2, 64).half(),
             "own_len": i(47, n) + 4, "q_len": i(nq, n) + 1, "head": f(vocab) * 9, "at": i(512, vocab).long(), "temp": torch.full((n * nq,), 0.7, device="cuda"),
             "tok": i(vocab, n, nq - 1), "ua": torch.rand((n, nq - 1), generator=g, device="cuda") * 1e-4,
             "us": torch.rand((n,), generator=g, device="cuda")}
 
 
-def test_a_step_of_all_operators(sv):
+FORMS = pytest.mark.parametrize("vocab,rank", [(3001, 16), (33001, 128)])  # one launch a call, and two
+
+
+@FORMS
+def test_a_step_of_all_operators(sv, vocab, rank):
     """The four together, each stage held to its definition on the stage before's output."""
-    s = _step_inputs()
+    s = _step_inputs(vocab=vocab, rank=rank)
     q, o, p, t, a = _step(sv, s)
     h = {k: (v.float() if v.is_floating_point() else v).cpu().numpy() for k, v in s.items() if hasattr(v, "cpu")}
     want, bound = ref.lora(h["x"], h["a"], h["b"], h["scale"], h["ids"], h["base"])
@@ -770,20 +774,23 @@ def test_beside_a_quantized_projection(sv):
     assert bool((out[t["ids"] < 0] == t["base"][t["ids"] < 0]).all())
 
 
-def test_repeated_calls_give_the_same_bits(sv):
-    s = _step_inputs(n=33, nq=3)
+@FORMS
+def test_repeated_calls_give_the_same_bits(sv, vocab, rank):
+    s = _step_inputs(n=33, nq=3, vocab=vocab, rank=rank)
     first = _step(sv, s)
     for _ in range(3):
         for x, y in zip(first, _step(sv, s)):
             assert bool((x == y).all())
 
 
-def test_captured_steps_replay(sv):
+@FORMS
+def test_captured_steps_replay(sv, vocab, rank):
     """Two captured graphs of the step, replayed in turn on inputs that change in place, with eager calls and other
     allocations between the replays: each replay equals the eager result."""
     import torch
 
-    a, b = _step_inputs(), _step_inputs(n=3, nq=2, seed=9)
+    form = {"vocab": vocab, "rank": rank}
+    a, b = _step_inputs(**form), _step_inputs(n=3, nq=2, seed=9, **form)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -797,7 +804,8 @@ def test_captured_steps_replay(sv):
         with torch.cuda.graph(g):
             out = _step(sv, s)
         graphs.append((g, out, s))
-    fresh = [_step_inputs(seed=20 + k) for k in range(3)], [_step_inputs(n=3, nq=2, seed=30 + k) for k in range(3)]
+    fresh = ([_step_inputs(seed=20 + k, **form) for k in range(3)],
+             [_step_inputs(n=3, nq=2, seed=30 + k, **form) for k in range(3)])
     for k in range(3):
         for (g, out, s), new in zip(graphs, fresh):
             for key in ("x", "ids", "own_len", "q_len", "us", "ua", "tok"):
@@ -812,10 +820,11 @@ def test_captured_steps_replay(sv):
                 assert bool((x == y).all()), k
 
 
-def test_steps_on_two_streams(sv):
+@FORMS
+def test_steps_on_two_streams(sv, vocab, rank):
     import torch
 
-    sets = [_step_inputs(n=20, nq=3, seed=k) for k in (1, 2)]
+    sets = [_step_inputs(n=20, nq=3, vocab=vocab, rank=rank, seed=k) for k in (1, 2)]
     want = [_step(sv, s) for s in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in sets]
@@ -831,12 +840,13 @@ def test_steps_on_two_streams(sv):
                 assert bool((x == y).all())
 
 
-def test_calls_from_two_threads(sv):
+@FORMS
+def test_calls_from_two_threads(sv, vocab, rank):
     import threading
 
     import torch
 
-    sets = [_step_inputs(n=20, nq=3, seed=k) for k in (3, 4)]
+    sets = [_step_inputs(n=20, nq=3, vocab=vocab, rank=rank, seed=k) for k in (3, 4)]
     want = [_step(sv, s) for s in sets]
     torch.cuda.synchronize()
     got, errors = [None, None], []
