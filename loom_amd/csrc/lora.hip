@@ -417,11 +417,11 @@ __device__ __forceinline__ int lora_tiles(const LoraParams &P, size_t t0, LoraTi
 }
 
 // y for every LORA_Z-th tile of a block and one of ks splits of the columns: W waves take an equal part each, their sums
-// meet in LDS.  The second launch adds the splits, once for every 64 rows, so there are as few as fill the chip.  RT: tiles
+// meet in LDS.  The second launch adds the splits, once a work group, so there are as few as fill the chip.  RT: tiles
 // of 16 ranks.  A wave reads 128 bytes of every row of A_e and the same columns of x at a time, whole cache lines in one
 // instruction, and gives them their places through a piece of LDS of its own: loaded as the products want them, 16 rows a
 // quarter line each, rows a power of two apart throw each other's lines out of the cache (4096 columns, rank 64, 1408
-// vectors: 41 us).
+// vectors: 41 us for 27 this way).
 constexpr int LORA_Z = LORA_BLOCK / 16;
 __host__ __device__ constexpr int lora_y_waves(int rt) { return rt <= 8 ? 8 : 4; }
 template <typename T, int RT>
