@@ -843,7 +843,9 @@ size_t loomhip_lora_ws(const loomhip_lora *l, size_t n);
  * `vocab` values (temperature f32 [n] or NULL: 1), rows at the given strides;
  * probs may be logits itself with the same stride.  A temperature that is
  * not positive (or so small that 1/T passes f32) gives 1 at the first maximum
- * and 0 elsewhere, the frame's greedy pick.  A row of -inf alone gives zeros.
+ * and 0 elsewhere, the frame's greedy pick (NaN logits passed over; at any
+ * other temperature they make the row NaN).  A row of -inf alone gives zeros,
+ * and so does a greedy one of -inf and NaN.
  * n up to 65535 rows; DECLINED otherwise. */
 int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const float *temperature,
                             float *probs, size_t out_stride, void *ws, size_t ws_bytes, void *stream);

@@ -50,7 +50,8 @@ __device__ __forceinline__ void row_part(const float *x, size_t v0, size_t vocab
 // a work group can hold takes one launch; a longer one two: each (row, split)
 // reduces its values to (max, sum of exponentials, first index of the max);
 // then each (row, split) merges the row's records and writes its probabilities.
-// T not positive, NaN or so small that 1/T passes f32: 1 at the first maximum.
+// T not positive, NaN or so small that 1/T passes f32: 1 at the first maximum
+// among the numbers (a NaN logit makes a row of any other T NaN).
 // Bound by bytes: 160 rows of 151936 take 25 us for the sums (3.9 TB/s) and 31
 // for the second read, mostly from the last-level cache, and the write.
 struct ProbRec {
@@ -81,8 +82,8 @@ __device__ __forceinline__ ProbScale prob_scale(const float *temperature, size_t
 }
 
 __device__ __forceinline__ void max_first(float &m, int &at, float m2, int at2) {
-    // the larger value; of equal ones the lower index; a NaN stays
-    const bool take = m2 > m || (m2 == m && at2 < at) || (m2 != m2 && (m == m || at2 < at));
+    // the larger value; of equal ones the lower index; a NaN is never taken
+    const bool take = m2 > m || (m2 == m && at2 < at);
     m = take ? m2 : m;
     at = take ? at2 : at;
 }
@@ -115,13 +116,13 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *
     m = sm[0], at = sa[0];
     for (int w = 1; w < SMP_THREADS / 64; w++)
         max_first(m, at, sm[w], sa[w]);
+    const float from = m == -__builtin_inff() ? 0.0f : m; // nothing above -inf: zeros, or the NaN among them
     float l = 0.0f;
-    if (m != -__builtin_inff())
 #pragma unroll
-        for (int i = 0; i < NV; i++)
+    for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                l += exp_scaled(v[i][c] - m, sc.hi, sc.lo);
+        for (int c = 0; c < 4; c++)
+            l += exp_scaled(v[i][c] - from, sc.hi, sc.lo);
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
     if (lane == 0)
@@ -159,20 +160,21 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *_
     float l = 0.0f;
     for (int s = lane; s < splits; s += 64) {
         const ProbRec r = rec[row * splits + s];
-        l += r.m == -__builtin_inff() ? 0.0f : r.l * exp_scaled(r.m - m, sc.hi, sc.lo);
+        l += r.m == -__builtin_inff() ? r.l : r.l * exp_scaled(r.m - m, sc.hi, sc.lo);
     }
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
-    const float inv = 1.0f / l;
-    const bool none = m == -__builtin_inff(); // every logit is -inf: no token has a probability
+    // nothing above -inf: no token has a probability, zeros (NaN by l where there is one among them)
+    const float inv = l == 0.0f ? 1.0f : 1.0f / l;
+    at = m == -__builtin_inff() ? -1 : at;
+    m = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const size_t k = v0 + ((size_t)i * SMP_THREADS + tid) * 4;
         smp_f4 e;
 #pragma unroll
         for (int c = 0; c < 4; c++)
-            e[c] = none ? 0.0f
-                   : sc.greedy ? (k + c == (size_t)at ? 1.0f : 0.0f) : exp_scaled(v[i][c] - m, sc.hi, sc.lo) * inv;
+            e[c] = sc.greedy ? ((int64_t)(k + c) == at ? 1.0f : 0.0f) : exp_scaled(v[i][c] - m, sc.hi, sc.lo) * inv;
         if (k + 4 <= vocab) {
             __builtin_nontemporal_store(e, (smp_f4u *)(p + k));
         } else {
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(THREADS) void probs_row_kernel(const float *__restr
         m = sm[lane % W], at = sa[lane % W];
         for (int o = 1; o < W; o *= 2)
             max_first(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
-        at = m == -__builtin_inff() ? -1 : at; // every logit is -inf: no token has a probability
+        at = m == -__builtin_inff() ? -1 : at; // nothing above -inf: no token has a probability
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
