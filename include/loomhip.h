@@ -844,7 +844,8 @@ size_t loomhip_lora_ws(const loomhip_lora *l, size_t n);
  * probs may be logits itself with the same stride.  A temperature that is
  * not positive (or so small that 1/T passes f32) gives 1 at the first maximum
  * and 0 elsewhere, the frame's greedy pick (NaN logits passed over; at any
- * other temperature they make the row NaN).  A row of -inf alone gives zeros,
+ * other temperature they make the row NaN); an infinite one weighs finite
+ * logits alike and -inf as nothing.  A row of -inf alone gives zeros,
  * and so does a greedy one of -inf and NaN.
  * n up to 65535 rows; DECLINED otherwise. */
 int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const float *temperature,

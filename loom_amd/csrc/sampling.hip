@@ -50,6 +50,7 @@ __device__ __forceinline__ void row_part(const float *x, size_t v0, size_t vocab
 // a work group can hold takes one launch; a longer one two: each (row, split)
 // reduces its values to (max, sum of exponentials, first index of the max);
 // then each (row, split) merges the row's records and writes its probabilities.
+// T infinite: finite logits weigh alike, -inf still nothing.
 // T not positive, NaN or so small that 1/T passes f32: 1 at the first maximum
 // among the numbers (a NaN logit makes a row of any other T NaN).
 // Bound by bytes: 160 rows of 151936 take 25 us for the sums (3.9 TB/s) and 31
@@ -77,7 +78,8 @@ struct ProbScale {
 __device__ __forceinline__ ProbScale prob_scale(const float *temperature, size_t row) {
     const float t = temperature ? temperature[row] : 1.0f;
     const double c = 0x1.71547652b82fep+0 / (double)t;
-    const float hi = (float)c;
+    // an infinite T weighs finite logits alike: the smallest factor there is, not 0, which times a masked -inf is NaN
+    const float hi = (float)c == 0.0f ? 0x1p-149f : (float)c;
     return {hi, (float)(c - (double)hi), !(t > 0.0f) || !(hi < __builtin_inff())};
 }
 

@@ -37,3 +37,18 @@ def test_token_probs_rows_with_nan(sv, vocab):
     assert np.isnan(got[5:8]).all()
     w, bound = ref.token_probs(x[8:], t[8:])
     _within(got[8:], w, bound)
+
+
+@pytest.mark.parametrize("vocab", [700, 4096, 4097, 20000, 40001, 40960])
+def test_token_probs_infinite_temperature(sv, vocab):
+    """Every finite logit alike, a masked one still nothing; whatever the vocabulary leaves of its last part."""
+    x = (_rng(4, vocab).standard_normal((3, vocab)) * 50).astype(np.float32)
+    x[1, vocab // 3:] = -np.inf
+    x[2, 1::2] = np.finfo(np.float32).min
+    got = sv.token_probs_dev(_dev(x), _dev(np.full(3, np.inf, np.float32))).cpu().numpy().astype(np.float64)
+    live = np.isfinite(x)
+    want = live / live.sum(1, keepdims=True)
+    # exponentials of exactly 1 and their sum, a whole number below 2^24; the division and the last product round.  The
+    # exponent of a logit 2^128 below the others is held to 2^-20 of its share.
+    bound = want * (2 * ref.EPS + np.array([0.0, 0.0, 2.0 ** -19])[:, None])
+    _within(got, want, bound)
