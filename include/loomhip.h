@@ -808,7 +808,10 @@ typedef struct {
  * zero where a row sees nothing.  out rows j >= q_len[i] are left as they
  * were, or set to zero if zero_rest is not 0.  own_len and q_len are clamped into [0, own->rows] and [0, n_q]; rows
  * of the cache past a query's own are not part of its result, whatever they
- * hold (a cached NaN or infinity makes the rows that see it NaN).
+ * hold.  For the rows that see it, a value that is NaN or infinite makes its
+ * element of the result NaN, a key with a NaN all of it, and a key with an
+ * infinity too, unless its score is minus infinity: then it may also count as
+ * a row not seen.
  * prefix->rows or own->rows may be 0 (no rows; pointers unused).
  * head_dim a multiple of 8 up to 256, strides multiples of 8 (rows at most
  * 2^23 apart), pointers at a multiple of 16 bytes, n up to 65535, n_q up to

@@ -793,8 +793,11 @@ __global__ __launch_bounds__(PA_THREADS) void prefix_attn_merge_kernel(PrefixAtt
             o[e] += __shfl_xor(o[e], x);
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l; // nothing seen: zero
+    // An infinity here comes from a cached one, which the weights' low parts (0, or below it) turn into NaN in some rows
+    // and not in others: NaN in all.  Zero times anything finite adds nothing.
+    o *= inv;
     if (g == 0 && d < P.hd)
-        *(pa_f4 *)(P.out + (size_t)row * P.hd + d) = o * inv;
+        *(pa_f4 *)(P.out + (size_t)row * P.hd + d) = o + o * 0.0f;
 }
 
 // How a call is cut into items.

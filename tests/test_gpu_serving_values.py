@@ -1,10 +1,10 @@
 """The batched serving operators on the device at values and layouts beside the
-ordinary: no number among the logits of a greedy row."""
+ordinary: no number among the logits or in the caches, an infinite temperature."""
 import numpy as np
 import pytest
 
 import serving_ref as ref
-from test_gpu_serving import _dev, _rng, _within, sv  # noqa: F401
+from test_gpu_serving import _attn, _attn_case, _attn_ref, _dev, _rng, _within, sv  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +52,54 @@ def test_token_probs_infinite_temperature(sv, vocab):
     # exponent of a logit 2^128 below the others is held to 2^-20 of its share.
     bound = want * (2 * ref.EPS + np.array([0.0, 0.0, 2.0 ** -19])[:, None])
     _within(got, want, bound)
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lanes", [1, 40])
+def test_prefix_attn_cached_value_that_is_no_number(sv, lanes, hd, bad):
+    """One element of one value row, its key an ordinary one or of no weight: that column of the rows that see it is NaN,
+    wherever the row stands, and nothing else changes."""
+    c = _attn_case(8, 2, hd, 300, lanes, 3, 75)
+    c["own_len"][:] = 67
+    c["q_len"][:] = 3
+    want, bound = _attn_ref(c)
+    for where, row, first in (("vp", 0, 0), ("vp", 299, 0), ("vp", 130, 0), ("vo", 3, 0), ("vo", 65, 1), ("vo", 66, 2)):
+        for weightless in (False, True):
+            d = {k: v.copy() if isinstance(v, np.ndarray) else v for k, v in c.items()}
+            at = (row, 1, 5) if where == "vp" else (0, row, 1, 5)
+            d[where][at] = bad
+            w, b = want, bound
+            if weightless:  # far below every other score
+                d["k" + where[1]][at[:-1]] = 0
+                d["k" + where[1]][at[:-2] + (1, slice(0, 8))] = -6e4
+                d["q"][..., :8] = np.abs(d["q"][..., :8]) + 1
+                w, b = _attn_ref(d | {where: c[where]})
+            got = _attn(sv, d).cpu().numpy()
+            hit = np.zeros(got.shape, bool)
+            hit[slice(None) if where == "vp" else 0, first:, 4:, 5] = True
+            assert np.isnan(got[hit]).all(), (where, row, weightless)
+            _within(got[~hit], w[~hit], b[~hit], f"{where} {row}")
+
+
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prefix_attn_cached_key_that_is_no_number(sv, hd, bad):
+    """One element of one key row: NaN makes the rows that see it NaN; an infinity does so too, or its score is minus
+    infinity and they are what they are without it.  Other key heads and rows that do not see it keep their results."""
+    c = _attn_case(8, 2, hd, 150, 3, 2, 40)
+    c["own_len"][:] = 33
+    c["q_len"][:] = 2
+    want, bound = _attn_ref(c)
+    c["kp"][77, 1, 3] = bad
+    gone = dict(c, kp=np.delete(c["kp"], 77, 0), vp=np.delete(c["vp"], 77, 0))
+    without, wbound = _attn_ref(gone)
+    got = _attn(sv, c).cpu().numpy()
+    _within(got[:, :, :4], want[:, :, :4], bound[:, :, :4], "the other key head")
+    for i in range(3):
+        for j in range(2):
+            for h in range(4, 8):
+                if np.isnan(bad) or (c["q"][i, j, h, 3] > 0) == (bad > 0):
+                    assert np.isnan(got[i, j, h]).all()
+                elif not np.isnan(got[i, j, h]).all():
+                    _within(got[i, j, h], without[i, j, h], wbound[i, j, h], "without the key")
