@@ -829,8 +829,9 @@ size_t loomhip_prefix_attn_ws(size_t prefix_rows, size_t own_rows, size_t n, siz
  * base_t alone where ids[t] is not in [0, n_adapters).  a [n_adapters][rank]
  * [cols], b [n_adapters][rows][rank] of `type` (F32, F16, BF16; adapters of
  * lower rank zero-padded), scale f32, ids int32; x, base, out f32 rows at the
- * given strides.  base may be out itself (in place) or NULL (zeros).  f32
- * products and sums.  rank up to 256; DECLINED otherwise. */
+ * given strides (column groups of one buffer at one stride will do, sets of
+ * rows at two strides must lie apart).  base may be out itself (in place) or
+ * NULL (zeros).  f32 products and sums.  rank up to 256; DECLINED otherwise. */
 typedef struct {
     int type;
     size_t n_adapters, rank, rows, cols;

@@ -43,12 +43,6 @@ struct LoraParams {
 
 constexpr size_t LORA_MAX_N = 65535 * 64; // vectors, and rows: the launches' work groups
 
-// Whether two device ranges [p, p + elements) share a byte.
-static bool overlap(const void *p, size_t pn, const void *q, size_t qn) {
-    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-    return a < b + qn * 4 && b < a + pn * 4;
-}
-
 static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, const int32_t *ids, const float *base,
                       size_t base_stride, size_t n, float *out, size_t out_stride, LoraParams &P) {
     if (!l)
@@ -70,10 +64,10 @@ static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, co
     if ((uintptr_t)l->a % es || (uintptr_t)l->b % es || (uintptr_t)x % 4 || (uintptr_t)out % 4 || (uintptr_t)base % 4)
         return fail(LOOMHIP_ERR_ARG, "lora: a pointer is not aligned to its elements");
     // every vector's rows are read and written by different work groups
-    const size_t on = n ? (n - 1) * out_stride + l->rows : 0;
-    if (n && overlap(out, on, x, (n - 1) * x_stride + l->cols))
+    if (rows_overlap(out, out_stride, l->rows, x, x_stride, l->cols, n))
         return fail(LOOMHIP_ERR_ARG, "lora: out overlaps x");
-    if (n && base && !(base == out && base_stride == out_stride) && overlap(out, on, base, (n - 1) * base_stride + l->rows))
+    if (base && !(base == out && base_stride == out_stride) &&
+        rows_overlap(out, out_stride, l->rows, base, base_stride, l->rows, n))
         return fail(LOOMHIP_ERR_ARG, "lora: out overlaps base without being it");
     P = {l->a, l->b, l->scale, l->n_adapters, l->rows, l->cols, (int)l->rank, x, base, ids, out, n, x_stride,
          base_stride, out_stride, nullptr, 0, 1};

@@ -308,6 +308,23 @@ int require_device() {
     return LOOMHIP_OK;
 }
 
+bool rows_overlap(const float *p, size_t p_stride, size_t pw, const float *q, size_t q_stride, size_t qw, size_t n) {
+    if (n == 0)
+        return false;
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    const uintptr_t a_end = a + ((n - 1) * p_stride + pw) * 4, b_end = b + ((n - 1) * q_stride + qw) * 4;
+    if (a >= b_end || b >= a_end)
+        return false;
+    if (p_stride != q_stride || n == 1)
+        return true;
+    // q begins k rows and r bytes after p, r within a row: its row j meets p's row j + k, and j + k + 1 where it runs
+    // past the row's end
+    const int64_t s = (int64_t)p_stride * 4, d = (int64_t)(b - a), rows = (int64_t)n;
+    const int64_t k = d >= 0 ? d / s : -((-d + s - 1) / s), r = d - k * s;
+    const auto both = [&](int64_t shift) { return -rows < shift && shift < rows; };
+    return (r < (int64_t)pw * 4 && both(k)) || (r + (int64_t)qw * 4 > s && both(k + 1));
+}
+
 } // namespace lh
 
 using namespace lh;

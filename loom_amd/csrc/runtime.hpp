@@ -42,6 +42,9 @@ int fail(int code, const char *fmt, ...);
 int hip_fail(hipError_t e, const char *what);
 int require_ready();
 int require_device(); // require_ready, and the library's device is the current one
+// Whether two sets of n rows of f32, `pw` and `qw` values wide, share an element.  Exact at one stride (column groups of
+// one buffer lie beside each other); at two, whether their ranges meet.
+bool rows_overlap(const float *p, size_t p_stride, size_t pw, const float *q, size_t q_stride, size_t qw, size_t n);
 hipStream_t stream_of(void *s);
 int upload_weights(int t, const void *host, size_t rows, size_t cols, size_t planes, void **dev);
 void clear_weight_cache();

@@ -1,10 +1,11 @@
 """The batched serving operators on the device at values and layouts beside the
-ordinary: no number among the logits or in the caches, an infinite temperature."""
+ordinary: no number among the logits or in the caches, an infinite temperature,
+columns of one buffer."""
 import numpy as np
 import pytest
 
 import serving_ref as ref
-from test_gpu_serving import _attn, _attn_case, _attn_ref, _dev, _rng, _within, sv  # noqa: F401
+from test_gpu_serving import _attn, _attn_case, _attn_ref, _dev, _lora_case, _lora_ref, _rng, _within, sv  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +104,21 @@ def test_prefix_attn_cached_key_that_is_no_number(sv, hd, bad):
                     assert np.isnan(got[i, j, h]).all()
                 elif not np.isnan(got[i, j, h]).all():
                     _within(got[i, j, h], without[i, j, h], wbound[i, j, h], "without the key")
+
+
+def test_lora_columns_of_one_buffer(sv):
+    """x, base and out side by side in the rows of one buffer share no element; what lies between them stays."""
+    import torch
+
+    for n, rank in ((37, 24), (901, 250)):  # vectors one by one, and tiles of them
+        t = _lora_case(n, 200, 128, rank, 5, "f16")
+        want, bound = _lora_ref(t)
+        wide = torch.full((n, 600), 3.25, device="cuda")
+        x, base, out = wide[:, :128], wide[:, 150:350], wide[:, 390:590]
+        x.copy_(t["x"])
+        base.copy_(t["base"])
+        assert sv.lora_dev(x, t["a"], t["b"], t["scale"], t["ids"], base=base, out=out) is out
+        _within(out.cpu().numpy(), want, bound)
+        assert bool((x == t["x"]).all()) and bool((base == t["base"]).all())
+        for gap in (wide[:, 128:150], wide[:, 350:390], wide[:, 590:]):
+            assert bool((gap == 3.25).all())

@@ -1,0 +1,57 @@
+"""What the batched serving operators take and refuse by where their tensors
+lie, without a GPU: a call that passes its checks ends at the missing device."""
+import ctypes as C
+
+import pytest
+import torch
+
+import loom_amd
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: a GPU would be given them")
+
+FAKE = 0x1000
+PASSED = loom_amd.ERR_INIT
+
+
+def _lora(x, xs, base, bs, out, os, n=4, rows=64, cols=32):
+    d = loom_amd.LoraDesc(loom_amd.F16, 2, 8, rows, cols, FAKE, FAKE, FAKE)
+    return loom_amd.lib().loomhip_lora_dev(C.byref(d), x, xs, FAKE, base, bs, n, out, os, FAKE, 1 << 40, None)
+
+
+AT = 0x100000  # a buffer
+
+
+def _takes(x, xs, base, bs, out, os, n, rows, cols):
+    """The definition: the elements of out's rows, and of x's and base's."""
+    def elements(p, s, w):
+        return {p + 4 * (i * s + c) for i in range(n) for c in range(w)}
+
+    o = elements(out, os, rows)
+    same = base == out and bs == os
+    return not (o & elements(x, xs, cols)) and (base is None or same or not (o & elements(base, bs, rows)))
+
+
+def test_lora_column_groups_of_one_buffer():
+    """Every placement of out against x and base in rows of 24 values: taken exactly where no element is shared."""
+    n, rows, cols, s = 3, 5, 4, 24
+    taken = 0
+    for d in range(-3 * s - 8, 3 * s + 9):  # out's first element from x's
+        out = AT + 4 * d
+        for base in (None, out, AT + 4 * 10, AT + 4 * (s + 10)):
+            want = _takes(AT, s, base, s, out, s, n, rows, cols)
+            taken += want
+            assert _lora(AT, s, base, s, out, s, n, rows, cols) == (PASSED if want else loom_amd.ERR_ARG), (d, base)
+    assert taken > 100
+    for d in range(-8, 9):  # rows one after the other, and a single row
+        for n, s in ((3, 5), (1, 5), (1, 1000)):
+            out = AT + 4 * d
+            want = _takes(AT, s, None, s, out, s, n, 5, 4)
+            assert _lora(AT, s, None, s, out, s, n, 5, 4) == (PASSED if want else loom_amd.ERR_ARG), (d, n, s)
+
+
+def test_lora_rows_at_two_strides_lie_apart():
+    """At two strides the ranges count: refused where they meet, though rows might pass between each other."""
+    assert _lora(AT, 32, None, 64, AT + 4 * 16, 256) == loom_amd.ERR_ARG
+    assert _lora(AT, 32, None, 64, AT + 4 * 32 * 4, 256) == PASSED
+    assert _lora(AT, 256, None, 64, AT + 4 * (3 * 256 + 32), 64) == PASSED
+    assert _lora(AT, 256, None, 64, AT + 4 * (3 * 256 + 31), 64) == loom_amd.ERR_ARG
