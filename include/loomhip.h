@@ -845,7 +845,8 @@ size_t loomhip_lora_ws(const loomhip_lora *l, size_t n);
 
 /* Token probabilities: probs[r] = softmax(logits[r] / temperature[r]) over
  * `vocab` values (temperature f32 [n] or NULL: 1), rows at the given strides;
- * probs may be logits itself with the same stride.  A temperature that is
+ * probs may be logits itself with the same stride, or share no element with
+ * them (as adapters' rows).  A temperature that is
  * not positive (or so small that 1/T passes f32) gives 1 at the first maximum
  * and 0 elsewhere, the frame's greedy pick (NaN logits passed over; at any
  * other temperature they make the row NaN); an infinite one weighs finite

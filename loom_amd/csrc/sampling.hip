@@ -138,10 +138,11 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *
 }
 
 template <int NV>
-__global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *__restrict__ logits, size_t vocab,
-                                                                  size_t stride, const float *__restrict__ temperature,
-                                                                  int splits, const ProbRec *__restrict__ rec,
-                                                                  float *__restrict__ probs, size_t out_stride) {
+__global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *logits, size_t vocab, size_t stride,
+                                                                  const float *__restrict__ temperature, int splits,
+                                                                  const ProbRec *__restrict__ rec, float *probs,
+                                                                  size_t out_stride) {
+    // probs may be logits: a thread reads its values before it writes them
     // The parts in the reduction's order backwards, eight at a time: a part stays with its XCD, and those read last
     // may still be in its L2.
     const int item = (int)((gridDim.x - 1 - blockIdx.x) & ~7u) + (int)(blockIdx.x & 7);
@@ -190,9 +191,9 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *_
 
 // The same of a row that one work group holds in registers, in one launch.
 template <int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void probs_row_kernel(const float *__restrict__ logits, size_t vocab, size_t stride,
-                                                            const float *__restrict__ temperature,
-                                                            float *__restrict__ probs, size_t out_stride) {
+__global__ __launch_bounds__(THREADS) void probs_row_kernel(const float *logits, size_t vocab, size_t stride,
+                                                            const float *__restrict__ temperature, float *probs,
+                                                            size_t out_stride) {
     constexpr int W = THREADS / 64;
     __shared__ float sm[W], sl[W];
     __shared__ int sa[W];
@@ -643,6 +644,8 @@ int loomhip_token_probs_dev(const float *logits, size_t n, size_t vocab, size_t 
         return fail(LOOMHIP_ERR_ARG, "token_probs: a pointer is not aligned to its elements");
     if (stride < vocab || out_stride < vocab)
         return fail(LOOMHIP_ERR_ARG, "token_probs: row stride %zu / %zu below %zu values", stride, out_stride, vocab);
+    if (!(logits == probs && (stride == out_stride || n == 1)) && rows_overlap(probs, out_stride, vocab, logits, stride, vocab, n))
+        return fail(LOOMHIP_ERR_ARG, "token_probs: probs overlaps logits without being them");
     const size_t need = loomhip_token_probs_ws(n, vocab);
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
         return fail(LOOMHIP_ERR_ARG, "token_probs: the workspace takes %zu bytes at a multiple of 16, got %zu", need,

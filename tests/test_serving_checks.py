@@ -49,6 +49,23 @@ def test_lora_column_groups_of_one_buffer():
             assert _lora(AT, s, None, s, out, s, n, 5, 4) == (PASSED if want else loom_amd.ERR_ARG), (d, n, s)
 
 
+def _probs(logits, stride, probs, os, n=3, vocab=5):
+    return loom_amd.lib().loomhip_token_probs_dev(logits, n, vocab, stride, None, probs, os, FAKE, 1 << 40, None)
+
+
+def test_token_probs_over_its_logits():
+    """In place with the same rows, or rows that share no element."""
+    for s in (5, 11, 24):
+        logits = {AT + 4 * (i * s + c) for i in range(3) for c in range(5)}
+        for d in range(-3 * s - 8, 3 * s + 9):
+            want = d == 0 or not logits & {a + 4 * d for a in logits}
+            assert _probs(AT, s, AT + 4 * d, s) == (PASSED if want else loom_amd.ERR_ARG), (s, d)
+    for s, os in ((5, 6), (6, 5), (24, 5)):  # the same first element, other rows
+        assert _probs(AT, s, AT, os) == loom_amd.ERR_ARG
+        assert "overlaps" in loom_amd.last_error()
+    assert _probs(AT, 5, AT, 6, n=1) == PASSED and _probs(AT, 5, AT + 4, 6, n=1) == loom_amd.ERR_ARG
+
+
 def test_lora_rows_at_two_strides_lie_apart():
     """At two strides the ranges count: refused where they meet, though rows might pass between each other."""
     assert _lora(AT, 32, None, 64, AT + 4 * 16, 256) == loom_amd.ERR_ARG
