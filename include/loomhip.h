@@ -814,7 +814,7 @@ typedef struct {
  * a row not seen.
  * prefix->rows or own->rows may be 0 (no rows; pointers unused).
  * head_dim a multiple of 8 up to 256, strides multiples of 8 (rows at most
- * 2^23 apart), pointers at a multiple of 16 bytes, n up to 65535, n_q up to
+ * 2^23 apart; of dimensions longer than one), pointers at a multiple of 16 bytes, n up to 65535, n_q up to
  * 4096; DECLINED otherwise. */
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
                             const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,

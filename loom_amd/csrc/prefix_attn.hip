@@ -887,7 +887,8 @@ static bool pa_served(size_t n, size_t n_q, size_t n_heads, size_t n_kv, size_t 
            hd % 8 == 0 && hd <= PA_MAX_HD && n * n_q * n_heads <= 0x2000000;
 }
 
-static int kv_rows_check(const loomhip_kv_rows *r, size_t n_kv, size_t hd, bool lanes, const char *what) {
+// lanes: how many r holds.  The stride of a dimension of one has no part in the layout.
+static int kv_rows_check(const loomhip_kv_rows *r, size_t n_kv, size_t hd, size_t lanes, const char *what) {
     if (!r || r->rows == 0)
         return LOOMHIP_OK;
     if (!r->k || !r->v)
@@ -896,10 +897,10 @@ static int kv_rows_check(const loomhip_kv_rows *r, size_t n_kv, size_t hd, bool 
         return fail(LOOMHIP_DECLINED, "prefix_attn: %zu %s rows not served", r->rows, what);
     if (r->row_stride < hd && r->rows > 1)
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: %s row stride %zu below a head", what, r->row_stride);
-    if (r->row_stride > PA_MAX_STRIDE)
+    if (r->row_stride > PA_MAX_STRIDE && r->rows > 1)
         return fail(LOOMHIP_DECLINED, "prefix_attn: %s rows %zu elements apart not served", what, r->row_stride);
-    if ((uintptr_t)r->k % 16 || (uintptr_t)r->v % 16 || r->row_stride % 8 || r->head_stride % 8 ||
-        (lanes && r->lane_stride % 8))
+    if ((uintptr_t)r->k % 16 || (uintptr_t)r->v % 16 || (r->rows > 1 && r->row_stride % 8) ||
+        (n_kv > 1 && r->head_stride % 8) || (lanes > 1 && r->lane_stride % 8))
         return fail(LOOMHIP_DECLINED, "prefix_attn: %s rows not at multiples of 16 bytes", what);
     return LOOMHIP_OK;
 }
@@ -927,9 +928,9 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
         return fail(LOOMHIP_DECLINED, "prefix_attn: head size %zu not served", head_dim);
     if (!pa_served(n, n_q, n_heads, n_kv_heads, head_dim))
         return fail(LOOMHIP_DECLINED, "prefix_attn: %zu lanes of %zu tokens, %zu heads not served", n, n_q, n_heads);
-    if (int rc = kv_rows_check(prefix, n_kv_heads, head_dim, false, "prefix"))
+    if (int rc = kv_rows_check(prefix, n_kv_heads, head_dim, 1, "prefix"))
         return rc;
-    if (int rc = kv_rows_check(own, n_kv_heads, head_dim, true, "own"))
+    if (int rc = kv_rows_check(own, n_kv_heads, head_dim, n, "own"))
         return rc;
     if (own && own->rows && !own_len)
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: own rows without their lengths");

@@ -79,7 +79,8 @@ def _kv_desc(k, v, lanes: bool, name: str):
                          "(or its bits as int16)")
     if 0 in shape:
         return _NO_ROWS
-    if v.stride() != stride or (stride[-1] != 1 and shape[-1] != 1):
+    if (v.stride() != stride and any(a != b for a, b, s in zip(stride, v.stride(), shape) if s > 1)) or (
+            stride[-1] != 1 and shape[-1] != 1):
         raise ValueError(f"{name}: keys and values of one layout, the values of a head one after the other")
     return KvRowsDesc(k.data_ptr(), v.data_ptr(), shape[-3], stride[0] if lanes else 0, stride[-3], stride[-2])
 

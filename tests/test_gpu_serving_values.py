@@ -1,6 +1,6 @@
 """The batched serving operators on the device at values and layouts beside the
 ordinary: no number among the logits or in the caches, an infinite temperature,
-columns of one buffer."""
+columns of one buffer, dimensions of one."""
 import numpy as np
 import pytest
 
@@ -122,3 +122,21 @@ def test_lora_columns_of_one_buffer(sv):
         assert bool((x == t["x"]).all()) and bool((base == t["base"]).all())
         for gap in (wide[:, 128:150], wide[:, 350:390], wide[:, 590:]):
             assert bool((gap == 3.25).all())
+
+
+def test_prefix_attn_dimensions_of_one(sv):
+    """A cache of one row, one key head or one lane: the stride of that dimension has no part in the layout."""
+    import torch
+
+    c = _attn_case(4, 1, 64, 1, 1, 1, 1)
+    c["own_len"][:] = 1
+    want, bound = _attn_ref(c, q_len=False)
+
+    def odd(name, keep):  # the same values, the strides of the dimensions of one set to `keep`
+        a = _dev(c[name])
+        return torch.as_strided(a, a.shape, tuple(k if s == 1 else st for s, st, k in zip(a.shape, a.stride(), keep)))
+
+    q, ln = _dev(c["q"]), _dev(c["own_len"])
+    for k, v in (((3, 7, 1), (3, 7, 1)), ((5, 64, 1), (64, 64, 1)), ((1 << 24, 12, 1), (0, 0, 1))):
+        got = sv.prefix_attn_dev(q, odd("kp", k), odd("vp", v), odd("ko", (9, *k)), odd("vo", (64, *v)), ln, c["scale"])
+        _within(got.cpu().numpy(), want, bound, f"{k} {v}")

@@ -72,3 +72,22 @@ def test_lora_rows_at_two_strides_lie_apart():
     assert _lora(AT, 32, None, 64, AT + 4 * 32 * 4, 256) == PASSED
     assert _lora(AT, 256, None, 64, AT + 4 * (3 * 256 + 32), 64) == PASSED
     assert _lora(AT, 256, None, 64, AT + 4 * (3 * 256 + 31), 64) == loom_amd.ERR_ARG
+
+
+def _attn(prefix, own, n=1, kv=1, hd=64):
+    L = loom_amd.lib()
+    return L.loomhip_prefix_attn_dev(C.byref(loom_amd.KvRowsDesc(FAKE, FAKE, *prefix)), C.byref(loom_amd.KvRowsDesc(FAKE, FAKE, *own)),
+                                     FAKE, FAKE, None, n, 1, 4, kv, hd, 0.125, FAKE, 0, FAKE, 1 << 40, None)
+
+
+def test_prefix_attn_strides_of_dimensions_of_one():
+    """rows, lane stride, row stride, head stride: what one lane, row or key head has no use for may be anything."""
+    fine = (16, 0, 128, 64)
+    assert _attn((16, 3, 128, 7), (8, 1029, 128, 12)) == PASSED                # a key head
+    assert _attn((1, 3, 7, 64), (1, 1024, 1 << 30, 64), n=2, kv=2) == PASSED   # a row
+    assert _attn(fine, (8, 1029, 128, 64), kv=2) == PASSED                     # a lane
+    for prefix, own, n, kv in (((16, 0, 127, 64), fine, 1, 1), (fine, (8, 1024, 132, 64), 1, 1), (fine, (8, 1029, 128, 64), 2, 1),
+                               ((16, 0, 128, 60), fine, 1, 2), (fine, (8, 1024, 128, 60), 1, 2),
+                               ((2, 0, 1 << 24, 64), fine, 1, 1)):
+        assert _attn(prefix, own, n, kv) == loom_amd.DECLINED
+    assert _attn((2, 0, 32, 64), fine) == loom_amd.ERR_ARG
