@@ -98,6 +98,8 @@ def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, 
     if len(shape) != 4 or q.dtype is not _F32 or not q.is_contiguous():
         raise ValueError("q: contiguous f32 [n, n_q, n_heads, head_dim]")
     n, n_q, heads, hd = shape
+    if (k_prefix is None) != (v_prefix is None) or (k_own is None) != (v_own is None):
+        raise ValueError("keys without values, or values without keys")
     pre = own = _NO_ROWS
     kv = None
     if k_prefix is not None:

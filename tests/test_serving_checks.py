@@ -91,3 +91,13 @@ def test_prefix_attn_strides_of_dimensions_of_one():
                                ((2, 0, 1 << 24, 64), fine, 1, 1)):
         assert _attn(prefix, own, n, kv) == loom_amd.DECLINED
     assert _attn((2, 0, 32, 64), fine) == loom_amd.ERR_ARG
+
+
+def test_prefix_attn_keys_without_values():
+    from loom_amd import serving
+
+    q, kp, ko = torch.zeros(2, 1, 4, 64), torch.zeros(8, 2, 64).half(), torch.zeros(2, 8, 2, 64).half()
+    ln = torch.ones(2, dtype=torch.int32)
+    for args in ((kp, None, ko, ko), (None, kp, ko, ko), (kp, kp, ko, None), (kp, kp, None, ko), (None, kp, None, ko)):
+        with pytest.raises(ValueError, match="keys without values"):
+            serving.prefix_attn_dev(q, *args, ln, 1.0)
