@@ -66,7 +66,7 @@ static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, co
     // every vector's rows are read and written by different work groups
     if (rows_overlap(out, out_stride, l->rows, x, x_stride, l->cols, n))
         return fail(LOOMHIP_ERR_ARG, "lora: out overlaps x");
-    if (base && !(base == out && base_stride == out_stride) &&
+    if (base && !(base == out && (base_stride == out_stride || n == 1)) &&
         rows_overlap(out, out_stride, l->rows, base, base_stride, l->rows, n))
         return fail(LOOMHIP_ERR_ARG, "lora: out overlaps base without being it");
     P = {l->a, l->b, l->scale, l->n_adapters, l->rows, l->cols, (int)l->rank, x, base, ids, out, n, x_stride,

@@ -42,6 +42,7 @@ def test_lora_column_groups_of_one_buffer():
             taken += want
             assert _lora(AT, s, base, s, out, s, n, rows, cols) == (PASSED if want else loom_amd.ERR_ARG), (d, base)
     assert taken > 100
+    assert _lora(AT, 4, AT + 400, 5, AT + 400, 9, 1, 5, 4) == PASSED  # in place, one row: its stride has no part in it
     for d in range(-8, 9):  # rows one after the other, and a single row
         for n, s in ((3, 5), (1, 5), (1, 1000)):
             out = AT + 4 * d
