@@ -151,6 +151,14 @@ __device__ inline int group_sum(int v) {
     return v;
 }
 
+// Orders this wave's LDS stores against its own reads by other lanes (the
+// LDS serves a wave's accesses in order; this keeps the compiler's order).
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
 // DPP move of a float (disabled rows keep `old`).
 template <int CTRL, int ROW_MASK = 0xF>
 __device__ inline float dpp_f(float old, float v) {

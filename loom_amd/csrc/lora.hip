@@ -481,6 +481,7 @@ __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(Lora
 #pragma unroll
                     for (int h = 0; h < 2; h++)
                         *(lora_u4 *)(as + (r * 16 + h * 8 + lane / 8) * AS + lane % 8 * 16) = av[r0 + r][h];
+                wave_lds_sync();
                 if (r0 == 0)
 #pragma unroll
                     for (int h = 0; h < 2; h++)
@@ -499,6 +500,7 @@ __global__ __launch_bounds__(64 * lora_y_waves(RT)) void lora_many_y_kernel(Lora
                         for (int c = 0; c < E; c++)
                             acc[r0 + r] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c], xf[h][c / 4][c % 4], acc[r0 + r], 0, 0, 0);
                     }
+                wave_lds_sync(); // read before the next stores
             }
         }
         __syncthreads();

@@ -651,14 +651,6 @@ template <> struct MmwBlk<LH_Q6_K> {
     }
 };
 
-// Orders this wave's LDS stores against its own reads by other lanes (the
-// LDS serves a wave's accesses in order; this keeps the compiler's order).
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-}
-
 constexpr int MMW_W = 4;          // waves per work group: four neighbouring row tiles, four staged tokens each
 constexpr int MMW_XL_COLS = 2048; // the tokens' whole rows are staged in LDS up to here
 
