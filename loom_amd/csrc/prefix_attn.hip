@@ -133,7 +133,7 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
                                         const uint16_t *__restrict__ vp, size_t stride, int k0, int k1, int border,
                                         int slot, const int *map, const int *lim, char *smem, int *flag) {
     using C = PaCfg<HDP, RW>;
-    constexpr int STEPS = HDP / 16, KB = C::KPW / 32, DB = HDP / 32;
+    constexpr int STEPS = HDP / 16, DB = HDP / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int half = lane >> 5, col = lane & 31;
     const int rw = wave % RW, kw = wave / RW;
@@ -294,12 +294,15 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
     // No block's own maximum is formed: the sum of eight weights, which is wanted anyway, tells whether one of them is
     // past what m allows (or no number); then m moves to this block's and the eight are formed again.
     float sub = 0.0f; // PA_SHIFT - m
-    const auto grow = [&](const pa_f16 &s) {
+    const auto largest = [](const pa_f16 &s) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; i++)
             mx = fmaxf(mx, s[i]);
-        const float m2 = fmaxf(m, pa_half_max(mx) * cs);
+        return mx;
+    };
+    const auto grow = [&](const pa_f16 &s) {
+        const float m2 = fmaxf(m, pa_half_max(largest(s)) * cs);
         const float f = m == m2 ? 1.0f : __builtin_amdgcn_exp2f(m - m2); // -inf before the first seen key: 0
         m = m2;
         sub = PA_SHIFT - (m == -__builtin_inff() ? 0.0f : m);
@@ -430,14 +433,6 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
     const auto nothing = [](auto) {};
     constexpr std::true_type yes;
     constexpr std::false_type no;
-    const auto largest = [&](const pa_f16 &s) {
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; i++)
-            mx = fmaxf(mx, s[i]);
-        return mx;
-    };
-
     __syncthreads(); // the queries are out of LDS
     if constexpr (C::PIPE) {
         char *cur = smem, *nxt = smem + C::TILE;
@@ -526,11 +521,7 @@ __device__ __forceinline__ void pa_item(const PrefixAttnParams &P, const uint16_
             pa_f16 s = scores(smem, 0, pa_f16{}, no, nullptr, 0, nothing);
             values_ahead(smem, 0);
             mask(s, kt, 0);
-            float mx = s[0]; // a block a tile: its maximum is as cheap as the check
-#pragma unroll
-            for (int i = 1; i < 16; i++)
-                mx = fmaxf(mx, s[i]);
-            if (__any(mx * cs > m + (14.0f - PA_SHIFT)))
+            if (__any(largest(s) * cs > m + (14.0f - PA_SHIFT))) // a block a tile: as cheap as the check of the sum
                 grow(s);
             if (m == -__builtin_inff())
                 sub = 0.0f; // nothing seen: every weight is 2^-inf
@@ -858,21 +849,15 @@ static size_t pa_ws_bytes(const PaPlan &p, size_t hd) {
     return p.slots ? 16 + p.rows * p.slots * (hd * 4 + sizeof(float2)) : 0;
 }
 
-template <int HDP, int RWP>
-static void pa_launch(const PaPlan &p, const PrefixAttnParams &P, size_t items, hipStream_t st) {
-    if (p.rwo == 1)
-        hipLaunchKernelGGL((prefix_attn_kernel<HDP, RWP, 1>), dim3(items), dim3(PA_THREADS), 0, st, P);
-    else
-        hipLaunchKernelGGL((prefix_attn_kernel<HDP, RWP, 2>), dim3(items), dim3(PA_THREADS), 0, st, P);
-}
 template <int HDP>
 static void pa_launch(const PaPlan &p, const PrefixAttnParams &P, size_t items, hipStream_t st) {
-    if (p.rwp == 1)
-        pa_launch<HDP, 1>(p, P, items, st);
+    const auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(items), dim3(PA_THREADS), 0, st, P); };
+    if (p.rwp == 1) // all lanes' rows are at most 32, and so are one's
+        run(prefix_attn_kernel<HDP, 1, 1>);
     else if (p.rwp == 2)
-        pa_launch<HDP, 2>(p, P, items, st);
+        p.rwo == 1 ? run(prefix_attn_kernel<HDP, 2, 1>) : run(prefix_attn_kernel<HDP, 2, 2>);
     else
-        pa_launch<HDP, 4>(p, P, items, st);
+        p.rwo == 1 ? run(prefix_attn_kernel<HDP, 4, 1>) : run(prefix_attn_kernel<HDP, 4, 2>);
 }
 
 } // namespace lh
