@@ -784,9 +784,9 @@ int loomhip_mla_layer_cached_dev(const loomhip_mla_attn *a, const float *const *
  * the same time on several streams or from several threads, each with a
  * workspace of its own: `ws` (device, at a multiple of 16 bytes, contents
  * undefined before and after) of at least the bytes the call's _ws function
- * gives for the same sizes (0: none, NULL will do).  Calls that can run at the same time, captured
- * graphs among them, must not share it.  Outputs must not overlap inputs
- * except where said.  n == 0 is OK and does nothing. */
+ * gives for the same sizes (0: none, NULL will do).  Calls that can run at the
+ * same time, captured graphs among them, must not share it.  Outputs must not
+ * overlap inputs except where said.  n == 0 is OK and does nothing. */
 
 /* Rows of an fp16 key or value cache: element (lane, row, head, i) of k and v
  * at lane * lane_stride + row * row_stride + head * head_stride + i
@@ -806,16 +806,22 @@ typedef struct {
  * reads key head h / (n_heads / n_kv_heads)):
  *   out = sum_t p_t v_t,  p = softmax over the row's t of scale * (q . k_t),
  * zero where a row sees nothing.  out rows j >= q_len[i] are left as they
- * were, or set to zero if zero_rest is not 0.  own_len and q_len are clamped into [0, own->rows] and [0, n_q]; rows
- * of the cache past a query's own are not part of its result, whatever they
- * hold.  For the rows that see it, a value that is NaN or infinite makes its
+ * were, or set to zero if zero_rest is not 0.  own_len and q_len are clamped
+ * into [0, own->rows] and [0, n_q]; rows of the cache past a query's own are
+ * not part of its result, whatever they hold.  For the rows that see it, a value that is NaN or infinite makes its
  * element of the result NaN, a key with a NaN all of it, and a key with an
  * infinity too, unless its score is minus infinity: then it may also count as
  * a row not seen.
- * prefix->rows or own->rows may be 0 (no rows; pointers unused).
+ * prefix->rows or own->rows may be 0 (no rows; pointers unused).  The work
+ * and the workspace are cut by them, not by own_len: own->rows should be what
+ * the longest lane holds, not what its buffer could (the strides stay the
+ * buffer's).  32 lanes of 512 rows behind 4096, 32 heads of 128 over 4 key
+ * heads: 25 us with own->rows 512, 28 with 4160, 37 with 16384.
  * head_dim a multiple of 8 up to 256, strides multiples of 8 (rows at most
- * 2^23 apart; of dimensions longer than one), pointers at a multiple of 16 bytes, n up to 65535, n_q up to
- * 4096; DECLINED otherwise. */
+ * 2^23 apart; of dimensions longer than one), pointers at a multiple of 16
+ * bytes, n up to 65535, n_q up to 4096, n * n_q * n_heads up to 2^25, up to
+ * 2^30 - 1 rows, fewer than 2^24 work items (a lane's key head is one at
+ * least, where there are own rows); DECLINED otherwise. */
 int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows *own, const float *q,
                             const int32_t *own_len, const int32_t *q_len, size_t n, size_t n_q, size_t n_heads,
                             size_t n_kv_heads, size_t head_dim, float scale, float *out, int zero_rest, void *ws,

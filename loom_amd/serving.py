@@ -91,7 +91,8 @@ def prefix_attn_dev(q, k_prefix, v_prefix, k_own, v_own, own_len, scale: float, 
     q f32 [n, n_q, n_heads, head_dim]; k_prefix, v_prefix fp16 [prefix, n_kv_heads, head_dim] (None: no prefix);
     k_own, v_own fp16 [n, rows, n_kv_heads, head_dim] (None: none), of which lane i holds own_len[i] (int32), the last
     q_len[i] of them its query tokens' own (int32; None: n_q each).  Caches of any row, head and lane strides that are
-    multiples of 8, a ``Decoder``'s at one layer among them.  Returns out f32 as q; rows past q_len[i] keep what an
+    multiples of 8, a ``Decoder``'s at one layer among them; the work is cut by `rows`, so pass what the longest lane holds
+    (a view) rather than a cache's whole length.  Returns out f32 as q; rows past q_len[i] keep what an
     ``out`` given holds, and are zero in one made here.
     """
     shape = q.shape

@@ -102,3 +102,19 @@ def test_prefix_attn_keys_without_values():
     for args in ((kp, None, ko, ko), (None, kp, ko, ko), (kp, kp, ko, None), (kp, kp, None, ko), (None, kp, None, ko)):
         with pytest.raises(ValueError, match="keys without values"):
             serving.prefix_attn_dev(q, *args, ln, 1.0)
+
+
+def test_prefix_attn_limits():
+    """n * n_q * n_heads up to 2^25, cache rows below 2^30, work items below 2^24."""
+    L = loom_amd.lib()
+
+    def call(n, nq, heads, kv, own=8, prefix=16):
+        kvs = (loom_amd.KvRowsDesc(FAKE, FAKE, rows, 0, kv * 64, 64) for rows in (prefix, own))
+        return L.loomhip_prefix_attn_dev(*map(C.byref, kvs), FAKE, FAKE, None, n, nq, heads, kv, 64, 0.125, FAKE, 0, FAKE,
+                                         1 << 50, None)
+
+    assert call(4096, 2048, 4, 2) == PASSED and call(4096, 2049, 4, 2) == loom_amd.DECLINED
+    assert call(8192, 4096, 1, 1) == PASSED and call(8192, 4097, 1, 1) == loom_amd.DECLINED
+    assert call(2, 1, 4, 2, own=(1 << 30) - 1) == PASSED and call(2, 1, 4, 2, own=1 << 30) == loom_amd.DECLINED
+    assert call(2, 1, 4, 2, prefix=(1 << 30) - 1) == PASSED and call(2, 1, 4, 2, prefix=1 << 30) == loom_amd.DECLINED
+    assert call(65535, 1, 255, 255, prefix=0) == PASSED and call(65535, 1, 257, 257, prefix=0) == loom_amd.DECLINED
