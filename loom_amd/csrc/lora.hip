@@ -704,8 +704,10 @@ static void lora_many(const LoraParams &P, hipStream_t st) {
 }
 
 // Whether the vectors are taken one by one: while all their reads of A_e and B_e, mostly from L2, stay under LORA_FEW
-// bytes.  Measured at 4096 x 2048, rank 64, fp16: 101 MB (128 vectors) 17 us one by one, 20 as tiles, 28 as tiles of
-// mixed requests; 201 MB 29, 21, 28; 403 MB 53, 23, 32.
+// bytes.  Measured at 4096 x 2048, rank 64, fp16 (bf16 the same): 101 MB (128 vectors) 18 us one by one, 21 as tiles, 28
+// as tiles of mixed requests; 201 MB 30, 21, 29; 403 MB 54, 23, 33.  f32: 101 MB (64 vectors) 13, 19; 201 MB 20, 21, 30;
+// 403 MB 36, 22, 30.  Rank 16, fp16: 101 MB 15, 18, 23; 201 MB 24, 23, 28.  At rank 256 the line lies too low (201 MB, 64
+// vectors, 41 for 55).
 template <class L>
 static bool lora_is_few(const L &l, size_t n, size_t es) {
     return n <= 65535 && (double)n * l.rank * (l.rows + l.cols) * es <= LORA_FEW;
@@ -713,6 +715,8 @@ static bool lora_is_few(const L &l, size_t n, size_t es) {
 // Of those, whether one launch does both steps: the second costs the host 3.5 us, and each work group reads A_e again.
 // Measured, in a graph, against two launches, fp16: A_e of 64 KB, rank 8, 1 vector 4.2 us for 5.1, 256 6.2 for 7.2; of
 // 128 KB, rank 16, 1 vector 5.5 for 5.3, 32 6.2 for 5.5, 256 9.3 for 10.1; rank 64, 1 vector 5.0 for 5.1, 32 8.1 for 7.3.
+// f32: 64 KB, rank 8, 1 vector 4.3 for 5.6, 32 4.5 for 5.9, 256 6.3 for 8.1; 128 KB, rank 16, 5.2 for 5.7, 5.9 for 5.9,
+// 10.1 for 11.2; 256 KB, rank 64, 1 vector 6.4 for 5.8.
 template <class L>
 static bool lora_is_one(const L &l, size_t n, size_t es) {
     return lora_is_few(l, n, es) && l.rank <= 64 && l.rank * l.cols * es <= LORA_SMALL;

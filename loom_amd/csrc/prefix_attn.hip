@@ -10,11 +10,14 @@
 // leave (m, l, o) records, the running maximum and sum of a softmax over their
 // range, and prefix_attn_merge_kernel joins a row's records.
 //
-// Products on the f16 matrix cores (v_mfma_f32_32x32x16_f16), exact to f32's
-// standard: the f32 query is scaled by a power of two of its own and split
-// into two f16 parts (22 significant bits) against the exact fp16 keys, the
-// weights p into two f16 parts against the exact fp16 values, f32 sums.  One
-// f16 part alone (11 bits) would leave 2e-4.
+// Products on the f16 matrix cores (v_mfma_f32_32x32x16_f16), two bits short
+// of f32: the f32 query is scaled by a power of two of its own and split into
+// two f16 parts (22 significant bits where f32 has 24; elements below 2^-16 of
+// the row's largest are off by up to 2^-38 of it) against the exact fp16 keys,
+// the weights p into two f16 parts against the exact fp16 values, f32 sums.
+// One f16 part alone (11 bits) would leave 2e-4.  A third part each would be
+// half as many products again; against 64 bits the error is 2e-7 to 5e-7 of the
+// output's size (elementary operations in f32: 3e-7 to 17e-7).
 //
 // S^T = K Q^T: a lane holds one query (column lane % 32) and, of each 32 keys,
 // the rows 8 (i / 4) + 4 (lane / 32) + i % 4, i < 16.  These registers are the
@@ -24,12 +27,13 @@
 // the LDS transpose read (ds_read_b64_tr_b16) gives from row-major values.
 // The softmax of a query needs one exchange between the two half waves.
 //
-// Measured, heads of 128, 32 over 4 key heads: 190 query tokens of 64 lanes
-// against 16384 shared and up to 640 own rows 114 us (128 at the clock that
-// sustained matrix work leaves), bound by the matrix cores (104 GFLOP in
-// two-part products, 910 TFLOP/s of the 1001 a large library product reaches),
-// the merge 9; 32 lanes of one token against 4096 and 512 rows 20 us
-// (27 MB), one round of short ranges, the merge 4.5.
+// Measured, heads of 128, 32 over 4 key heads, at the median of calls that
+// follow each other: 190 query tokens of 64 lanes against 16384 shared and up
+// to 640 own rows 130 us (121 at best: the clock falls under sustained matrix
+// work), bound by the matrix cores (104 GFLOP in two-part products, 800
+// TFLOP/s of the 1001 a large library product reaches), the merge 11; 32 lanes
+// of one token against 4096 and 512 rows 20.6 us (27 MB), one round of short
+// ranges, the merge 4.6.
 #include "runtime.hpp"
 #include <cmath>
 #include <type_traits>
@@ -657,7 +661,8 @@ __device__ __forceinline__ void pa_map(const PrefixAttnParams &P, int kvh, int r
 
 // The prefix's splits for `blocks` row blocks of every key head: a lane per candidate, the cheapest of
 //   rounds of the chip's work groups * (an item's start and end + its tiles) + records to be joined,
-// in the time of a 64-row tile, two work groups to a CU (3 us: measured start and end 8 us, 1024 records 0.3 us).
+// in the time of a 64-row tile, two work groups to a CU (3 us: measured start and end 8 us, 1024 records 0.3 us; at heads
+// of 128, and taken for the other sizes too).
 constexpr float PA_ITEM = 3.0f, PA_RECORD = 0.09f / 1024.0f;
 __host__ __device__ inline int pa_split_len(int rows, int splits) {
     return ((rows + splits - 1) / splits + 127) / 128 * 128;
@@ -806,7 +811,10 @@ static PaPlan pa_plan(size_t prefix_rows, size_t own_rows, size_t n, size_t n_q,
     // Rows of a prefix item, 32, 64 or 128: few rows are bound by an item's start and end, many by the matrix cores, whose
     // fragments serve twice as many products a wave at 128.  Measured, heads of 128, in blocks of 64 and of 128: 128 rows
     // a key head against 512 shared rows 13.8 us and 16.4, against 65536 54 and 57; 256 against 4096 20.5 and 24.5; 2048
-    // against 16384 166 and 149.
+    // against 16384 166 and 149.  In blocks of 32, 64 and 128, heads of 64: 32 rows against 4096 11.0, 11.6 and 12.9; 128
+    // 14.6, 13.8 and 14.5; 512 against 65536 210, 188 and 166; 2048 against 512 51, 48 and 54 (the line is too low
+    // there).  Heads of 256: 32 rows against 4096 21.6, 22.8 and 26.8; 256 29.7, 30.6 and 34.3; 2048 117, 87 and 87; 512
+    // against 65536 308, 208 and 185.
     p.rwp = all <= 32 ? 1 : all <= 256 ? 2 : 4;
     p.rwo = mine <= 32 ? 1 : 2;
     // the chip's work groups (two to a CU, one at head sizes over 128), shared by the tiles of the two kinds

@@ -53,8 +53,9 @@ __device__ __forceinline__ void row_part(const float *x, size_t v0, size_t vocab
 // T infinite: finite logits weigh alike, -inf still nothing.
 // T not positive, NaN or so small that 1/T passes f32: 1 at the first maximum
 // among the numbers (a NaN logit makes a row of any other T NaN).
-// Bound by bytes: 160 rows of 151936 take 25 us for the sums (3.9 TB/s) and 31
-// for the second read, mostly from the last-level cache, and the write.
+// Bound by bytes: 160 rows of 151936 take 22.6 us for the sums (4.3 TB/s) and
+// 31 for the second read, mostly from the last-level cache, and the write
+// (medians of calls that follow each other).
 struct ProbRec {
     float m, l;
     int32_t at;
@@ -285,7 +286,7 @@ constexpr size_t PROBS_ROW = 32768;
 // launches: each (lane, part of the row) finds r and sums its values; then one
 // work group per lane scans the parts' sums and the one part that holds the
 // token.  One work group holds a shorter row, and does both.  Bound by bytes:
-// 64 lanes of 151936 values take 13 us for two rows each (5.8 TB/s), then 6.
+// 64 lanes of 151936 values take 13.6 us for two rows each (5.7 TB/s), then 6.
 struct VerifyParams {
     const float *target, *draft; // [n][k+1][vocab], [n][k][vocab] or null
     const int32_t *tok, *n_draft;
