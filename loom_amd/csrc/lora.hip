@@ -61,7 +61,8 @@ static int lora_check(const loomhip_lora *l, const float *x, size_t x_stride, co
     if (x_stride < l->cols || out_stride < l->rows || (base && base_stride < l->rows))
         return fail(LOOMHIP_ERR_ARG, "lora: a row stride below its row");
     const size_t es = l->type == LH_F32 ? 4 : 2;
-    if ((uintptr_t)l->a % es || (uintptr_t)l->b % es || (uintptr_t)x % 4 || (uintptr_t)out % 4 || (uintptr_t)base % 4)
+    if ((uintptr_t)l->a % es || (uintptr_t)l->b % es ||
+        ((uintptr_t)l->scale | (uintptr_t)x | (uintptr_t)ids | (uintptr_t)out | (uintptr_t)base) % 4)
         return fail(LOOMHIP_ERR_ARG, "lora: a pointer is not aligned to its elements");
     // every vector's rows are read and written by different work groups
     if (rows_overlap(out, out_stride, l->rows, x, x_stride, l->cols, n))

@@ -927,6 +927,8 @@ int loomhip_prefix_attn_dev(const loomhip_kv_rows *prefix, const loomhip_kv_rows
         return rc;
     if (own && own->rows && !own_len)
         return fail(LOOMHIP_ERR_ARG, "prefix_attn: own rows without their lengths");
+    if (((uintptr_t)own_len | (uintptr_t)q_len) % 4)
+        return fail(LOOMHIP_ERR_ARG, "prefix_attn: lengths not aligned to their elements");
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
         return fail(LOOMHIP_DECLINED, "prefix_attn: q or out not at a multiple of 16 bytes");
     const PaPlan p = pa_plan(prefix ? prefix->rows : 0, own ? own->rows : 0, n, n_q, n_heads, n_kv_heads, head_dim,

@@ -118,3 +118,22 @@ def test_prefix_attn_limits():
     assert call(2, 1, 4, 2, own=(1 << 30) - 1) == PASSED and call(2, 1, 4, 2, own=1 << 30) == loom_amd.DECLINED
     assert call(2, 1, 4, 2, prefix=(1 << 30) - 1) == PASSED and call(2, 1, 4, 2, prefix=1 << 30) == loom_amd.DECLINED
     assert call(65535, 1, 255, 255, prefix=0) == PASSED and call(65535, 1, 257, 257, prefix=0) == loom_amd.DECLINED
+
+
+def test_pointers_aligned_to_their_elements():
+    """Lengths, ids and scales as well: a uniform load drops an address's low bits."""
+    L = loom_amd.lib()
+    kv = loom_amd.KvRowsDesc(FAKE, FAKE, 16, 1024, 128, 64)
+
+    def attn(own_len, q_len):
+        return L.loomhip_prefix_attn_dev(C.byref(kv), C.byref(kv), FAKE, own_len, q_len, 2, 1, 4, 2, 64, 0.125, FAKE, 0, FAKE,
+                                         1 << 40, None)
+
+    def lora(scale, ids):
+        d = loom_amd.LoraDesc(loom_amd.F16, 2, 8, 64, 32, FAKE, FAKE, scale)
+        return L.loomhip_lora_dev(C.byref(d), AT, 32, ids, None, 64, 4, 2 * AT, 64, FAKE, 1 << 40, None)
+
+    assert attn(FAKE + 4, FAKE + 8) == PASSED and lora(FAKE + 4, FAKE + 8) == PASSED
+    for off in (1, 2, 3):
+        for rc in (attn(FAKE + off, None), attn(FAKE, FAKE + off), lora(FAKE + off, FAKE), lora(FAKE, FAKE + off)):
+            assert rc == loom_amd.ERR_ARG and "aligned" in loom_amd.last_error()
