@@ -49,7 +49,7 @@ extern "C" {
 #define LOOMHIP_Q8_0 8
 #define LOOMHIP_Q4_K 12
 #define LOOMHIP_Q6_K 14
-#define LOOMHIP_BF16 30 /* adapters (loomhip_lora) only */
+#define LOOMHIP_BF16 30 /* adapters (loomhip_lora) and pages (loomhip_pages) only */
 
 /* gating (src/gguf/moe.zig:36-44) */
 #define LOOMHIP_GATING_SOFTMAX 1
@@ -884,6 +884,106 @@ int loomhip_verify_drafts_dev(const float *target_probs, const float *draft_prob
                               size_t vocab, int32_t *tokens_out, int32_t *n_accepted, void *ws, size_t ws_bytes,
                               void *stream);
 size_t loomhip_verify_drafts_ws(size_t n, size_t vocab);
+
+/* Heads of n tokens, head_dim values each, on their way through a norm and a
+ * rotation: head h of token t at x + t * x_stride + h * head_dim (a column
+ * group of one projection's output will do), its result likewise at out.  out
+ * may be x itself at the same stride; otherwise outputs share no element with
+ * inputs or each other.  norm: f32 [head_dim], NULL for none. */
+typedef struct {
+    const float *x;
+    size_t x_stride;
+    float *out;
+    size_t out_stride;
+    const float *norm;
+    size_t n_heads; /* 0: none of these */
+} loomhip_heads;
+/* The rotation by position: the first `rot` values of a head (even, 0: none)
+ * in pairs (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved, pair i by
+ * pos * freqs[i] (freqs f64 [rot / 2], radians a position; the angle is formed
+ * in 64 bits).  pos int32 [n]; a token of a negative position is padding:
+ * nothing of it is read or written.  eps: the norms'. */
+typedef struct {
+    const int32_t *pos;
+    const double *freqs;
+    size_t rot;
+    int interleaved;
+    float eps;
+} loomhip_rope;
+/* Queries and keys of n tokens, each head normed (x / sqrt(mean x^2 + eps) *
+ * norm, where it has a norm), then rotated.  k may be NULL.  head_dim a
+ * multiple of 8 up to 256, up to 4096 heads each and 2^24 tokens; DECLINED
+ * otherwise. */
+int loomhip_qk_norm_rope_dev(const loomhip_heads *q, const loomhip_heads *k, const loomhip_rope *r, size_t n,
+                             size_t head_dim, void *stream);
+
+/* A paged key and value cache: a pool of n_pages pages of page_size rows
+ * (any number) of F16 or BF16, element (page, row, head, i) of k and v at page
+ * * page_stride + row * row_stride + head * head_stride + i, and a table int32
+ * [n_lanes][table_width] (rows table_stride apart) of the pages that hold each
+ * lane's positions 0 .. page_size - 1, page_size .. and so on.  An entry
+ * outside [0, n_pages) is no page: its positions cannot be written and are not
+ * seen, so a lane's early pages may be given back.  Strides (of dimensions
+ * longer than one) multiples of 8, k and v at a multiple of 16 bytes, up to
+ * 2^31 - 1 positions a lane and 2^35 values a pool; DECLINED otherwise. */
+typedef struct {
+    void *k, *v;
+    int type;
+    size_t n_pages, page_size;
+    size_t page_stride, row_stride, head_stride;
+    const int32_t *table;
+    size_t n_lanes, table_width, table_stride;
+} loomhip_pages;
+/* Keys and values of n tokens into the cache: token t at position r->pos[t] of
+ * lane lanes[t] (int32; NULL: lane t), keys normed and rotated as by
+ * loomhip_qk_norm_rope_dev (k->out unused), values as they are (f32
+ * [n][k->n_heads][head_dim], tokens v_stride apart), each rounded once to the
+ * cache's type (f16 past 65504 is infinite).  A token whose position has no
+ * page, or whose lane is outside the table, is not stored.  Two tokens at one
+ * position of one lane leave a row of unspecified ones of their values.  q, if
+ * not NULL: the tokens' queries, normed and rotated to q->out in the same
+ * launch (q->out may be q->x). */
+int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, const loomhip_heads *k, const float *v,
+                             size_t v_stride, const int32_t *lanes, const loomhip_rope *r, size_t n, size_t head_dim,
+                             void *stream);
+
+/* Attention of one new token of each of n lanes over its pages: lane i sees
+ * the first len[i] (int32; clamped into [0, table_width * page_size])
+ * positions, the new token's own among them, of those the last `window` where
+ * window is not 0, and none of a page that its table does not have.  q, out f32
+ * [n][n_heads][head_dim]; out = sum_t p_t v_t, p the softmax of scale *
+ * (q . k_t) (head h over key head h / (n_heads / n_kv_heads)), zero where a lane
+ * sees nothing.  Rows that are not seen are not part of the result whatever they hold;
+ * for the heads that see it, a value that is NaN or infinite makes its element
+ * of the result NaN, a key with a NaN all of it, and a key with an infinity
+ * too, unless its score is minus infinity.  The work is cut on the device by
+ * len, not by the table's width.  n lanes of the table's n_lanes; head_dim a
+ * multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^24; DECLINED
+ * otherwise. */
+int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
+                           size_t n_kv_heads, size_t head_dim, float scale, size_t window, float *out, void *ws,
+                           size_t ws_bytes, void *stream);
+size_t loomhip_paged_attn_ws(size_t max_rows, size_t n, size_t n_heads, size_t n_kv_heads, size_t head_dim);
+
+/* Log probabilities of given tokens, with the rows' entropy and likeliest
+ * alternatives: of row r of logits (f32, `vocab` values, rows `stride` apart),
+ * with T = temperature[r] (f32 [n], or NULL: 1),
+ *   lp_v = log softmax(logits / T)_v
+ *   logprobs[r] = lp of tokens[r] (int32; -inf where it is no token)
+ *   entropy[r]  = -sum_v p_v lp_v                       (natural logarithms)
+ *   top_ids[r], top_logprobs[r] [top]: the `top` largest logits in descending
+ *     order, of equal ones the lower index first, and their lp; -1 and -inf
+ *     where the row has no more.
+ * NaN logits are never among the top; any NaN or +inf makes the row's log
+ * probabilities and its entropy NaN.  A temperature that is not positive (or
+ * so small that 1/T passes f32): the first maximum has probability 1, as in
+ * loomhip_token_probs_dev (its lp 0, every other -inf, the entropy 0); an
+ * infinite one weighs finite logits alike and -inf as nothing.  A row of -inf
+ * alone: -inf, entropy 0.  top up to 32, n up to 65535; DECLINED otherwise. */
+int loomhip_token_logprobs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const int32_t *tokens,
+                               const float *temperature, size_t top, float *logprobs, float *entropy, int32_t *top_ids,
+                               float *top_logprobs, void *ws, size_t ws_bytes, void *stream);
+size_t loomhip_token_logprobs_ws(size_t n, size_t vocab, size_t top);
 
 #ifdef __cplusplus
 }

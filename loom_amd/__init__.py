@@ -257,6 +257,29 @@ class LoraDesc(C.Structure):
                 ("cols", C.c_size_t), ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
 
 
+class HeadsDesc(C.Structure):
+    """Mirror of ``loomhip_heads`` in include/loomhip.h."""
+
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_size_t), ("out", C.c_void_p), ("out_stride", C.c_size_t),
+                ("norm", C.c_void_p), ("n_heads", C.c_size_t)]
+
+
+class RopeDesc(C.Structure):
+    """Mirror of ``loomhip_rope`` in include/loomhip.h."""
+
+    _fields_ = [("pos", C.c_void_p), ("freqs", C.c_void_p), ("rot", C.c_size_t), ("interleaved", C.c_int),
+                ("eps", C.c_float)]
+
+
+class PagesDesc(C.Structure):
+    """Mirror of ``loomhip_pages`` in include/loomhip.h."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_pages", C.c_size_t),
+                ("page_size", C.c_size_t), ("page_stride", C.c_size_t), ("row_stride", C.c_size_t),
+                ("head_stride", C.c_size_t), ("table", C.c_void_p), ("n_lanes", C.c_size_t),
+                ("table_width", C.c_size_t), ("table_stride", C.c_size_t)]
+
+
 def header_symbols() -> list[str]:
     """Every function name declared in include/loomhip.h."""
     text = open(HEADER).read()
@@ -386,6 +409,13 @@ def lib() -> C.CDLL:
         "loomhip_token_probs_ws": (sz, [sz, sz]),
         "loomhip_verify_drafts_dev": (i, [vp, vp, vp, vp, vp, vp, sz, sz, sz, vp, vp, vp, sz, vp]),
         "loomhip_verify_drafts_ws": (sz, [sz, sz]),
+        "loomhip_qk_norm_rope_dev": (i, [C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), C.POINTER(RopeDesc), sz, sz, vp]),
+        "loomhip_paged_append_dev": (i, [C.POINTER(PagesDesc), C.POINTER(HeadsDesc), C.POINTER(HeadsDesc), vp, sz, vp,
+                                         C.POINTER(RopeDesc), sz, sz, vp]),
+        "loomhip_paged_attn_dev": (i, [C.POINTER(PagesDesc), vp, vp, sz, sz, sz, sz, f, sz, vp, vp, sz, vp]),
+        "loomhip_paged_attn_ws": (sz, [sz, sz, sz, sz, sz]),
+        "loomhip_token_logprobs_dev": (i, [vp, sz, sz, sz, vp, vp, sz, vp, vp, vp, vp, vp, sz, vp]),
+        "loomhip_token_logprobs_ws": (sz, [sz, sz, sz]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -1,0 +1,400 @@
+// paged_attn.hip -- attention of one new token of every lane over its pages.
+//
+//   out = sum_t p_t v_t,  p = softmax of scale * (q . k_t) over the rows t seen
+//
+// The query heads of a key head (up to 16) are the columns of the matrix
+// products.  A work group's four waves take a lane's rows in turn, a tile
+// of rows each: no wave waits for another before the end, where their running
+// maxima, sums and products are joined.
+//
+// Products on the matrix cores, in the cache's own type (mfma 16x16x32), exact
+// in the cached values and near f32 in the others: an f16 cache takes the query
+// (scaled by a power of two of its own) and the weights in two f16 parts (22
+// bits), a bf16 cache in three bf16 parts (24).  The sums are f32.
+//
+// S^T = K Q^T: a lane holds one query head (column lane % 16) and, of each 32
+// rows, the rows 4 (lane / 16) + i and 16 + 4 (lane / 16) + i, i < 4.  These
+// eight weights are the B operand of O^T = V^T P^T as they stand, if its 8
+// contracted indices mean those rows; the A operand's lane then needs the same
+// rows of one value column, which two LDS transpose reads (ds_read_b64_tr_b16)
+// give from row-major values.
+#include "runtime.hpp"
+
+#include <type_traits>
+
+namespace lh {
+
+typedef _Float16 pg_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pg_b8 __attribute__((ext_vector_type(8)));
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
+
+int pages_check(const loomhip_pages *c, size_t n_kv, size_t hd, const char *fn);
+
+constexpr int PG_THREADS = 256, PG_WAVES = PG_THREADS / 64;
+constexpr int PG_MAX_HD = 256;
+constexpr int PG_COLS = 16; // query heads of an item
+
+// f16: two parts of a value, of a size that the second is normal; bf16: three, of f32's own range.
+struct PgF16 {
+    typedef pg_h8 v8;
+    typedef _Float16 elem;
+    static constexpr int PARTS = 2;
+    static constexpr float SHIFT = 14.0f; // weights are 2^(s - m + SHIFT), at most 2^14: their second parts stay normal
+    static __device__ __forceinline__ pg_f4 mfma(v8 a, v8 b, pg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+struct PgBf16 {
+    typedef pg_b8 v8;
+    typedef __bf16 elem;
+    static constexpr int PARTS = 3;
+    static constexpr float SHIFT = 0.0f;
+    static __device__ __forceinline__ pg_f4 mfma(v8 a, v8 b, pg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <class T>
+__device__ __forceinline__ void pg_split(float x, int e, typename T::v8 (&p)[T::PARTS]) {
+#pragma unroll
+    for (int i = 0; i < T::PARTS; i++) {
+        const typename T::elem h = (typename T::elem)x;
+        p[i][e] = h;
+        x -= (float)h;
+    }
+}
+
+struct PagedAttnParams {
+    loomhip_pages c;
+    const float *q;
+    const int32_t *len;
+    int n, n_heads, n_kv, hd, group, blocks; // group: query heads of a key head, in `blocks` blocks of PG_COLS
+    uint32_t window;                         // 0: none
+    float scale;
+    float *out;
+};
+
+// Rows [first, end) that lane i sees.
+__device__ __forceinline__ void pg_span(const PagedAttnParams &P, int i, uint32_t &first, uint32_t &end) {
+    const uint32_t most = (uint32_t)(P.c.page_size * P.c.table_width);
+    const int len = P.len[i];
+    end = len < 0 ? 0 : (uint32_t)len < most ? (uint32_t)len : most;
+    first = P.window && P.window < end ? end - P.window : 0;
+}
+
+// A value and its row's partners in the other three rows of 16 lanes.
+__device__ __forceinline__ float pg_max4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float pg_sum4(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Tile rows are padded in LDS so that fragment reads spread over the banks: keys
+// are read as 16 bytes of sixteen rows, values as 32 bytes of four rows.
+template <int HDP>
+struct PgCfg {
+    static constexpr int KT = HDP == 64 ? 64 : 32;   // rows of a wave's tile
+    static constexpr int CH = HDP / 8, RPI = 64 / CH; // 16-byte chunks of a row, rows a load instruction takes
+    static constexpr int NL = KT / RPI;              // loads of a tile's keys, and of its values
+    static constexpr int KS = HDP * 2 + 16, VS = HDP * 2 + 32, VO = KT * KS;
+    static constexpr int WAVE = KT * (KS + VS); // bytes of a wave's tile
+    static constexpr int OS = HDP + 4;          // floats from a head's joined sums to the next
+    static constexpr int JOIN = PG_COLS * OS * 4;
+    static constexpr int BYTES = PG_WAVES * (WAVE > JOIN ? WAVE : JOIN);
+};
+
+// Query heads [h0, h0 + heads) of lane i, which read key head kvh, against its
+// rows [r0, r1): the four waves' (m, l, o), in LDS.
+template <class T, int HDP>
+__device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh, int h0, int heads, uint32_t r0,
+                                        uint32_t r1, char *smem, float (*sm)[PG_COLS], float (*sl)[PG_COLS]) {
+    using C = PgCfg<HDP>;
+    constexpr int STEPS = HDP / 32, DB = HDP / 16, NB = C::KT / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, col = lane & 15;
+    const int hd = P.hd;
+    char *tile = smem + wave * C::WAVE;
+
+    // the query's parts: 8 (lane / 16) + j of every 32 values
+    typename T::v8 qp[STEPS][T::PARTS];
+    float cs = P.scale * 0x1.715476p+0f; // scores in log2 units
+    {
+        const float *q = P.q + ((size_t)i * P.n_heads + h0 + (col < heads ? col : 0)) * hd;
+        float v[STEPS][8], amax = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int d = s * 32 + quad * 8;
+            const bool in = col < heads && d < hd;
+            const pg_f4 a = *(const pg_f4 *)(q + (d < hd ? d : 0)), b = *(const pg_f4 *)(q + (d < hd ? d : 0) + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[s][e] = in ? a[e] : 0.0f;
+                v[s][e + 4] = in ? b[e] : 0.0f;
+                amax = fmaxf(amax, fmaxf(fabsf(v[s][e]), fabsf(v[s][e + 4])));
+            }
+        }
+        float f = 1.0f;
+        if (T::PARTS == 2) { // the largest element brought to 2^13 .. 2^14
+            amax = pg_max4(amax);
+            const int e = (int)(__float_as_uint(amax) >> 23);
+            const int k = e > 0 && e < 255 ? (140 - e > 120 ? 120 : 140 - e < -120 ? -120 : 140 - e) : 0;
+            f = __uint_as_float((uint32_t)(127 + k) << 23);
+            cs *= __uint_as_float((uint32_t)(127 - k) << 23);
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                pg_split<T>(v[s][e] * f, e, qp[s]);
+    }
+
+    // staging: the lane's chunk of a row, the first of its rows
+    const int chunk = (lane % C::CH) * 8 < hd ? lane % C::CH : hd / 8 - 1; // past the head's end: the last one again
+    const uint16_t *kb = (const uint16_t *)P.c.k + (size_t)kvh * P.c.head_stride + chunk * 8;
+    const uint16_t *vb = (const uint16_t *)P.c.v + (size_t)kvh * P.c.head_stride + chunk * 8;
+    const int32_t *table = P.c.table + (size_t)i * P.c.table_stride;
+    const uint32_t ps = (uint32_t)P.c.page_size;
+    const uint32_t row_units = (uint32_t)(P.c.row_stride / 8);
+    pg_u4 rk[C::NL], rv[C::NL];
+    // The tile that starts at row `at`: where the lane's row (lane % KT) begins, in 16-byte units, and which rows are
+    // there.  A row that is not (past the end, on no page) is loaded as the pool's first.
+    const auto page_of = [&](uint32_t at) {
+        const uint32_t r = at + lane % C::KT;
+        return r < r1 ? table[r / ps] : -1;
+    };
+    const auto place = [&](uint32_t at, int32_t page, uint32_t &unit) {
+        const uint32_t r = at + lane % C::KT;
+        const bool in = r < r1 && page >= 0 && (uint32_t)page < (uint32_t)P.c.n_pages;
+        unit = in ? (uint32_t)((size_t)page * (P.c.page_stride / 8) + (size_t)(r % ps) * row_units) : 0u;
+        return __ballot(in);
+    };
+    const auto load = [&](uint32_t unit) {
+#pragma unroll
+        for (int c = 0; c < C::NL; c++) {
+            const size_t at = (size_t)(uint32_t)__shfl((int)unit, c * C::RPI + lane / C::CH) * 8;
+            rk[c] = *(const pg_u4 *)(kb + at);
+            rv[c] = *(const pg_u4 *)(vb + at);
+        }
+    };
+
+    pg_f4 o[DB];
+#pragma unroll
+    for (int b = 0; b < DB; b++)
+        o[b] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -__builtin_inff(), l = 0.0f;
+    constexpr uint64_t ALL = C::KT == 64 ? ~0ull : (1ull << 32) - 1;
+
+    const int st = (lane / C::CH) * C::KS + (lane % C::CH) * 16, vt = C::VO + (lane / C::CH) * C::VS + (lane % C::CH) * 16;
+    const int k_at = col * C::KS + quad * 16, v_at = C::VO + (4 * quad + (col >> 2)) * C::VS + 8 * (col & 3);
+    const auto value_frag = [&](int b, int db) {
+        const auto at = (__attribute__((address_space(3))) char *)(tile + v_at) + b * 32 * C::VS + db * 32;
+        const pg_s4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4 *)at);
+        const pg_s4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4 *)(at + 16 * C::VS));
+        return __builtin_bit_cast(typename T::v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    uint32_t at = r0 + wave * C::KT, unit;
+    uint64_t live = 0;
+    int32_t next = -1;
+    if (at < r1) {
+        live = place(at, page_of(at), unit) & ALL;
+        next = page_of(at + PG_WAVES * C::KT);
+        load(unit);
+    }
+    for (; at < r1; at += PG_WAVES * C::KT) {
+        const uint64_t here = live;
+        live = place(at + PG_WAVES * C::KT, next, unit) & ALL;
+        next = page_of(at + 2 * PG_WAVES * C::KT);
+        wave_lds_sync(); // the reads of the tile before
+#pragma unroll
+        for (int c = 0; c < C::NL; c++) {
+            *(pg_u4 *)(tile + st + c * C::RPI * C::KS) = rk[c];
+            if (here != ALL && !(here >> (c * C::RPI + lane / C::CH) & 1))
+                rv[c] = pg_u4{0, 0, 0, 0}; // a weight of zero times what lies there
+            *(pg_u4 *)(tile + vt + c * C::RPI * C::VS) = rv[c];
+        }
+        if (at + PG_WAVES * C::KT < r1)
+            load(unit);
+        wave_lds_sync();
+        if (here == 0)
+            continue;
+        float s[NB][8], mx = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                pg_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = 0; x < STEPS; x++) {
+                    const auto kf = *(const typename T::v8 *)(tile + k_at + (b * 32 + h * 16) * C::KS + x * 64);
+#pragma unroll
+                    for (int p = T::PARTS - 1; p >= 0; p--)
+                        acc = T::mfma(kf, qp[x][p], acc);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    s[b][h * 4 + e] = acc[e] * cs;
+            }
+        if (here != ALL) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (!(here >> (b * 32 + (e / 4) * 16 + quad * 4 + e % 4) & 1))
+                        s[b][e] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                mx = fmaxf(mx, s[b][e]);
+        if (__any(mx > m)) {
+            const float m2 = fmaxf(m, pg_max4(mx));
+            const float f = m == m2 ? 1.0f : __builtin_amdgcn_exp2f(m - m2); // 0 at the first
+            m = m2;
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+                o[b] *= f;
+        }
+        const float sub = T::SHIFT - (m == -__builtin_inff() ? 0.0f : m);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            typename T::v8 pp[T::PARTS];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float w = __builtin_amdgcn_exp2f(s[b][e] + sub);
+                l += w;
+                pg_split<T>(w, e, pp);
+            }
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                const auto vf = value_frag(b, d);
+#pragma unroll
+                for (int p = T::PARTS - 1; p >= 0; p--)
+                    o[d] = T::mfma(vf, pp[p], o[d]);
+            }
+        }
+    }
+    l = pg_sum4(l);
+    m = pg_max4(m); // equal already
+    __syncthreads(); // all tiles are read: their room is the join's
+    float *so = (float *)smem + wave * PG_COLS * C::OS + col * C::OS + quad * 4;
+#pragma unroll
+    for (int b = 0; b < DB; b++)
+        *(pg_f4 *)(so + b * 16) = o[b];
+    if (quad == 0)
+        sm[wave][col] = m, sl[wave][col] = l;
+    __syncthreads();
+}
+
+template <class T, int HDP>
+__global__ __launch_bounds__(PG_THREADS, HDP == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams P) {
+    using C = PgCfg<HDP>;
+    __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
+    __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
+    const int block = blockIdx.x % P.blocks, ik = blockIdx.x / P.blocks, i = ik / P.n_kv, kvh = ik - i * P.n_kv;
+    const int h0 = kvh * P.group + block * PG_COLS;
+    const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
+    uint32_t r0, r1;
+    pg_span(P, i, r0, r1);
+    pg_rows<T, HDP>(P, i, kvh, h0, heads, r0, r1, smem, sm, sl);
+    const float *so = (const float *)smem;
+    for (int x = threadIdx.x; x < heads * (HDP / 4); x += PG_THREADS) {
+        const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
+        float M = sm[0][h];
+#pragma unroll
+        for (int w = 1; w < PG_WAVES; w++)
+            M = fmaxf(M, sm[w][h]);
+        float L = 0.0f;
+        pg_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < PG_WAVES; w++) {
+            const float f = sm[w][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][h] - M);
+            L += sl[w][h] * f;
+            a += *(const pg_f4 *)(so + (w * PG_COLS + h) * C::OS + d) * f;
+        }
+        a *= L == 0.0f ? 0.0f : 1.0f / L; // nothing seen: zero
+        // an infinity here comes from a cached one, which the weights' second parts turn into NaN for some: NaN for all
+        if (d < P.hd)
+            *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = a + a * 0.0f;
+    }
+}
+
+} // namespace lh
+
+using namespace lh;
+
+// The sizes the kernels index in 32 bits.
+static bool pg_served(size_t n, size_t n_heads, size_t n_kv, size_t hd) {
+    return n && n <= 65535 && n_heads && n_kv && n_heads % n_kv == 0 && hd && hd % 8 == 0 && hd <= PG_MAX_HD &&
+           n_heads <= 65535 && n * n_heads <= (size_t)1 << 24;
+}
+
+extern "C" {
+
+size_t loomhip_paged_attn_ws(size_t max_rows, size_t n, size_t n_heads, size_t n_kv_heads, size_t head_dim) {
+    return 0;
+}
+
+int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
+                           size_t n_kv_heads, size_t head_dim, float scale, size_t window, float *out, void *ws,
+                           size_t ws_bytes, void *stream) {
+    const char *fn = "paged_attn";
+    if (n == 0)
+        return LOOMHIP_OK;
+    if (!q || !out || !len || n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads)
+        return fail(LOOMHIP_ERR_ARG, "%s: null argument, or %zu heads over %zu key heads", fn, n_heads, n_kv_heads);
+    if (!pg_served(n, n_heads, n_kv_heads, head_dim))
+        return fail(LOOMHIP_DECLINED, "%s: %zu lanes of %zu heads of %zu not served", fn, n, n_heads, head_dim);
+    if (int rc = pages_check(c, n_kv_heads, head_dim, fn))
+        return rc;
+    if (n > c->n_lanes)
+        return fail(LOOMHIP_ERR_ARG, "%s: %zu lanes, a table of %zu", fn, n, c->n_lanes);
+    if ((uintptr_t)len % 4)
+        return fail(LOOMHIP_ERR_ARG, "%s: lengths not aligned to their elements", fn);
+    if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
+        return fail(LOOMHIP_DECLINED, "%s: q or out not at a multiple of 16 bytes", fn);
+    if (int rc = require_device())
+        return rc;
+    PagedAttnParams P = {};
+    P.c = *c;
+    P.q = q;
+    P.len = len;
+    P.n = (int)n;
+    P.n_heads = (int)n_heads;
+    P.n_kv = (int)n_kv_heads;
+    P.hd = (int)head_dim;
+    P.group = (int)(n_heads / n_kv_heads);
+    P.blocks = (P.group + PG_COLS - 1) / PG_COLS;
+    P.window = window > 0x7fffffff ? 0 : (uint32_t)window; // longer than any lane: none
+    P.scale = scale;
+    P.out = out;
+    hipStream_t st = stream_of(stream);
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        const dim3 g(n * n_kv_heads * P.blocks), b(PG_THREADS);
+        if (head_dim <= 64)
+            hipLaunchKernelGGL((paged_attn_kernel<T, 64>), g, b, 0, st, P);
+        else if (head_dim <= 128)
+            hipLaunchKernelGGL((paged_attn_kernel<T, 128>), g, b, 0, st, P);
+        else
+            hipLaunchKernelGGL((paged_attn_kernel<T, 256>), g, b, 0, st, P);
+    };
+    if (c->type == LH_F16)
+        run(PgF16{});
+    else
+        run(PgBf16{});
+    note_launch();
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "paged_attn launch");
+}
+
+} // extern "C"

@@ -5,7 +5,14 @@ model runs between the projections and the next token.
   read once for all lanes, each lane's own rows beside it;
 * ``lora_dev`` -- the low-rank adapters of many requests beside one projection;
 * ``token_probs_dev`` -- probabilities from logits at a temperature;
-* ``verify_drafts_dev`` -- drafted tokens against the target's probabilities.
+* ``verify_drafts_dev`` -- drafted tokens against the target's probabilities;
+* ``qk_norm_rope_dev`` -- queries and keys normed for each head and rotated by
+  their positions;
+* ``paged_append_dev`` -- the same on the way of keys and values into the pages
+  of a cache;
+* ``paged_attn_dev`` -- attention of each request's new token over its pages;
+* ``token_logprobs_dev`` -- log probabilities of given tokens, entropies and the
+  likeliest alternatives.
 
 Tensors are torch device tensors on the current device, which is the one
 ``loom_amd.init`` was given; the calls run on torch's current stream, take
@@ -21,11 +28,13 @@ import functools
 
 import torch
 
-from . import BF16, F16, F32, KvRowsDesc, LoomHipError, LoraDesc, OK, last_error, lib
+from . import (BF16, F16, F32, HeadsDesc, KvRowsDesc, LoomHipError, LoraDesc, OK, PagesDesc, RopeDesc, last_error,
+               lib)
 
 _F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
 _LORA_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _HALF = (torch.float16, torch.int16)
+_PAGE_TYPES = {torch.float16: F16, torch.int16: F16, torch.bfloat16: BF16}
 
 # A serving step makes hundreds of these calls, each a few microseconds of device work: the checks below are plain
 # comparisons, messages are formed only when one fails, and workspace sizes are remembered by the sizes they follow from.
@@ -67,6 +76,16 @@ def _probs_ws(n: int, vocab: int) -> int:
 @functools.lru_cache(maxsize=4096)
 def _verify_ws(n: int, vocab: int) -> int:
     return lib().loomhip_verify_drafts_ws(n, vocab)
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_attn_ws(*sizes) -> int:
+    return lib().loomhip_paged_attn_ws(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _logprobs_ws(n: int, vocab: int, top: int) -> int:
+    return lib().loomhip_token_logprobs_ws(n, vocab, top)
 
 
 _NO_ROWS = KvRowsDesc()
@@ -242,4 +261,194 @@ def verify_drafts_dev(target_probs, draft_tokens, u_accept, u_sample, draft_prob
     return tokens, accepted
 
 
-__all__ = ["lora_dev", "prefix_attn_dev", "token_probs_dev", "verify_drafts_dev"]
+def _heads_ok(t, n: int, heads: int, hd: int) -> bool:
+    """f32 [n, heads, hd], a token's heads one after the other, the tokens apart."""
+    if t.shape != (n, heads, hd) or t.dtype is not _F32:
+        return False
+    s = t.stride()
+    return t.is_contiguous() or ((hd == 1 or s[2] == 1) and (heads == 1 or s[1] == hd) and (n == 1 or s[0] >= heads * hd))
+
+
+def _heads_desc(x, out, norm, heads: int):
+    return HeadsDesc(x.data_ptr(), x.stride(0), None if out is None else out.data_ptr(),
+                     0 if out is None else out.stride(0), None if norm is None else norm.data_ptr(), heads)
+
+
+def _rope_desc(pos, freqs, n: int, eps: float, interleaved: bool):
+    if pos.shape != (n,) or pos.dtype is not _I32 or not pos.is_contiguous():
+        raise ValueError("pos: int32, one a token")
+    if freqs is None:
+        return RopeDesc(pos.data_ptr(), None, 0, 0, eps)
+    if freqs.dim() != 1 or freqs.dtype is not torch.float64 or not freqs.is_contiguous():
+        raise ValueError("freqs: f64 [rotated values / 2]")
+    return RopeDesc(pos.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0], interleaved, eps)
+
+
+def _norm_ok(norm, hd: int) -> bool:
+    return norm is None or _is(norm, _F32, hd)
+
+
+def qk_norm_rope_dev(q, k, pos, freqs, q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False,
+                     q_out=None, k_out=None):
+    """Queries and keys normed for each head, then rotated by their positions.
+
+    q f32 [n, n_heads, head_dim], k f32 [n, n_kv_heads, head_dim] or None, a token's heads one after the other (column
+    groups of one projection's output serve as they lie); pos int32 [n], a negative one being padding whose rows are
+    left as they were (undefined in an output made here); freqs f64 [r / 2]: the first r values of a head are rotated,
+    pair i by pos * freqs[i] radians, formed in 64 bits (None: no rotation); pairs (i, i + r / 2), or (2 i, 2 i + 1)
+    where ``interleaved``.  q_norm, k_norm f32 [head_dim]: weights of x / sqrt(mean x^2 + eps) (None: no norm).
+    ``q_out=q`` and ``k_out=k`` work in place.  Returns (q_out, k_out).
+    """
+    if q.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError("q [n, n_heads, head_dim], k [n, n_kv_heads, head_dim]")
+    n, heads, hd = q.shape
+    rope = _rope_desc(pos, freqs, n, eps, interleaved)
+    if not _norm_ok(q_norm, hd) or not _norm_ok(k_norm, hd):
+        raise ValueError(f"q_norm, k_norm: contiguous f32 [{hd}]")
+    if not _heads_ok(q, n, heads, hd) or not (q_out is None or _heads_ok(q_out, n, heads, hd)):
+        raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
+    if k is None:
+        if k_out is not None:
+            raise ValueError("k_out without k")
+    elif not _heads_ok(k, n, k.shape[1], hd) or not (k_out is None or _heads_ok(k_out, n, k.shape[1], hd)):
+        raise ValueError("k, k_out: f32 [n, n_kv_heads, head_dim] as q, a token's heads one after the other")
+    dev, stream = _place(q, k, pos, freqs, q_norm, k_norm, q_out, k_out)
+    if q_out is None:
+        q_out = torch.empty((n, heads, hd), dtype=_F32, device=dev)
+    kd = None
+    if k is not None:
+        if k_out is None:
+            k_out = torch.empty(k.shape, dtype=_F32, device=dev)
+        kd = C.byref(_heads_desc(k, k_out, k_norm, k.shape[1]))
+    rc = lib().loomhip_qk_norm_rope_dev(C.byref(_heads_desc(q, q_out, q_norm, heads)), kd, C.byref(rope), n, hd, stream)
+    if rc != OK:
+        _fail("qk_norm_rope_dev", rc)
+    return q_out, k_out
+
+
+def _pages_desc(k_pages, v_pages, table, kv: int, hd: int):
+    shape, stride = k_pages.shape, k_pages.stride()
+    kind = _PAGE_TYPES.get(k_pages.dtype)
+    if len(shape) != 4 or v_pages.shape != shape or kind is None or v_pages.dtype != k_pages.dtype:
+        raise ValueError("k_pages, v_pages: of one shape, [n_pages, page_size, n_kv_heads, head_dim], fp16 (or its bits as "
+                         "int16) or bf16")
+    if shape[2] != kv or shape[3] != hd:
+        raise ValueError(f"pages of {shape[2]} heads of {shape[3]}, not {kv} of {hd}")
+    if (v_pages.stride() != stride and any(a != b for a, b, s in zip(stride, v_pages.stride(), shape) if s > 1)) or (
+            stride[3] != 1 and hd != 1):
+        raise ValueError("k_pages, v_pages: of one layout, the values of a head one after the other")
+    if table.dim() != 2 or table.dtype is not _I32 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise ValueError("table: int32 [lanes, pages], a lane's entries one after the other")
+    return PagesDesc(k_pages.data_ptr(), v_pages.data_ptr(), kind, shape[0], shape[1], stride[0], stride[1], stride[2],
+                     table.data_ptr(), table.shape[0], table.shape[1], table.stride(0))
+
+
+def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None, k_norm=None, q=None, q_norm=None,
+                     eps: float = 1e-6, interleaved: bool = False, q_out=None):
+    """Keys and values of n tokens into a paged cache, the keys normed and rotated on the way (`qk_norm_rope_dev`).
+
+    k, v f32 [n, n_kv_heads, head_dim]; k_pages, v_pages fp16 or bf16 [n_pages, page_size, n_kv_heads, head_dim] (any
+    strides that are multiples of 8; the values of a head one after the other); table int32 [lanes, pages of a lane];
+    token t goes to position pos[t] of lane lanes[t] (int32 [n]; None: lane t).  A token of a negative position is
+    padding; one whose position has no page in the table (an entry outside the pool, a position past it) is not stored.
+    Two tokens must not have one position of one lane.  q f32 [n, n_heads, head_dim]: the tokens' queries, normed and
+    rotated in the same launch; returns q_out (``q_out=q``: in place), None without q.
+    """
+    if k.dim() != 3:
+        raise ValueError("k [n, n_kv_heads, head_dim]")
+    n, kv, hd = k.shape
+    rope = _rope_desc(pos, freqs, n, eps, interleaved)
+    if not _norm_ok(q_norm, hd) or not _norm_ok(k_norm, hd):
+        raise ValueError(f"q_norm, k_norm: contiguous f32 [{hd}]")
+    if not _heads_ok(k, n, kv, hd) or not _heads_ok(v, n, kv, hd):
+        raise ValueError("k, v: f32 [n, n_kv_heads, head_dim], a token's heads one after the other")
+    if lanes is not None and not _is(lanes, _I32, n):
+        raise ValueError("lanes: int32, one a token")
+    pages = _pages_desc(k_pages, v_pages, table, kv, hd)
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q_out without q")
+    elif q.dim() != 3 or not _heads_ok(q, n, q.shape[1], hd) or not (q_out is None or _heads_ok(q_out, n, q.shape[1], hd)):
+        raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
+    dev, stream = _place(k, v, k_pages, v_pages, table, pos, lanes, freqs, k_norm, q, q_norm, q_out)
+    qd = None
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=_F32, device=dev)
+        qd = C.byref(_heads_desc(q, q_out, q_norm, q.shape[1]))
+    rc = lib().loomhip_paged_append_dev(C.byref(pages), qd, C.byref(_heads_desc(k, None, k_norm, kv)), v.data_ptr(),
+                                        v.stride(0), None if lanes is None else lanes.data_ptr(), C.byref(rope), n, hd,
+                                        stream)
+    if rc != OK:
+        _fail("paged_append_dev", rc)
+    return q_out
+
+
+def paged_attn_dev(q, k_pages, v_pages, table, lens, scale: float, window: int = 0, out=None):
+    """Attention of one new token of each of n lanes over its pages.
+
+    q f32 [n, n_heads, head_dim] (rotated); pages and table as `paged_append_dev` fills them, n lanes or more; lane i
+    sees its first lens[i] (int32) positions, its new token's own among them, of those the last ``window`` where that is
+    not 0, and none of a page that the table does not have.  Zero where it sees nothing.  Returns out f32 as q.
+    """
+    shape = q.shape
+    if len(shape) != 3 or q.dtype is not _F32 or not q.is_contiguous():
+        raise ValueError("q: contiguous f32 [n, n_heads, head_dim]")
+    n, heads, hd = shape
+    if k_pages.dim() != 4:
+        raise ValueError("k_pages, v_pages [n_pages, page_size, n_kv_heads, head_dim]")
+    kv = k_pages.shape[2]
+    pages = _pages_desc(k_pages, v_pages, table, kv, hd)
+    if not _is(lens, _I32, n):
+        raise ValueError("lens: int32 [n]")
+    if window < 0:
+        raise ValueError("window: 0 or more")
+    if out is not None and not _is(out, _F32, *shape):
+        raise ValueError("out: as q")
+    dev, stream = _place(q, k_pages, v_pages, table, lens, out)
+    if out is None:
+        out = torch.empty_like(q)
+    nb = _paged_attn_ws(pages.page_size * pages.table_width, n, heads, kv, hd)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    rc = lib().loomhip_paged_attn_dev(C.byref(pages), q.data_ptr(), lens.data_ptr(), n, heads, kv, hd, scale, window,
+                                      out.data_ptr(), ws.data_ptr() if nb else None, nb, stream)
+    if rc != OK:
+        _fail("paged_attn_dev", rc)
+    return out
+
+
+def token_logprobs_dev(logits, tokens, top: int = 0, temperature=None):
+    """Log probabilities of given tokens under softmax(logits / temperature), the rows' entropies and alternatives.
+
+    logits f32 [..., vocab] contiguous, tokens int32 of the leading shape (one outside the vocabulary: -inf), temperature
+    f32 of it (None: 1; not positive: the first maximum alone has a probability).  Returns (logprobs, entropy) f32 of the
+    leading shape and (top_ids int32, top_logprobs f32) [..., top]: the largest logits in descending order, the lower
+    index first among equals, NaN never among them; -1 and -inf where a row has no more.
+    """
+    shape = logits.shape
+    if not shape or logits.dtype is not _F32 or not logits.is_contiguous():
+        raise ValueError("logits: contiguous f32")
+    lead, vocab = shape[:-1], shape[-1]
+    n = logits.numel() // vocab if vocab else 0
+    if not _is(tokens, _I32, *lead):
+        raise ValueError("tokens: int32, one a row")
+    if temperature is not None and not _is(temperature, _F32, *lead):
+        raise ValueError("temperature: f32, one a row")
+    if top < 0:
+        raise ValueError("top: 0 or more")
+    dev, stream = _place(logits, tokens, temperature)
+    lp, entropy = torch.empty(lead, dtype=_F32, device=dev), torch.empty(lead, dtype=_F32, device=dev)
+    ids, tops = torch.empty((*lead, top), dtype=_I32, device=dev), torch.empty((*lead, top), dtype=_F32, device=dev)
+    nb = _logprobs_ws(n, vocab, top)
+    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    rc = lib().loomhip_token_logprobs_dev(logits.data_ptr(), n, vocab, vocab, tokens.data_ptr(),
+                                          None if temperature is None else temperature.data_ptr(), top, lp.data_ptr(),
+                                          entropy.data_ptr(), ids.data_ptr(), tops.data_ptr(),
+                                          ws.data_ptr() if nb else None, nb, stream)
+    if rc != OK:
+        _fail("token_logprobs_dev", rc)
+    return lp, entropy, ids, tops
+
+
+__all__ = ["lora_dev", "paged_append_dev", "paged_attn_dev", "prefix_attn_dev", "qk_norm_rope_dev", "token_logprobs_dev",
+           "token_probs_dev", "verify_drafts_dev"]
