@@ -65,6 +65,12 @@ __device__ __forceinline__ void pg_split(float x, int e, typename T::v8 (&p)[T::
     }
 }
 
+// The items, (lane, key head, block) numbered in this order, that a run of rows begins in the middle of, and leaves in
+// the middle of after their first row; -1: none.
+struct PgDesc {
+    int32_t head, tail;
+};
+
 struct PagedAttnParams {
     loomhip_pages c;
     const float *q;
@@ -73,6 +79,9 @@ struct PagedAttnParams {
     uint32_t window;                         // 0: none
     float scale;
     float *out;
+    PgDesc *desc; // [runs]
+    float *part;  // [runs][2][PG_COLS][hd]
+    float2 *ml;   // [runs][2][PG_COLS]
 };
 
 // Rows [first, end) that lane i sees.
@@ -295,8 +304,39 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
     __syncthreads();
 }
 
+// What the waves left joined, for the thread's head and four columns: 2^(m - M) o summed, and M and l.
+template <int HDP>
+__device__ __forceinline__ pg_f4 pg_join(const char *smem, float (*sm)[PG_COLS], float (*sl)[PG_COLS], int h, int d,
+                                         float &M, float &L) {
+    using C = PgCfg<HDP>;
+    const float *so = (const float *)smem;
+    M = sm[0][h];
+#pragma unroll
+    for (int w = 1; w < PG_WAVES; w++)
+        M = fmaxf(M, sm[w][h]);
+    L = 0.0f;
+    pg_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < PG_WAVES; w++) {
+        const float f = sm[w][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][h] - M);
+        L += sl[w][h] * f;
+        a += *(const pg_f4 *)(so + (w * PG_COLS + h) * C::OS + d) * f;
+    }
+    return a;
+}
+// The result of sums a and L: zero where nothing was seen.  An infinity here comes from a cached one, which the
+// weights' second parts turn into NaN for some heads and not for others: NaN for all.
+__device__ __forceinline__ pg_f4 pg_result(pg_f4 a, float L) {
+    a *= L == 0.0f ? 0.0f : 1.0f / L;
+    return a + a * 0.0f;
+}
+
+template <int HDP>
+constexpr int pg_groups = HDP == 256 ? 1 : 2; // work groups of a CU (LDS and registers)
+
+// One item (lane, key head, block of its query heads) a work group: all of the lane's rows.
 template <class T, int HDP>
-__global__ __launch_bounds__(PG_THREADS, HDP == 256 ? 1 : 2) void paged_attn_kernel(PagedAttnParams P) {
+__global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
@@ -306,26 +346,177 @@ __global__ __launch_bounds__(PG_THREADS, HDP == 256 ? 1 : 2) void paged_attn_ker
     uint32_t r0, r1;
     pg_span(P, i, r0, r1);
     pg_rows<T, HDP>(P, i, kvh, h0, heads, r0, r1, smem, sm, sl);
-    const float *so = (const float *)smem;
     for (int x = threadIdx.x; x < heads * (HDP / 4); x += PG_THREADS) {
         const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
-        float M = sm[0][h];
-#pragma unroll
-        for (int w = 1; w < PG_WAVES; w++)
-            M = fmaxf(M, sm[w][h]);
-        float L = 0.0f;
-        pg_f4 a = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < PG_WAVES; w++) {
-            const float f = sm[w][h] == M ? 1.0f : __builtin_amdgcn_exp2f(sm[w][h] - M);
-            L += sl[w][h] * f;
-            a += *(const pg_f4 *)(so + (w * PG_COLS + h) * C::OS + d) * f;
-        }
-        a *= L == 0.0f ? 0.0f : 1.0f / L; // nothing seen: zero
-        // an infinity here comes from a cached one, which the weights' second parts turn into NaN for some: NaN for all
+        float M, L;
+        const pg_f4 a = pg_join<HDP>(smem, sm, sl, h, d, M, L);
         if (d < P.hd)
-            *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = a + a * 0.0f;
+            *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = pg_result(a, L);
     }
+}
+
+// The same with the rows of all items laid end to end, in units of a tile for
+// each wave, and cut into equal runs, one for each work group of the grid (as
+// many as the chip holds at a time): the lengths decide on the device who does
+// what.  An item that lies in one run is finished there.  Of one that runs on,
+// every work group leaves a record (m, l, o), at most two each: of the item
+// that came from before (slot 0) and of the one that goes on (slot 1).
+template <class T, int HDP>
+__global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_kernel(PagedAttnParams P) {
+    using C = PgCfg<HDP>;
+    constexpr uint32_t UNIT = PG_WAVES * C::KT;
+    __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
+    __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
+    __shared__ uint64_t scan[PG_WAVES];
+    __shared__ uint64_t before; // units before the run's first lane
+    __shared__ int found;       // that lane
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = blockIdx.x, W = gridDim.x;
+    const uint32_t items = (uint32_t)P.n_kv * P.blocks; // of a lane
+    const auto units = [&](int i) {
+        uint32_t first, end;
+        pg_span(P, i, first, end);
+        return (end - first + UNIT - 1) / UNIT;
+    };
+    // lanes that see nothing
+    for (int i = w; i < P.n; i += W)
+        if (units(i) == 0)
+            for (int x = tid * 4; x < P.n_heads * P.hd; x += PG_THREADS * 4)
+                *(pg_f4 *)(P.out + (size_t)i * P.n_heads * P.hd + x) = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    // every thread's lanes, a run of them, and their units
+    const int per = (P.n + PG_THREADS - 1) / PG_THREADS;
+    uint64_t mine = 0;
+    for (int i = tid * per; i < (tid + 1) * per && i < P.n; i++)
+        mine += units(i);
+    uint64_t upto = mine;
+    for (int o = 1; o < 64; o *= 2) {
+        const uint64_t x = (uint64_t)__shfl_up((long long)upto, o);
+        upto += lane >= o ? x : 0;
+    }
+    if (lane == 63)
+        scan[wave] = upto;
+    __syncthreads();
+    uint64_t all = 0;
+#pragma unroll
+    for (int x = 0; x < PG_WAVES; x++) {
+        upto += x < wave ? scan[x] : 0;
+        all += scan[x];
+    }
+    const uint64_t total = all * items;
+    const int runs = total < (uint64_t)W ? (int)total : W;
+    if (w >= runs) {
+        if (tid == 0)
+            P.desc[w] = {-1, -1};
+        return;
+    }
+    const auto run_at = [&](int x) { return total / runs * x + total % runs * x / runs; };
+    const uint64_t from = run_at(w), to = run_at(w + 1);
+    if ((upto - mine) * items <= from && from < upto * items) {
+        uint64_t sum = upto - mine;
+        int i = tid * per;
+        for (uint32_t u = units(i); (sum + u) * items <= from; u = units(++i))
+            sum += u;
+        found = i, before = sum;
+    }
+    __syncthreads();
+    int i = found;
+    uint32_t u = units(i);
+    const uint64_t rest = from - before * items; // into the lane's units
+    uint32_t item = (uint32_t)(rest / u), j = (uint32_t)(rest - (uint64_t)item * u);
+    PgDesc desc = {-1, -1};
+    for (uint64_t at = from; at < to;) {
+        const uint32_t j1 = to - at < u - j ? j + (uint32_t)(to - at) : u; // units [j, j1) of the item's u
+        const int kvh = item / P.blocks, block = item - kvh * P.blocks, h0 = kvh * P.group + block * PG_COLS;
+        const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
+        uint32_t first, end;
+        pg_span(P, i, first, end);
+        const uint32_t r1 = end - first < j1 * UNIT ? end : first + j1 * UNIT;
+        pg_rows<T, HDP>(P, i, kvh, h0, heads, first + j * UNIT, r1, smem, sm, sl);
+        const bool whole = j == 0 && j1 == u;
+        const int slot = w * 2 + (j == 0);
+        if (!whole)
+            (j ? desc.head : desc.tail) = i * (int)items + (int)item;
+        for (int x = tid; x < heads * (HDP / 4); x += PG_THREADS) {
+            const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
+            float M, L;
+            const pg_f4 a = pg_join<HDP>(smem, sm, sl, h, d, M, L);
+            if (d < P.hd) {
+                if (whole)
+                    *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = pg_result(a, L);
+                else
+                    *(pg_f4 *)(P.part + ((size_t)slot * PG_COLS + h) * P.hd + d) = a;
+            }
+            if (!whole && d == 0)
+                P.ml[slot * PG_COLS + h] = make_float2(M, L);
+        }
+        __syncthreads(); // the join is read: its room is the next tiles'
+        at += j1 - j;
+        j = 0;
+        if (j1 == u && ++item == items) {
+            item = 0;
+            while (at < to && (u = units(++i)) == 0) {
+            }
+        }
+    }
+    if (tid == 0)
+        P.desc[w] = desc;
+}
+
+// An item's records joined, a work group for a query head of the item that
+// goes on from run blockIdx.x: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
+template <int HDP>
+__global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnParams P, int runs) {
+    constexpr int LPR = HDP / 4, PAR = PG_THREADS / LPR; // threads of a record, records side by side
+    __shared__ pg_f4 so[PAR][LPR];
+    __shared__ float sl[PAR];
+    const int w = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+    const int seg = P.desc[w].tail;
+    if (seg < 0)
+        return;
+    const int items = P.n_kv * P.blocks, i = seg / items, item = seg - i * items, kvh = item / P.blocks;
+    const int block = item - kvh * P.blocks;
+    if (h >= P.group - block * PG_COLS)
+        return;
+    int n = 1; // records: this run's second and the next runs' first ones
+    for (int x = w + 1; x < runs; x += 64) {
+        const int k = __popcll(__ballot(x + lane < runs && P.desc[x + lane].head == seg));
+        n += k;
+        if (k < 64)
+            break;
+    }
+    const auto slot = [&](int r) { return r == 0 ? w * 2 + 1 : (w + r) * 2; };
+    float M = -__builtin_inff();
+    for (int r = lane; r < n; r += 64)
+        M = fmaxf(M, P.ml[slot(r) * PG_COLS + h].x);
+    M = wave_max(M);
+    const int g = tid / LPR, d = tid % LPR * 4;
+    float l = 0.0f;
+    pg_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int r = g; r < n; r += PAR) {
+        const int s = slot(r) * PG_COLS + h;
+        const float2 ml = P.ml[s];
+        const pg_f4 v = d < P.hd ? *(const pg_f4 *)(P.part + (size_t)s * P.hd + d) : pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        l += ml.y * f;
+        o += v * f;
+    }
+    so[g][tid % LPR] = o;
+    if (d == 0)
+        sl[g] = l;
+    __syncthreads();
+    if (g == 0 && d < P.hd) {
+#pragma unroll
+        for (int x = 1; x < PAR; x++)
+            o += so[x][tid], l += sl[x];
+        *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + kvh * P.group + block * PG_COLS + h) * P.hd + d) = pg_result(o, l);
+    }
+}
+
+// Work groups that run at a time.
+static int pg_runs(size_t hd) { return hd > 128 ? 256 : 512; }
+constexpr size_t PG_WHOLE = 256; // rows up to which a lane is not cut
+static size_t pg_ws_bytes(size_t max_rows, size_t hd) {
+    return max_rows <= PG_WHOLE ? 0 : (size_t)pg_runs(hd) * (sizeof(PgDesc) + 2 * PG_COLS * (hd * 4 + sizeof(float2)));
 }
 
 } // namespace lh
@@ -341,7 +532,7 @@ static bool pg_served(size_t n, size_t n_heads, size_t n_kv, size_t hd) {
 extern "C" {
 
 size_t loomhip_paged_attn_ws(size_t max_rows, size_t n, size_t n_heads, size_t n_kv_heads, size_t head_dim) {
-    return 0;
+    return pg_served(n, n_heads, n_kv_heads, head_dim) ? pg_ws_bytes(max_rows, head_dim) : 0;
 }
 
 int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
@@ -362,6 +553,9 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
         return fail(LOOMHIP_ERR_ARG, "%s: lengths not aligned to their elements", fn);
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
         return fail(LOOMHIP_DECLINED, "%s: q or out not at a multiple of 16 bytes", fn);
+    const size_t need = pg_ws_bytes(c->page_size * c->table_width, head_dim);
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
+        return fail(LOOMHIP_ERR_ARG, "%s: the workspace takes %zu bytes at a multiple of 16, got %zu", fn, need, ws_bytes);
     if (int rc = require_device())
         return rc;
     PagedAttnParams P = {};
@@ -378,21 +572,38 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
     P.scale = scale;
     P.out = out;
     hipStream_t st = stream_of(stream);
-    const auto run = [&](auto type) {
+    const int runs = pg_runs(head_dim);
+    if (need) {
+        P.desc = (PgDesc *)ws;
+        P.ml = (float2 *)(P.desc + runs);
+        P.part = (float *)(P.ml + runs * 2 * PG_COLS);
+    }
+    const auto run = [&](auto type, auto size) {
         using T = decltype(type);
-        const dim3 g(n * n_kv_heads * P.blocks), b(PG_THREADS);
+        constexpr int HDP = decltype(size)::value;
+        if (!need) {
+            hipLaunchKernelGGL((paged_attn_kernel<T, HDP>), dim3(n * n_kv_heads * P.blocks), dim3(PG_THREADS), 0, st, P);
+            note_launch();
+            return;
+        }
+        hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP>), dim3(runs), dim3(PG_THREADS), 0, st, P);
+        hipLaunchKernelGGL((paged_attn_join_kernel<HDP>), dim3(runs, P.group < PG_COLS ? P.group : PG_COLS),
+                           dim3(PG_THREADS), 0, st, P, runs);
+        note_launch();
+        note_launch();
+    };
+    const auto sized = [&](auto type) {
         if (head_dim <= 64)
-            hipLaunchKernelGGL((paged_attn_kernel<T, 64>), g, b, 0, st, P);
+            run(type, std::integral_constant<int, 64>{});
         else if (head_dim <= 128)
-            hipLaunchKernelGGL((paged_attn_kernel<T, 128>), g, b, 0, st, P);
+            run(type, std::integral_constant<int, 128>{});
         else
-            hipLaunchKernelGGL((paged_attn_kernel<T, 256>), g, b, 0, st, P);
+            run(type, std::integral_constant<int, 256>{});
     };
     if (c->type == LH_F16)
-        run(PgF16{});
+        sized(PgF16{});
     else
-        run(PgBf16{});
-    note_launch();
+        sized(PgBf16{});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "paged_attn launch");
 }
