@@ -19,7 +19,10 @@
 namespace lh {
 
 constexpr int LP_MAX_TOP = 32;
-constexpr int LP_LIST = 1024;      // values collected at most
+constexpr int LP_WAVES = SMP_THREADS / 64;
+constexpr int LP_LIST = 64;        // values collected of a wave at most
+constexpr int LP_PAD = 8;          // they are read in pieces of this
+constexpr int LP_SPARE = 4;        // threads whose maxima reach the bound beside the k
 constexpr int LP_JOIN_N = 16;      // entries a thread joins
 constexpr size_t LP_JOIN = SMP_THREADS * LP_JOIN_N; // a row's parts times top at most
 constexpr size_t LP_ROW = 32768;   // one launch up to this row
@@ -57,103 +60,169 @@ __device__ __forceinline__ float lp_value(uint32_t o) {
 // A value's key: the larger one is the better, of equal values the one of the lower index; 0 is no value.
 __device__ __forceinline__ uint64_t lp_key(float x, int id) { return (uint64_t)lp_order(x) << 32 | (uint32_t)~id; }
 
-template <int THREADS>
 struct LpShared {
-    static constexpr int W = THREADS / 64;
-    float m[W], s[W], z[W];
-    int at[W];
-    uint64_t key[W];
-    int count;
-    __attribute__((aligned(16))) uint64_t list[LP_LIST + 2];
+    float m[LP_WAVES], s[LP_WAVES], z[LP_WAVES];
+    int at[LP_WAVES];
+    uint32_t top[SMP_THREADS], bound;
+    bool ties;
+    uint64_t key[LP_WAVES];
+    uint32_t count[LP_WAVES];
+    __attribute__((aligned(16))) uint64_t list[LP_WAVES][LP_LIST];
     LpTop best[LP_MAX_TOP];
 };
 
 // The k best of the work group's values (x(j) with index id(j), j < N, of every thread; NaN and indices from `end` on
-// are none) into sh.best, in order.
-template <int THREADS, int N, class X, class Id>
-__device__ __forceinline__ void lp_select(int k, X x, Id id, int end, LpShared<THREADS> &sh) {
-    constexpr int W = THREADS / 64;
+// are none) into sh.best, in order, for the first wave to read.
+template <int N, class X, class Id>
+__device__ __forceinline__ void lp_select(int k, X x, Id id, int end, LpShared &sh) {
+    constexpr int W = LP_WAVES, LIST = LP_LIST, Q = N % 4 ? 1 : 4; // values are looked at by Q
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const auto here = [&](int j) { return x(j) == x(j) && id(j) < end; };
-    float mx = -__builtin_inff();
+    float mq[N / Q], mx = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < N; j++)
-        mx = fmaxf(mx, x(j));
+    for (int j = 0; j < N / Q; j++) {
+        mq[j] = x(j * Q);
+#pragma unroll
+        for (int c = 1; c < Q; c++)
+            mq[j] = fmaxf(mq[j], x(j * Q + c));
+        mx = fmaxf(mx, mq[j]);
+    }
     bool any = mx > -__builtin_inff();
     if (!any) { // -inf is a value too
 #pragma unroll
         for (int j = 0; j < N; j++)
             any |= here(j);
     }
-    // the wave's k-th largest of its lanes' maxima: the largest number that k of them reach
-    const uint32_t o = any ? lp_order(mx) : 0;
-    uint32_t t = 0;
-    for (int b = 31; b >= 0; b--)
-        if (__popcll(__ballot(o >= (t | 1u << b))) >= k)
-            t |= 1u << b;
-    int last = end - 1; // of the values equal to it those up to this index
-    if (t) {
-        const uint64_t eq = __ballot(o == t);
-        const int need = k - __popcll(__ballot(o > t));
-        if (__popcll(eq) > need) { // the need-th lowest of the lanes' first indices
-            int first = 0x7fffffff;
-            if (o == t)
+    // The bound: a number that k of the threads' maxima reach and not many more, or the k-th largest of them.  The first
+    // wave looks for it, bit by bit.
+    sh.top[tid] = any ? lp_order(mx) : 0;
+    __syncthreads();
+    constexpr uint32_t LEAST = 0x007fffffu; // the order of -inf
+    if (wave == 0) {
+        uint32_t o[W], t = 0;
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (x(j) == mx && id(j) < first)
-                        first = id(j);
-            uint32_t below = 0;
-            for (int b = 30; b >= 0; b--)
-                if (__popcll(__ballot((uint32_t)first < (below | 1u << b))) < need)
-                    below |= 1u << b;
-            last = (int)below;
+        for (int w = 0; w < W; w++)
+            o[w] = sh.top[w * 64 + lane];
+        const auto reach = [&](uint32_t t) {
+            int c = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                c += __popcll(__ballot(o[w] >= t));
+            return c;
+        };
+        int b = 31, most = 0; // how many reach t
+        // the largest's sign and most of its exponent are most often those of the k-th largest too
+        float big = lp_value(o[0] > LEAST ? o[0] : LEAST);
+#pragma unroll
+        for (int w = 1; w < W; w++)
+            big = fmaxf(big, lp_value(o[w] > LEAST ? o[w] : LEAST));
+        const uint32_t head = lp_order(wave_max(big)) & 0xff000000u;
+        if (head && reach(head) >= k) {
+            t = head;
+            most = reach(head);
+            b = 23;
+        }
+        for (; b >= 0 && (most < k || most > k + LP_SPARE); b--) {
+            const int c = reach(t | 1u << b);
+            t |= c >= k ? 1u << b : 0;
+            most = c >= k ? c : most;
+        }
+        if (lane == 0) {
+            sh.bound = t && t < LEAST ? LEAST : t;
+            sh.ties = t && most > k + LP_SPARE;
         }
     }
-    if (lane == 0)
-        sh.key[wave] = t ? (uint64_t)t << 32 | (uint32_t)~last : 0;
-    if (tid == 0)
-        sh.count = 0;
     __syncthreads();
-    uint64_t bound = sh.key[0];
+    const uint32_t t = sh.bound;
+    int upto = end - 1; // of the values equal to it those up to this index
+    if (sh.ties) {      // many are equal to it: up to the index that makes up k of the threads' first ones
+        int first = 0x7fffffff;
+        if (sh.top[tid] == t)
 #pragma unroll
-    for (int w = 1; w < W; w++)
-        bound = sh.key[w] > bound ? sh.key[w] : bound;
-    const float from = bound ? lp_value((uint32_t)(bound >> 32)) : -__builtin_inff();
-    const int upto = bound ? (int)~(uint32_t)bound : end - 1;
-    const auto reaches = [&](int j) { return x(j) > from || (x(j) == from && id(j) <= upto); };
-    int mine = 0;
-#pragma unroll
-    for (int j = 0; j < N; j++)
-        mine += reaches(j);
-    int at = mine ? atomicAdd(&sh.count, mine) : 0;
-    if (mine) {
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            if (reaches(j)) {
-                if (at < LP_LIST)
-                    sh.list[at] = lp_key(x(j), id(j));
-                at++;
-            }
-    }
-    __syncthreads();
-    const int count = sh.count;
-    if (count <= LP_LIST) {
-        if (tid == 0)
-            sh.list[count] = 0; // read in pairs
-        for (int r = count + tid; r < k; r += THREADS)
-            sh.best[r] = {-__builtin_inff(), -1};
+            for (int j = 0; j < N; j++)
+                if (x(j) == mx && id(j) < first)
+                    first = id(j);
+        const uint64_t over = __ballot(sh.top[tid] > t);
+        if (lane == 0)
+            sh.count[wave] = __popcll(over);
         __syncthreads();
-        for (int c = tid; c < count; c += THREADS) {
-            const uint64_t key = sh.list[c];
-            int rank = 0;
-            for (int j = 0; j < count; j += 2)
-                rank += (sh.list[j] > key) + (sh.list[j + 1] > key);
-            if (rank < k)
-                sh.best[rank] = {lp_value((uint32_t)(key >> 32)), (int)~(uint32_t)key};
+        sh.top[tid] = (uint32_t)first;
+        __syncthreads();
+        uint32_t o[W], below = 0;
+        int need = k;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            o[w] = sh.top[w * 64 + lane];
+            need -= (int)sh.count[w];
+        }
+        for (int b = 30; b >= 0; b--) {
+            int c = 0;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                c += __popcll(__ballot(o[w] < (below | 1u << b)));
+            below |= c < need ? 1u << b : 0;
+        }
+        upto = (int)below;
+        __syncthreads(); // count is read
+    }
+    const float from = t ? lp_value(t) : -__builtin_inff();
+    // what reaches the bound, into the wave's part of the list
+    uint32_t mine = 0;
+    const auto collect = [&](auto reaches) {
+#pragma unroll
+        for (int g = 0; g < N / Q; g++)
+            if (__any(mq[g] >= from))
+#pragma unroll
+                for (int j = g * Q; j < g * Q + Q; j++) {
+                    const uint64_t b = __ballot(reaches(j));
+                    if (b) {
+                        const uint32_t at = mine + __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32),
+                                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+                        if ((b >> lane & 1) && at < LIST)
+                            sh.list[wave][at] = lp_key(x(j), id(j));
+                        mine += __popcll(b);
+                    }
+                }
+    };
+    if (__any(mx >= from)) {
+        if (from > -__builtin_inff() && upto == end - 1) // no tie to be told apart: the index says nothing
+            collect([&](int j) { return x(j) >= from; });
+        else
+            collect([&](int j) { return x(j) > from || (x(j) == from && id(j) <= upto); });
+    }
+    if (lane == 0)
+        sh.count[wave] = mine;
+    if (mine + lane < LIST) // zeros, before no other, behind them
+        sh.list[wave][mine + lane] = 0;
+    __syncthreads();
+    uint32_t most = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        all += sh.count[w];
+        most = sh.count[w] > most ? sh.count[w] : most;
+    }
+    if (most <= LIST) {
+        if (wave == 0) {
+            if ((uint32_t)lane >= all && lane < k)
+                sh.best[lane] = {-__builtin_inff(), -1};
+            // sixteen of each wave's at a time, each counting those before it
+            for (uint32_t i = lane & 15; i - (lane & 15) < most; i += 16) {
+                const uint64_t key = sh.list[lane >> 4][i];
+                int rank = 0;
+                for (uint32_t j = 0; j < most; j += LP_PAD)
+#pragma unroll
+                    for (int w = 0; w < W; w++)
+#pragma unroll
+                        for (int e = 0; e < LP_PAD; e++)
+                            rank += sh.list[w][j + e] > key;
+                if (key && rank < k)
+                    sh.best[rank] = {lp_value((uint32_t)(key >> 32)), (int)~(uint32_t)key};
+            }
+            wave_lds_sync();
         }
     } else {
         uint64_t before = ~0ull;
-        for (int r = 0; r < k; r++) { // count > k: there are k
+        for (int r = 0; r < k; r++) { // there are k
             uint64_t best = 0;
 #pragma unroll
             for (int j = 0; j < N; j++) {
@@ -175,62 +244,77 @@ __device__ __forceinline__ void lp_select(int k, X x, Id id, int end, LpShared<T
             if (tid == 0)
                 sh.best[r] = {lp_value((uint32_t)(best >> 32)), (int)~(uint32_t)best};
         }
+        __syncthreads();
     }
-    __syncthreads();
 }
 
-// A row's results from its sums and its best: lp, entropy and the alternatives, by the work group's first lanes.
+// A row's sums, and of them every thread's log S.
 struct LpRow {
     float m;
     double s, z;
     int at;
 };
-__device__ __forceinline__ float lp_of(const LpRow &r, const ProbScale &sc, float t, float x, int id) {
-    if (sc.greedy)
-        return id == r.at && r.m > -__builtin_inff() ? 0.0f : -__builtin_inff();
-    if (r.s != r.s)
-        return __builtin_nanf("");
-    if (x == -__builtin_inff())
-        return x;
-    return (float)(((double)x - (double)r.m) / (double)t - log(r.s));
+// The given token and its logit, loaded by every thread before anything is waited for.
+struct LpGiven {
+    int id;
+    float x;
+};
+__device__ __forceinline__ LpGiven lp_given(const LogprobParams &P, size_t row) {
+    const int id = P.tokens[row];
+    const bool in = id >= 0 && (uint32_t)id < (uint32_t)P.vocab;
+    return {in ? id : -1, P.logits[row * P.stride + (in ? id : 0)]};
 }
+// A row's results: a thread of the first wave for each of the best, one of the second for the given token, of the third
+// for the entropy.
 __device__ __forceinline__ void lp_write(const LogprobParams &P, size_t row, const LpRow &r, const ProbScale &sc,
-                                         const LpTop *best) {
+                                         const LpGiven &g, const LpTop *best) {
     const int tid = threadIdx.x;
-    const float t = P.temperature ? P.temperature[row] : 1.0f;
-    if (tid == 0) {
-        const int64_t id = P.tokens[row];
-        P.lp[row] = id >= 0 && id < (int64_t)P.vocab ? lp_of(r, sc, t, P.logits[row * P.stride + id], (int)id)
-                                                     : -__builtin_inff();
-        // nothing above -inf: no token has a probability
-        P.entropy[row] = sc.greedy || r.s == 0.0 ? 0.0f : (float)(log(r.s) - r.z / r.s);
-    }
+    if (tid >= P.top && tid != 64 && tid != 128)
+        return;
+    const LpTop b = tid < P.top ? best[tid] : LpTop{g.x, g.id};
+    const double log_s = log(r.s);
+    float lp;
+    if (b.id < 0)
+        lp = -__builtin_inff();
+    else if (sc.greedy)
+        lp = b.id == r.at && r.m > -__builtin_inff() ? 0.0f : -__builtin_inff();
+    else if (r.s != r.s)
+        lp = __builtin_nanf("");
+    else if (b.x == -__builtin_inff())
+        lp = b.x;
+    else
+        lp = (float)(((double)b.x - (double)r.m) / (P.temperature ? (double)P.temperature[row] : 1.0) - log_s);
     if (tid < P.top) {
-        const LpTop b = best[tid];
         P.top_ids[row * P.top + tid] = b.id;
-        P.top_lp[row * P.top + tid] = b.id < 0 ? -__builtin_inff() : lp_of(r, sc, t, b.x, b.id);
+        P.top_lp[row * P.top + tid] = lp;
+    } else if (tid == 64) {
+        P.lp[row] = lp;
+    } else { // nothing above -inf: no token has a probability
+        P.entropy[row] = sc.greedy || r.s == 0.0 ? 0.0f : (float)(log_s - r.z / r.s);
     }
 }
 
 // (m, S, Z) of the values a work group holds; Z in z log2 e.
-template <int THREADS, int NV>
-__device__ __forceinline__ LpRec lp_sums(const smp_f4 (&v)[NV], size_t v0, const ProbScale &sc, LpShared<THREADS> &sh) {
-    constexpr int W = THREADS / 64;
+template <int NV>
+__device__ __forceinline__ LpRec lp_sums(const smp_f4 (&v)[NV], size_t v0, const ProbScale &sc, LpShared &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float m = -__builtin_inff();
     int at = 0x7fffffff;
+    bool nan = false;
     if (sc.greedy) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++)
-                max_first(m, at, v[i][c], (int)(v0 + ((size_t)i * THREADS + tid) * 4 + c));
+                max_first(m, at, v[i][c], (int)(v0 + ((size_t)i * SMP_THREADS + tid) * 4 + c));
         for (int o = 1; o < 64; o *= 2)
             max_first(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
-    } else { // fmaxf passes a NaN over; its exponential is NaN, and with it the sums
+    } else { // fmaxf passes a NaN over
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-            m = fmaxf(fmaxf(fmaxf(m, v[i][0]), v[i][1]), fmaxf(v[i][2], v[i][3]));
+        for (int i = 0; i < NV; i++) {
+            m = fmaxf(m, fmaxf(fmaxf(fmaxf(v[i][0], v[i][1]), v[i][2]), v[i][3]));
+            nan |= __builtin_isunordered(v[i][0], v[i][1]) | __builtin_isunordered(v[i][2], v[i][3]);
+        }
         m = wave_max(m);
     }
     if (lane == 0)
@@ -238,20 +322,36 @@ __device__ __forceinline__ LpRec lp_sums(const smp_f4 (&v)[NV], size_t v0, const
     __syncthreads();
     m = sh.m[0], at = sh.at[0];
 #pragma unroll
-    for (int w = 1; w < W; w++)
+    for (int w = 1; w < LP_WAVES; w++)
         max_first(m, at, sh.m[w], sh.at[w]);
     if (sc.greedy)
         return {m, 1.0f, 0.0f, at};
-    const float from = m == -__builtin_inff() ? 0.0f : m;
+    // (x - m) / T log2 e = d hi + d lo; d no further below than where the exponential has long been 0, so that neither
+    // product is infinite.  At a T that no f32 is that far below, -inf is told apart.
+    const float from = m == -__builtin_inff() ? 0.0f : m, least = -300.0f / sc.hi;
     float s = 0.0f, z = 0.0f;
+    const auto add = [&](float x, bool finite) {
+        const float d = finite ? fmaxf(x - from, least) : x - from, h = __builtin_fmaf(d, sc.hi, d * sc.lo);
+        const float e = __builtin_amdgcn_exp2f(h);
+        s += e;
+        z = __builtin_fmaf(e, h, z);
+    };
+    if (least > -3.0e38f) {
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+        for (int i = 0; i < NV; i++)
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const float d = v[i][c] - from, e = exp_scaled(d, sc.hi, sc.lo);
-            s += e;
-            z = __builtin_fmaf(e, fmaxf(d * sc.hi, -200.0f), z); // e is 0 from -150 on, where d * hi may be -inf
-        }
+            for (int c = 0; c < 4; c++)
+                add(v[i][c], true);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (v[i][c] != -__builtin_inff())
+                    add(v[i][c], false);
+    }
+    if (nan || m == __builtin_inff()) // lost on the way
+        s = __builtin_nanf("");
     for (int o = 1; o < 64; o *= 2) {
         s += __shfl_xor(s, o);
         z += __shfl_xor(z, o);
@@ -261,54 +361,70 @@ __device__ __forceinline__ LpRec lp_sums(const smp_f4 (&v)[NV], size_t v0, const
     __syncthreads();
     s = sh.s[0], z = sh.z[0];
 #pragma unroll
-    for (int w = 1; w < W; w++)
+    for (int w = 1; w < LP_WAVES; w++)
         s += sh.s[w], z += sh.z[w];
     return {m, s, z, at};
 }
 
-template <int THREADS, int NV>
-__global__ __launch_bounds__(THREADS) void logprobs_row_kernel(LogprobParams P) {
-    __shared__ LpShared<THREADS> sh;
+// The values of row part v0 .. that a thread holds, as lp_select takes them.
+template <int NV>
+__device__ __forceinline__ void lp_best(const LogprobParams &P, const smp_f4 (&v)[NV], size_t v0, LpShared &sh) {
+    const int first = (int)v0 + (int)threadIdx.x * 4;
+    lp_select<NV * 4>(
+        P.top, [&](int j) { return v[j / 4][j % 4]; }, [&](int j) { return first + (j / 4) * SMP_THREADS * 4 + j % 4; },
+        (int)P.vocab, sh);
+}
+
+template <int NV>
+__global__ __launch_bounds__(SMP_THREADS, NV == 32 ? 1 : 2) void logprobs_row_kernel(LogprobParams P) {
+    __shared__ LpShared sh;
     const size_t row = blockIdx.x;
-    const int tid = threadIdx.x;
     smp_f4 v[NV];
-    row_part<NV, THREADS>(P.logits + row * P.stride, 0, P.vocab, -__builtin_inff(), v);
+    row_part<NV>(P.logits + row * P.stride, 0, P.vocab, -__builtin_inff(), v);
+    const LpGiven given = lp_given(P, row);
     const ProbScale sc = prob_scale(P.temperature, row);
-    const LpRec r = lp_sums<THREADS, NV>(v, 0, sc, sh);
+    const LpRec r = lp_sums<NV>(v, 0, sc, sh);
     if (P.top)
-        lp_select<THREADS, NV * 4>(
-            P.top, [&](int j) { return v[j / 4][j % 4]; },
-            [&](int j) { return ((j / 4) * THREADS + tid) * 4 + j % 4; }, (int)P.vocab, sh);
-    lp_write(P, row, {r.m, (double)r.s, (double)r.z * 0x1.62e42fefa39efp-1, r.at}, sc, sh.best);
+        lp_best<NV>(P, v, 0, sh);
+    lp_write(P, row, {r.m, (double)r.s, (double)r.z * 0x1.62e42fefa39efp-1, r.at}, sc, given, sh.best);
 }
 
 template <int NV>
 __global__ __launch_bounds__(SMP_THREADS) void logprobs_part_kernel(LogprobParams P) {
-    __shared__ LpShared<SMP_THREADS> sh;
+    __shared__ LpShared sh;
     const size_t row = blockIdx.x / P.splits, part = blockIdx.x;
     const int tid = threadIdx.x;
     const size_t v0 = (part - row * P.splits) * (NV * SMP_THREADS * 4);
     smp_f4 v[NV];
     row_part<NV>(P.logits + row * P.stride, v0, P.vocab, -__builtin_inff(), v);
     const ProbScale sc = prob_scale(P.temperature, row);
-    const LpRec r = lp_sums<SMP_THREADS, NV>(v, v0, sc, sh);
+    const LpRec r = lp_sums<NV>(v, v0, sc, sh);
     if (tid == 0)
         P.rec[part] = r;
     if (P.top) {
-        lp_select<SMP_THREADS, NV * 4>(
-            P.top, [&](int j) { return v[j / 4][j % 4]; },
-            [&](int j) { return (int)v0 + ((j / 4) * SMP_THREADS + tid) * 4 + j % 4; }, (int)P.vocab, sh);
+        lp_best<NV>(P, v, v0, sh);
         if (tid < P.top)
             P.list[part * P.top + tid] = sh.best[tid];
     }
 }
 
+// N: entries of the parts' best that a thread takes
+template <int N>
 __global__ __launch_bounds__(SMP_THREADS) void logprobs_join_kernel(LogprobParams P) {
-    __shared__ LpShared<SMP_THREADS> sh;
+    __shared__ LpShared sh;
     __shared__ double ss[SMP_THREADS / 64], sz[SMP_THREADS / 64];
     const size_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const LpRec *rec = P.rec + row * P.splits;
+    LpTop e[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int i = j * SMP_THREADS + tid;
+        e[j] = {__builtin_nanf(""), -1};
+        if (i < P.splits * P.top)
+            e[j] = P.list[row * P.splits * P.top + i];
+    }
+    const LpGiven given = lp_given(P, row);
     const ProbScale sc = prob_scale(P.temperature, row);
     float m = -__builtin_inff();
     int at = 0x7fffffff;
@@ -344,27 +460,18 @@ __global__ __launch_bounds__(SMP_THREADS) void logprobs_join_kernel(LogprobParam
     for (int w = 1; w < SMP_THREADS / 64; w++)
         s += ss[w], z += sz[w];
     if (P.top) {
-        const LpTop *list = P.list + row * P.splits * P.top;
-        const int all = P.splits * P.top;
-        LpTop e[LP_JOIN_N];
 #pragma unroll
-        for (int j = 0; j < LP_JOIN_N; j++) {
-            const int i = j * SMP_THREADS + tid;
-            e[j] = {__builtin_nanf(""), 0};
-            if (i < all) {
-                e[j] = list[i];
-                e[j].x = e[j].id < 0 ? __builtin_nanf("") : e[j].x;
-            }
-        }
-        lp_select<SMP_THREADS, LP_JOIN_N>(
+        for (int j = 0; j < N; j++)
+            e[j].x = e[j].id < 0 ? __builtin_nanf("") : e[j].x;
+        lp_select<N>(
             P.top, [&](int j) { return e[j].x; }, [&](int j) { return e[j].id; }, (int)P.vocab, sh);
     }
-    lp_write(P, row, {m, s, z * 0x1.62e42fefa39efp-1, at}, sc, sh.best);
+    lp_write(P, row, {m, s, z * 0x1.62e42fefa39efp-1, at}, sc, given, sh.best);
 }
 
 static RowCut lp_cut(size_t n, size_t vocab, size_t top) {
     // as many parts as fill the chip, and no more than one work group joins
-    size_t groups = 1024;
+    size_t groups = 2048;
     const size_t most = top ? LP_JOIN / top : LP_JOIN;
     if ((groups + n - 1) / n > most)
         groups = most * n;
@@ -407,12 +514,18 @@ int loomhip_token_logprobs_dev(const float *logits, size_t n, size_t vocab, size
     LogprobParams P = {logits, vocab, stride, tokens, temperature, (int)top, 1, logprobs, entropy, top_ids, top_logprobs,
                        nullptr, nullptr};
     if (vocab <= LP_ROW) {
+        const auto run = [&](auto nv) {
+            constexpr int NV = decltype(nv)::value;
+            hipLaunchKernelGGL((logprobs_row_kernel<NV>), dim3(n), dim3(SMP_THREADS), 0, st, P);
+        };
         if (vocab <= 4096)
-            hipLaunchKernelGGL((logprobs_row_kernel<256, 4>), dim3(n), dim3(256), 0, st, P);
+            run(std::integral_constant<int, 4>{});
+        else if (vocab <= 8192)
+            run(std::integral_constant<int, 8>{});
         else if (vocab <= 16384)
-            hipLaunchKernelGGL((logprobs_row_kernel<1024, 4>), dim3(n), dim3(1024), 0, st, P);
+            run(std::integral_constant<int, 16>{});
         else
-            hipLaunchKernelGGL((logprobs_row_kernel<1024, 8>), dim3(n), dim3(1024), 0, st, P);
+            run(std::integral_constant<int, 32>{});
         note_launch();
     } else {
         const RowCut cut = lp_cut(n, vocab, top);
@@ -428,7 +541,13 @@ int loomhip_token_logprobs_dev(const float *logits, size_t n, size_t vocab, size
             hipLaunchKernelGGL((logprobs_part_kernel<8>), g, dim3(SMP_THREADS), 0, st, P);
         else
             hipLaunchKernelGGL((logprobs_part_kernel<16>), g, dim3(SMP_THREADS), 0, st, P);
-        hipLaunchKernelGGL(logprobs_join_kernel, dim3(n), dim3(SMP_THREADS), 0, st, P);
+        const size_t entries = cut.splits * top;
+        if (entries <= SMP_THREADS)
+            hipLaunchKernelGGL(logprobs_join_kernel<1>, dim3(n), dim3(SMP_THREADS), 0, st, P);
+        else if (entries <= SMP_THREADS * 4)
+            hipLaunchKernelGGL(logprobs_join_kernel<4>, dim3(n), dim3(SMP_THREADS), 0, st, P);
+        else
+            hipLaunchKernelGGL(logprobs_join_kernel<LP_JOIN_N>, dim3(n), dim3(SMP_THREADS), 0, st, P);
         note_launch();
         note_launch();
     }
