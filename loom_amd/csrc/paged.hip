@@ -26,15 +26,15 @@ struct RopeParams {
     // queries, keys, values (of 0 heads where there are none); out NULL: into the pages
     const float *x[3];
     size_t xs[3];
-    float *out[3];
-    size_t os[3];
-    const float *norm[3];
+    float *out[2];
+    size_t os[2];
+    const float *norm[2];
     int heads[3];
     const int32_t *pos;
     const double *freqs;
     int rot, interleaved;
     float eps;
-    int hd, chunks; // chunks: groups of HB heads a token
+    int hd;
     size_t n;
     loomhip_pages c;
     const int32_t *lanes;
@@ -65,179 +65,154 @@ __device__ __forceinline__ bool rp_slot(const RopeParams &P, size_t t, int pos, 
     return true;
 }
 
-// GP lanes (a power of two, at least hd / 8 of them) take a head, each four
-// pairs, HB heads one after the other with all their loads in flight; cosines
-// and sines are formed once for the HB heads.  VEC: the four pairs are two
-// times four consecutive values (rot a multiple of 8).
-template <int GP, int HB, bool VEC>
+// A work group takes RP_THREADS / GP heads of a token: GP lanes (a power of two, at least hd / 8 of them) a head, each
+// four pairs.  The token's cosines and sines are formed once, by a thread a pair, while the heads are on their way.
+// VEC: the four pairs are two times four consecutive values (rot a multiple of 8).
+template <int GP, bool VEC>
 __global__ __launch_bounds__(RP_THREADS) void rope_kernel(RopeParams P) {
-    const int g = threadIdx.x % GP;
-    const size_t item = (size_t)blockIdx.x * (RP_THREADS / GP) + threadIdx.x / GP;
-    const size_t t = item / P.chunks;
-    if (t >= P.n)
-        return;
+    constexpr int PAIRS = GP * 4;
+    __shared__ __attribute__((aligned(16))) float cosines[PAIRS], sines[PAIRS];
+    const int tid = threadIdx.x, g = tid % GP;
+    const size_t t = blockIdx.x;
     const int pos = P.pos[t];
     if (pos < 0) // padding
         return;
-    const int h0 = (int)(item - t * P.chunks) * HB, all = P.heads[0] + P.heads[1] + P.heads[2];
+    // the group's head: its kind (0 query, 1 key, 2 value) and its number
+    const int at = blockIdx.y * (RP_THREADS / GP) + tid / GP;
+    const int kind = at < P.heads[0] ? 0 : at < P.heads[0] + P.heads[1] ? 1 : 2;
+    const int h = at - (kind > 0 ? P.heads[0] : 0) - (kind > 1 ? P.heads[1] : 0);
     const int p0 = g * 4, half = P.rot / 2;
-    const bool mine = g < P.hd / 8, turn = VEC ? p0 < half : p0 < half;
+    const bool mine = g < P.hd / 8 && h < (kind == 0 ? P.heads[0] : kind == 1 ? P.heads[1] : P.heads[2]);
+    const bool turn = kind < 2 && p0 < half;
     const bool split = VEC && turn && !P.interleaved; // values p0 .. and p0 + rot / 2 .., not 2 p0 ..
+    const bool pairs = VEC || kind == 2;              // in two times four consecutive values
     const int at_a = split ? p0 : 2 * p0, at_b = split ? p0 + half : 2 * p0 + 4;
 
-    // a head's kind (0 query, 1 key, 2 value) and its number
-    const auto head_of = [&](int h, int &kind) {
-        kind = h < P.heads[0] ? 0 : h < P.heads[0] + P.heads[1] ? 1 : 2;
-        return h - (kind > 0 ? P.heads[0] : 0) - (kind > 1 ? P.heads[1] : 0);
-    };
-    rp_f4 va[HB], vb[HB];
-#pragma unroll
-    for (int j = 0; j < HB; j++) {
-        va[j] = vb[j] = rp_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (mine && h0 + j < all) {
-            int kind;
-            const int h = head_of(h0 + j, kind);
-            const float *x = P.x[kind] + t * P.xs[kind] + (size_t)h * P.hd;
-            if (VEC || kind == 2) {
-                const bool s = split && kind != 2;
-                va[j] = *(const rp_f4u *)(x + (s ? at_a : 2 * p0));
-                vb[j] = *(const rp_f4u *)(x + (s ? at_b : 2 * p0 + 4));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    va[j][e] = x[rp_first(P, p0 + e)];
-                    vb[j][e] = x[rp_second(P, p0 + e)];
-                }
-            }
-        }
-    }
-    size_t row = 0;
-    const bool paged = h0 + HB > P.heads[0] && !P.out[1] && rp_slot(P, t, pos, row);
-    // (cos, sin) of the four pairs
-    float cs[4], sn[4];
-    if (h0 < P.heads[0] + P.heads[1] && mine && turn) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            cs[e] = 1.0f, sn[e] = 0.0f;
-            if (p0 + e < half) {
-                const double turns = (double)pos * (P.freqs[p0 + e] * 0x1.45f306dc9c883p-3);
-                const float x = (float)(2.0 * (turns - __builtin_rint(turns)));
-                sincospif(x, &sn[e], &cs[e]);
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < HB; j++) {
-        if (h0 + j >= all)
-            break;
-        int kind;
-        const int h = head_of(h0 + j, kind);
-        // (a, b) of the four pairs
-        rp_f4 a = va[j], b = vb[j];
-        if (VEC && !split) {
-            a = rp_f4{va[j][0], va[j][2], vb[j][0], vb[j][2]};
-            b = rp_f4{va[j][1], va[j][3], vb[j][1], vb[j][3]};
-        }
-        if (kind < 2) {
-            if (const float *w = P.norm[kind]) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    ss += a[e] * a[e] + b[e] * b[e];
-                ss += dpp_f<0xB1>(ss, ss);
-                ss += dpp_f<0x4E>(ss, ss);
-                ss += dpp_f<0x141>(ss, ss);
-                if (GP > 8)
-                    ss += dpp_f<0x140>(ss, ss);
-                if (GP > 16)
-                    ss += __shfl_xor(ss, 16);
-                const float r = 1.0f / sqrtf(ss / (float)P.hd + P.eps);
-                if (mine)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        a[e] = a[e] * r * w[rp_first(P, p0 + e)];
-                        b[e] = b[e] * r * w[rp_second(P, p0 + e)];
-                    }
-            }
-            if (turn && mine) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float u = a[e];
-                    a[e] = __builtin_fmaf(u, cs[e], -(b[e] * sn[e]));
-                    b[e] = __builtin_fmaf(b[e], cs[e], u * sn[e]);
-                }
-            }
-        }
-        if (!mine)
-            continue;
-        const bool to_pages = !P.out[kind];
-        if (to_pages && !paged)
-            continue;
-        const bool bf16 = P.c.type == LOOMHIP_BF16;
-        uint16_t *page = (uint16_t *)(kind == 1 ? P.c.k : P.c.v) + row + (size_t)h * P.c.head_stride;
-        float *out = P.out[kind] + t * P.os[kind] + (size_t)h * P.hd;
-        if (VEC || kind == 2) {
-            const bool s = split && kind != 2;
-            rp_f4 x = a, y = b;
-            if (VEC && !split) { // back beside each other
-                x = rp_f4{a[0], b[0], a[1], b[1]};
-                y = rp_f4{a[2], b[2], a[3], b[3]};
-            }
-            const int i = s ? at_a : 2 * p0, k = s ? at_b : 2 * p0 + 4;
-            if (to_pages) {
-                rp_u4 ux, uy;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    ux[e] = rp_half(x[e], bf16), uy[e] = rp_half(y[e], bf16);
-                *(rp_u4 *)(page + i) = ux;
-                *(rp_u4 *)(page + k) = uy;
-            } else {
-                *(rp_f4u *)(out + i) = x;
-                *(rp_f4u *)(out + k) = y;
-            }
+    rp_f4 va = {0.0f, 0.0f, 0.0f, 0.0f}, vb = va, wa = va, wb = va;
+    const float *norm = kind == 0 ? P.norm[0] : kind == 1 ? P.norm[1] : nullptr;
+    // f(x), for the group's values in memory: as they lie, or pair by pair
+    const auto fetch = [&](const float *x, rp_f4 &a, rp_f4 &b) {
+        if (pairs) {
+            a = *(const rp_f4u *)(x + at_a);
+            b = *(const rp_f4u *)(x + at_b);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int i = rp_first(P, p0 + e), k = rp_second(P, p0 + e);
-                if (to_pages)
-                    page[i] = rp_half(a[e], bf16), page[k] = rp_half(b[e], bf16);
-                else
-                    out[i] = a[e], out[k] = b[e];
+                a[e] = x[rp_first(P, p0 + e)];
+                b[e] = x[rp_second(P, p0 + e)];
             }
         }
-    }
-}
-
-template <int HB, bool VEC>
-static void rope_launch(const RopeParams &P0, hipStream_t st) {
-    RopeParams P = P0;
-    P.chunks = (P.heads[0] + P.heads[1] + P.heads[2] + HB - 1) / HB;
-    const size_t items = P.n * P.chunks;
-    const auto run = [&](auto gp) {
-        constexpr int GP = decltype(gp)::value, per = RP_THREADS / GP;
-        hipLaunchKernelGGL((rope_kernel<GP, HB, VEC>), dim3((items + per - 1) / per), dim3(RP_THREADS), 0, st, P);
     };
-    if (P.hd <= 64)
-        run(std::integral_constant<int, 8>{});
-    else if (P.hd <= 128)
-        run(std::integral_constant<int, 16>{});
-    else
-        run(std::integral_constant<int, 32>{});
-    note_launch();
+    // four consecutive pairs of neighbours as first and second ones, and back
+    const auto part = [&](rp_f4 &a, rp_f4 &b) {
+        if (pairs && !split) {
+            const rp_f4 x = a, y = b;
+            a = rp_f4{x[0], x[2], y[0], y[2]};
+            b = rp_f4{x[1], x[3], y[1], y[3]};
+        }
+    };
+    if (mine) {
+        const float *x = kind == 0 ? P.x[0] : kind == 1 ? P.x[1] : P.x[2];
+        fetch(x + t * (kind == 0 ? P.xs[0] : kind == 1 ? P.xs[1] : P.xs[2]) + (size_t)h * P.hd, va, vb);
+        if (norm)
+            fetch(norm, wa, wb);
+    }
+    const bool to_pages = kind && !P.out[1];
+    size_t row = 0;
+    const bool stored = !to_pages || rp_slot(P, t, pos, row);
+    if (tid < half && (int)(blockIdx.y * (RP_THREADS / GP)) < P.heads[0] + P.heads[1]) {
+        const double turns = (double)pos * (P.freqs[tid] * 0x1.45f306dc9c883p-3);
+        float s, c;
+        sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+        cosines[tid] = c, sines[tid] = s;
+    } else if (tid < PAIRS) {
+        cosines[tid] = 1.0f, sines[tid] = 0.0f;
+    }
+    __syncthreads();
+    rp_f4 a = va, b = vb;
+    part(a, b);
+    if (norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            ss += a[e] * a[e] + b[e] * b[e];
+        ss += dpp_f<0xB1>(ss, ss);
+        ss += dpp_f<0x4E>(ss, ss);
+        ss += dpp_f<0x141>(ss, ss);
+        if (GP > 8)
+            ss += dpp_f<0x140>(ss, ss);
+        if (GP > 16)
+            ss += __shfl_xor(ss, 16);
+        const float r = 1.0f / sqrtf(ss / (float)P.hd + P.eps);
+        part(wa, wb);
+        a = a * r * wa;
+        b = b * r * wb;
+    }
+    if (turn) {
+        const rp_f4 c = *(const rp_f4 *)(cosines + p0), s = *(const rp_f4 *)(sines + p0);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float u = a[e];
+            a[e] = __builtin_fmaf(u, c[e], -(b[e] * s[e]));
+            b[e] = __builtin_fmaf(b[e], c[e], u * s[e]);
+        }
+    }
+    if (!mine || !stored)
+        return;
+    if (pairs && !split) {
+        const rp_f4 x = a, y = b;
+        a = rp_f4{x[0], y[0], x[1], y[1]};
+        b = rp_f4{x[2], y[2], x[3], y[3]};
+    }
+    if (to_pages) {
+        uint16_t *out = (uint16_t *)(kind == 1 ? P.c.k : P.c.v) + row + (size_t)h * P.c.head_stride;
+        rp_u4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            x[e] = rp_half(a[e], P.c.type == LOOMHIP_BF16), y[e] = rp_half(b[e], P.c.type == LOOMHIP_BF16);
+        if (pairs) {
+            *(rp_u4 *)(out + at_a) = x;
+            *(rp_u4 *)(out + at_b) = y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                out[rp_first(P, p0 + e)] = x[e], out[rp_second(P, p0 + e)] = y[e];
+        }
+    } else {
+        float *out = (kind ? P.out[1] : P.out[0]) + t * (kind ? P.os[1] : P.os[0]) + (size_t)h * P.hd;
+        if (pairs) {
+            *(rp_f4u *)(out + at_a) = a;
+            *(rp_f4u *)(out + at_b) = b;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                out[rp_first(P, p0 + e)] = a[e], out[rp_second(P, p0 + e)] = b[e];
+        }
+    }
 }
 
 static int rope_run(const RopeParams &P, const char *what, void *stream) {
     if (int rc = require_device())
         return rc;
     hipStream_t st = stream_of(stream);
-    const size_t heads = (size_t)P.heads[0] + P.heads[1] + P.heads[2];
-    if (P.rot % 8) {
-        rope_launch<1, false>(P, st);
-    } else if (P.n * heads <= 8192) {
-        rope_launch<1, true>(P, st);
-    } else {
-        rope_launch<4, true>(P, st);
-    }
+    const auto run = [&](auto gp, auto vec) {
+        constexpr int GP = decltype(gp)::value, GROUPS = RP_THREADS / GP;
+        const dim3 g(P.n, (P.heads[0] + P.heads[1] + P.heads[2] + GROUPS - 1) / GROUPS);
+        hipLaunchKernelGGL((rope_kernel<GP, decltype(vec)::value>), g, dim3(RP_THREADS), 0, st, P);
+    };
+    const auto sized = [&](auto vec) {
+        if (P.hd <= 64)
+            run(std::integral_constant<int, 8>{}, vec);
+        else if (P.hd <= 128)
+            run(std::integral_constant<int, 16>{}, vec);
+        else
+            run(std::integral_constant<int, 32>{}, vec);
+    };
+    if (P.rot % 8 == 0)
+        sized(std::true_type{});
+    else
+        sized(std::false_type{});
+    note_launch();
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, what);
 }
@@ -289,10 +264,12 @@ static void rope_set(RopeParams &P, const loomhip_rope *r, size_t n, size_t hd) 
 static void heads_set(RopeParams &P, int kind, const loomhip_heads *s) {
     P.x[kind] = s->x;
     P.xs[kind] = s->x_stride;
-    P.out[kind] = s->out;
-    P.os[kind] = s->out_stride;
-    P.norm[kind] = s->norm;
     P.heads[kind] = (int)s->n_heads;
+    if (kind < 2) {
+        P.out[kind] = s->out;
+        P.os[kind] = s->out_stride;
+        P.norm[kind] = s->norm;
+    }
 }
 
 // What every call over pages asks of them (paged_attn.hip too).
