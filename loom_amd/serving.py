@@ -31,7 +31,7 @@ import torch
 from . import (BF16, F16, F32, HeadsDesc, KvRowsDesc, LoomHipError, LoraDesc, OK, PagesDesc, RopeDesc, last_error,
                lib)
 
-_F32, _I32, _U8 = torch.float32, torch.int32, torch.uint8
+_F32, _F64, _I32, _U8 = torch.float32, torch.float64, torch.int32, torch.uint8
 _LORA_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _HALF = (torch.float16, torch.int16)
 _PAGE_TYPES = {torch.float16: F16, torch.int16: F16, torch.bfloat16: BF16}
@@ -261,17 +261,14 @@ def verify_drafts_dev(target_probs, draft_tokens, u_accept, u_sample, draft_prob
     return tokens, accepted
 
 
-def _heads_ok(t, n: int, heads: int, hd: int) -> bool:
-    """f32 [n, heads, hd], a token's heads one after the other, the tokens apart."""
+def _heads(t, n: int, heads: int, hd: int):
+    """The elements from token to token of f32 [n, heads, hd], a token's heads one after the other; None if t is no such."""
     if t.shape != (n, heads, hd) or t.dtype is not _F32:
-        return False
-    s = t.stride()
-    return t.is_contiguous() or ((hd == 1 or s[2] == 1) and (heads == 1 or s[1] == hd) and (n == 1 or s[0] >= heads * hd))
-
-
-def _heads_desc(x, out, norm, heads: int):
-    return HeadsDesc(x.data_ptr(), x.stride(0), None if out is None else out.data_ptr(),
-                     0 if out is None else out.stride(0), None if norm is None else norm.data_ptr(), heads)
+        return None
+    s0, s1, s2 = t.stride()
+    if (s2 == 1 or hd == 1) and (s1 == hd or heads == 1) and (s0 >= heads * hd or n <= 1):
+        return s0
+    return s0 if t.is_contiguous() else None
 
 
 def _rope_desc(pos, freqs, n: int, eps: float, interleaved: bool):
@@ -279,13 +276,18 @@ def _rope_desc(pos, freqs, n: int, eps: float, interleaved: bool):
         raise ValueError("pos: int32, one a token")
     if freqs is None:
         return RopeDesc(pos.data_ptr(), None, 0, 0, eps)
-    if freqs.dim() != 1 or freqs.dtype is not torch.float64 or not freqs.is_contiguous():
+    shape = freqs.shape
+    if len(shape) != 1 or freqs.dtype is not _F64 or not freqs.is_contiguous():
         raise ValueError("freqs: f64 [rotated values / 2]")
-    return RopeDesc(pos.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0], interleaved, eps)
+    return RopeDesc(pos.data_ptr(), freqs.data_ptr(), 2 * shape[0], interleaved, eps)
 
 
-def _norm_ok(norm, hd: int) -> bool:
-    return norm is None or _is(norm, _F32, hd)
+def _norm_ptr(norm, hd: int):
+    if norm is None:
+        return None
+    if norm.shape != (hd,) or norm.dtype is not _F32 or not norm.is_contiguous():
+        raise ValueError(f"q_norm, k_norm: contiguous f32 [{hd}]")
+    return norm.data_ptr()
 
 
 def qk_norm_rope_dev(q, k, pos, freqs, q_norm=None, k_norm=None, eps: float = 1e-6, interleaved: bool = False,
@@ -303,44 +305,54 @@ def qk_norm_rope_dev(q, k, pos, freqs, q_norm=None, k_norm=None, eps: float = 1e
         raise ValueError("q [n, n_heads, head_dim], k [n, n_kv_heads, head_dim]")
     n, heads, hd = q.shape
     rope = _rope_desc(pos, freqs, n, eps, interleaved)
-    if not _norm_ok(q_norm, hd) or not _norm_ok(k_norm, hd):
-        raise ValueError(f"q_norm, k_norm: contiguous f32 [{hd}]")
-    if not _heads_ok(q, n, heads, hd) or not (q_out is None or _heads_ok(q_out, n, heads, hd)):
+    qn, kn = _norm_ptr(q_norm, hd), _norm_ptr(k_norm, hd)
+    qs, qos = _heads(q, n, heads, hd), heads * hd
+    if q_out is not None:
+        qos = _heads(q_out, n, heads, hd)
+    if qs is None or qos is None:
         raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
-    if k is None:
+    if k is not None:
+        kv = k.shape[1]
+        ks, kos = _heads(k, n, kv, hd), kv * hd
         if k_out is not None:
-            raise ValueError("k_out without k")
-    elif not _heads_ok(k, n, k.shape[1], hd) or not (k_out is None or _heads_ok(k_out, n, k.shape[1], hd)):
-        raise ValueError("k, k_out: f32 [n, n_kv_heads, head_dim] as q, a token's heads one after the other")
+            kos = _heads(k_out, n, kv, hd)
+        if ks is None or kos is None:
+            raise ValueError("k, k_out: f32 [n, n_kv_heads, head_dim] as q, a token's heads one after the other")
+    elif k_out is not None:
+        raise ValueError("k_out without k")
     dev, stream = _place(q, k, pos, freqs, q_norm, k_norm, q_out, k_out)
     if q_out is None:
         q_out = torch.empty((n, heads, hd), dtype=_F32, device=dev)
     kd = None
     if k is not None:
         if k_out is None:
-            k_out = torch.empty(k.shape, dtype=_F32, device=dev)
-        kd = C.byref(_heads_desc(k, k_out, k_norm, k.shape[1]))
-    rc = lib().loomhip_qk_norm_rope_dev(C.byref(_heads_desc(q, q_out, q_norm, heads)), kd, C.byref(rope), n, hd, stream)
+            k_out = torch.empty((n, kv, hd), dtype=_F32, device=dev)
+        kd = C.byref(HeadsDesc(k.data_ptr(), ks, k_out.data_ptr(), kos, kn, kv))
+    rc = lib().loomhip_qk_norm_rope_dev(C.byref(HeadsDesc(q.data_ptr(), qs, q_out.data_ptr(), qos, qn, heads)), kd,
+                                        C.byref(rope), n, hd, stream)
     if rc != OK:
         _fail("qk_norm_rope_dev", rc)
     return q_out, k_out
 
 
 def _pages_desc(k_pages, v_pages, table, kv: int, hd: int):
-    shape, stride = k_pages.shape, k_pages.stride()
-    kind = _PAGE_TYPES.get(k_pages.dtype)
-    if len(shape) != 4 or v_pages.shape != shape or kind is None or v_pages.dtype != k_pages.dtype:
+    shape, stride, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
+    kind = _PAGE_TYPES.get(dtype)
+    if len(shape) != 4 or v_pages.shape != shape or kind is None or v_pages.dtype is not dtype:
         raise ValueError("k_pages, v_pages: of one shape, [n_pages, page_size, n_kv_heads, head_dim], fp16 (or its bits as "
                          "int16) or bf16")
-    if shape[2] != kv or shape[3] != hd:
-        raise ValueError(f"pages of {shape[2]} heads of {shape[3]}, not {kv} of {hd}")
+    n_pages, page_size, heads, dim = shape
+    if heads != kv or dim != hd:
+        raise ValueError(f"pages of {heads} heads of {dim}, not {kv} of {hd}")
+    s0, s1, s2, s3 = stride
     if (v_pages.stride() != stride and any(a != b for a, b, s in zip(stride, v_pages.stride(), shape) if s > 1)) or (
-            stride[3] != 1 and hd != 1):
+            s3 != 1 and hd != 1):
         raise ValueError("k_pages, v_pages: of one layout, the values of a head one after the other")
-    if table.dim() != 2 or table.dtype is not _I32 or (table.shape[1] > 1 and table.stride(1) != 1):
+    tshape, tstride = table.shape, table.stride()
+    if len(tshape) != 2 or table.dtype is not _I32 or (tstride[1] != 1 and tshape[1] > 1):
         raise ValueError("table: int32 [lanes, pages], a lane's entries one after the other")
-    return PagesDesc(k_pages.data_ptr(), v_pages.data_ptr(), kind, shape[0], shape[1], stride[0], stride[1], stride[2],
-                     table.data_ptr(), table.shape[0], table.shape[1], table.stride(0))
+    return PagesDesc(k_pages.data_ptr(), v_pages.data_ptr(), kind, n_pages, page_size, s0, s1, s2, table.data_ptr(),
+                     tshape[0], tshape[1], tstride[0])
 
 
 def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None, k_norm=None, q=None, q_norm=None,
@@ -358,26 +370,32 @@ def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None,
         raise ValueError("k [n, n_kv_heads, head_dim]")
     n, kv, hd = k.shape
     rope = _rope_desc(pos, freqs, n, eps, interleaved)
-    if not _norm_ok(q_norm, hd) or not _norm_ok(k_norm, hd):
-        raise ValueError(f"q_norm, k_norm: contiguous f32 [{hd}]")
-    if not _heads_ok(k, n, kv, hd) or not _heads_ok(v, n, kv, hd):
+    qn, kn = _norm_ptr(q_norm, hd), _norm_ptr(k_norm, hd)
+    ks, vs = _heads(k, n, kv, hd), _heads(v, n, kv, hd)
+    if ks is None or vs is None:
         raise ValueError("k, v: f32 [n, n_kv_heads, head_dim], a token's heads one after the other")
-    if lanes is not None and not _is(lanes, _I32, n):
+    if lanes is not None and (lanes.shape != (n,) or lanes.dtype is not _I32 or not lanes.is_contiguous()):
         raise ValueError("lanes: int32, one a token")
     pages = _pages_desc(k_pages, v_pages, table, kv, hd)
-    if q is None:
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("q [n, n_heads, head_dim]")
+        heads = q.shape[1]
+        qs, qos = _heads(q, n, heads, hd), heads * hd
         if q_out is not None:
-            raise ValueError("q_out without q")
-    elif q.dim() != 3 or not _heads_ok(q, n, q.shape[1], hd) or not (q_out is None or _heads_ok(q_out, n, q.shape[1], hd)):
-        raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
+            qos = _heads(q_out, n, heads, hd)
+        if qs is None or qos is None:
+            raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
     dev, stream = _place(k, v, k_pages, v_pages, table, pos, lanes, freqs, k_norm, q, q_norm, q_out)
     qd = None
     if q is not None:
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=_F32, device=dev)
-        qd = C.byref(_heads_desc(q, q_out, q_norm, q.shape[1]))
-    rc = lib().loomhip_paged_append_dev(C.byref(pages), qd, C.byref(_heads_desc(k, None, k_norm, kv)), v.data_ptr(),
-                                        v.stride(0), None if lanes is None else lanes.data_ptr(), C.byref(rope), n, hd,
+            q_out = torch.empty((n, heads, hd), dtype=_F32, device=dev)
+        qd = C.byref(HeadsDesc(q.data_ptr(), qs, q_out.data_ptr(), qos, qn, heads))
+    rc = lib().loomhip_paged_append_dev(C.byref(pages), qd, C.byref(HeadsDesc(k.data_ptr(), ks, None, 0, kn, kv)),
+                                        v.data_ptr(), vs, None if lanes is None else lanes.data_ptr(), C.byref(rope), n, hd,
                                         stream)
     if rc != OK:
         _fail("paged_append_dev", rc)
