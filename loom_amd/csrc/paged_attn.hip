@@ -35,6 +35,7 @@ int pages_check(const loomhip_pages *c, size_t n_kv, size_t hd, const char *fn);
 constexpr int PG_THREADS = 256, PG_WAVES = PG_THREADS / 64;
 constexpr int PG_MAX_HD = 256;
 constexpr int PG_COLS = 16; // query heads of an item
+constexpr size_t PG_WHOLE = 512; // rows up to which no lane is cut; half as many at head sizes over 128
 
 // f16: two parts of a value, of a size that the second is normal; bf16: three, of f32's own range.
 struct PgF16 {
@@ -65,10 +66,9 @@ __device__ __forceinline__ void pg_split(float x, int e, typename T::v8 (&p)[T::
     }
 }
 
-// The items, (lane, key head, block) numbered in this order, that a run of rows begins in the middle of, and leaves in
-// the middle of after their first row; -1: none.
+// A record's item (lane, key head, block, numbered in this order; -1 but for an item's first record) and how many it has.
 struct PgDesc {
-    int32_t head, tail;
+    int32_t item, pieces;
 };
 
 struct PagedAttnParams {
@@ -79,9 +79,11 @@ struct PagedAttnParams {
     uint32_t window;                         // 0: none
     float scale;
     float *out;
-    PgDesc *desc; // [runs]
-    float *part;  // [runs][2][PG_COLS][hd]
-    float2 *ml;   // [runs][2][PG_COLS]
+    int room, cols;    // work groups that run at a time; query heads of a record
+    uint32_t *records; // how many were left
+    PgDesc *desc;      // [records]
+    float2 *ml;        // [records][cols]
+    float *part;       // [records][cols][hd]
 };
 
 // Rows [first, end) that lane i sees.
@@ -184,12 +186,14 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         unit = in ? (uint32_t)((size_t)page * (P.c.page_stride / 8) + (size_t)(r % ps) * row_units) : 0u;
         return __ballot(in);
     };
+    // The rows' chunks, their places from the lanes that have them.  Read once, past the caches: 604 MB take 117 us, with
+    // plain loads 130.
     const auto load = [&](uint32_t unit) {
 #pragma unroll
         for (int c = 0; c < C::NL; c++) {
             const size_t at = (size_t)(uint32_t)__shfl((int)unit, c * C::RPI + lane / C::CH) * 8;
-            rk[c] = *(const pg_u4 *)(kb + at);
-            rv[c] = *(const pg_u4 *)(vb + at);
+            rk[c] = __builtin_nontemporal_load((const pg_u4 *)(kb + at));
+            rv[c] = __builtin_nontemporal_load((const pg_u4 *)(vb + at));
         }
     };
 
@@ -355,174 +359,233 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_kernel(
     }
 }
 
-// The same with the rows of all items laid end to end, in units of a tile for
-// each wave, and cut into equal runs, one for each work group of the grid (as
-// many as the chip holds at a time): the lengths decide on the device who does
-// what.  An item that lies in one run is finished there.  Of one that runs on,
-// every work group leaves a record (m, l, o), at most two each: of the item
-// that came from before (slot 0) and of the one that goes on (slot 1).
+// A value's sum over the wave, in all of it.
+__device__ __forceinline__ uint32_t pg_wave_sum(uint32_t v) {
+    const auto add = [](uint32_t a, int b) { return a + (uint32_t)b; };
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));
+    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// The same with long items cut into pieces, a work group a piece.  How, every
+// wave works out by itself from the lengths: a lane of u units (a tile for each
+// wave) is cut into p = ceil(u / L) pieces of equal length, L the smallest of
+// some lengths from the chip's share (all units over the work groups that run
+// at a time) to twice that at which the pieces run in one round of the chip; half the
+// share where there are too many items for that (the work groups then take
+// pieces in turn).  Pieces are numbered lane by lane, [piece][item], so that
+// the blocks of query heads that read the same rows run side by side.  A piece
+// of a lane that is cut leaves a record (m, l, o).
 template <class T, int HDP>
 __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
     constexpr uint32_t UNIT = PG_WAVES * C::KT;
+    constexpr int CUTS = 6, SIXTEENTHS[CUTS] = {16, 17, 18, 20, 24, 32}; // of the share
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
-    __shared__ uint64_t scan[PG_WAVES];
-    __shared__ uint64_t before; // units before the run's first lane
-    __shared__ int found;       // that lane
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = blockIdx.x, W = gridDim.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t items = (uint32_t)P.n_kv * P.blocks; // of a lane
+    // every thread's lanes, a run of them
+    const int per = (P.n + 63) / 64, i0 = lane * per, i1 = i0 + per < P.n ? i0 + per : P.n;
     const auto units = [&](int i) {
         uint32_t first, end;
         pg_span(P, i, first, end);
         return (end - first + UNIT - 1) / UNIT;
     };
-    // lanes that see nothing
-    for (int i = w; i < P.n; i += W)
-        if (units(i) == 0)
-            for (int x = tid * 4; x < P.n_heads * P.hd; x += PG_THREADS * 4)
-                *(pg_f4 *)(P.out + (size_t)i * P.n_heads * P.hd + x) = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    // every thread's lanes, a run of them, and their units
-    const int per = (P.n + PG_THREADS - 1) / PG_THREADS;
-    uint64_t mine = 0;
-    for (int i = tid * per; i < (tid + 1) * per && i < P.n; i++)
-        mine += units(i);
-    uint64_t upto = mine;
-    for (int o = 1; o < 64; o *= 2) {
-        const uint64_t x = (uint64_t)__shfl_up((long long)upto, o);
-        upto += lane >= o ? x : 0;
-    }
-    if (lane == 63)
-        scan[wave] = upto;
-    __syncthreads();
-    uint64_t all = 0;
+    const uint32_t u0 = i0 < i1 ? units(i0) : 0; // most often the only one
+    const auto each = [&](auto f) {
+        if (i0 < i1)
+            f(u0, i0);
+        for (int i = i0 + 1; i < i1; i++)
+            f(units(i), i);
+    };
+    uint32_t total = 0;
+    each([&](uint32_t u, int) { total += u; });
+    total = pg_wave_sum(total);
+    const uint64_t share = ((uint64_t)total * items + P.room - 1) / P.room;
+    constexpr uint64_t MOST = 1 << 28; // longer than any lane
+    const auto pieces = [](uint32_t u, uint32_t L) { return u ? (u + L - 1) / L : 1; };
+    uint32_t cut[CUTS], count[CUTS];
 #pragma unroll
-    for (int x = 0; x < PG_WAVES; x++) {
-        upto += x < wave ? scan[x] : 0;
-        all += scan[x];
+    for (int x = 0; x < CUTS; x++) {
+        const uint64_t c = (share * SIXTEENTHS[x] + 15) / 16;
+        cut[x] = c < 1 ? 1 : c > MOST ? (uint32_t)MOST : (uint32_t)c;
+        count[x] = 0;
     }
-    const uint64_t total = all * items;
-    const int runs = total < (uint64_t)W ? (int)total : W;
-    if (w >= runs) {
-        if (tid == 0)
-            P.desc[w] = {-1, -1};
-        return;
+    each([&](uint32_t u, int) {
+#pragma unroll
+        for (int x = 0; x < CUTS; x++)
+            count[x] += pieces(u, cut[x]);
+    });
+    uint32_t L = (share + 1) / 2 > MOST ? (uint32_t)MOST : (uint32_t)((share + 1) / 2);
+    L = L < 1 ? 1 : L;
+#pragma unroll
+    for (int x = CUTS - 1; x >= 0; x--)
+        if ((uint64_t)pg_wave_sum(count[x]) * items <= (uint64_t)P.room)
+            L = cut[x];
+    // pieces and records of the lanes up to this thread's last
+    uint32_t np = 0, nr = 0;
+    each([&](uint32_t u, int) {
+        const uint32_t p = pieces(u, L);
+        np += p;
+        nr += p > 1 ? p : 0;
+    });
+    uint32_t to_p = np, to_r = nr;
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t x = __shfl_up(to_p, o), y = __shfl_up(to_r, o);
+        to_p += lane >= o ? x : 0;
+        to_r += lane >= o ? y : 0;
     }
-    const auto run_at = [&](int x) { return total / runs * x + total % runs * x / runs; };
-    const uint64_t from = run_at(w), to = run_at(w + 1);
-    if ((upto - mine) * items <= from && from < upto * items) {
-        uint64_t sum = upto - mine;
-        int i = tid * per;
-        for (uint32_t u = units(i); (sum + u) * items <= from; u = units(++i))
-            sum += u;
-        found = i, before = sum;
-    }
-    __syncthreads();
-    int i = found;
-    uint32_t u = units(i);
-    const uint64_t rest = from - before * items; // into the lane's units
-    uint32_t item = (uint32_t)(rest / u), j = (uint32_t)(rest - (uint64_t)item * u);
-    PgDesc desc = {-1, -1};
-    for (uint64_t at = from; at < to;) {
-        const uint32_t j1 = to - at < u - j ? j + (uint32_t)(to - at) : u; // units [j, j1) of the item's u
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to_p, 63) * items;
+    if (blockIdx.x == 0 && tid == 63)
+        *P.records = to_r * items;
+    for (uint32_t w = blockIdx.x; w < all; w += gridDim.x) {
+        // its lane, by the thread that has it: the lane's pieces, those before it and the records before them
+        const bool has = (to_p - np) * items <= w && w < to_p * items;
+        uint32_t sum = to_p - np, rec = to_r - nr, p = 1, first = 0, end = 0;
+        int i = i0;
+        if (has) {
+            for (;; i++) {
+                p = pieces(i == i0 ? u0 : units(i), L);
+                if (w < (sum + p) * items)
+                    break;
+                sum += p;
+                rec += p > 1 ? p : 0;
+            }
+            pg_span(P, i, first, end);
+        }
+        const int src = __builtin_ctzll(__ballot(has));
+        const auto from = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, src); };
+        i = (int)from((uint32_t)i), p = from(p), sum = from(sum), rec = from(rec), first = from(first), end = from(end);
+        const uint32_t piece = (w - sum * items) / items, item = w - sum * items - piece * items;
+        const uint32_t u = (end - first + UNIT - 1) / UNIT;
+        const uint32_t a = u / p * piece + (piece < u % p ? piece : u % p), b = a + u / p + (piece < u % p);
         const int kvh = item / P.blocks, block = item - kvh * P.blocks, h0 = kvh * P.group + block * PG_COLS;
         const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
-        uint32_t first, end;
-        pg_span(P, i, first, end);
-        const uint32_t r1 = end - first < j1 * UNIT ? end : first + j1 * UNIT;
-        pg_rows<T, HDP>(P, i, kvh, h0, heads, first + j * UNIT, r1, smem, sm, sl);
-        const bool whole = j == 0 && j1 == u;
-        const int slot = w * 2 + (j == 0);
-        if (!whole)
-            (j ? desc.head : desc.tail) = i * (int)items + (int)item;
+        pg_rows<T, HDP>(P, i, kvh, h0, heads, first + a * UNIT, b == u ? end : first + b * UNIT, smem, sm, sl);
+        rec = rec * items + item * p + piece;
         for (int x = tid; x < heads * (HDP / 4); x += PG_THREADS) {
             const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
-            float M, L;
-            const pg_f4 a = pg_join<HDP>(smem, sm, sl, h, d, M, L);
+            float M, S;
+            const pg_f4 v = pg_join<HDP>(smem, sm, sl, h, d, M, S);
             if (d < P.hd) {
-                if (whole)
-                    *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = pg_result(a, L);
+                if (p == 1)
+                    *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + h0 + h) * P.hd + d) = pg_result(v, S);
                 else
-                    *(pg_f4 *)(P.part + ((size_t)slot * PG_COLS + h) * P.hd + d) = a;
+                    *(pg_f4 *)(P.part + ((size_t)rec * P.cols + h) * P.hd + d) = v;
             }
-            if (!whole && d == 0)
-                P.ml[slot * PG_COLS + h] = make_float2(M, L);
+            if (p > 1 && d == 0)
+                P.ml[(size_t)rec * P.cols + h] = make_float2(M, S);
         }
+        if (p > 1 && tid == 0)
+            P.desc[rec] = {piece == 0 ? (int32_t)(i * (int)items + (int)item) : -1, (int32_t)p};
         __syncthreads(); // the join is read: its room is the next tiles'
-        at += j1 - j;
-        j = 0;
-        if (j1 == u && ++item == items) {
-            item = 0;
-            while (at < to && (u = units(++i)) == 0) {
-            }
-        }
     }
-    if (tid == 0)
-        P.desc[w] = desc;
 }
 
-// An item's records joined, a work group for a query head of the item that
-// goes on from run blockIdx.x: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
+// An item's records joined, a wave for a query head of the item whose first
+// record is blockIdx.x, all four for each of their heads where there are many:
+// M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
 template <int HDP>
-__global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnParams P, int runs) {
-    constexpr int LPR = HDP / 4, PAR = PG_THREADS / LPR; // threads of a record, records side by side
-    __shared__ pg_f4 so[PAR][LPR];
-    __shared__ float sl[PAR];
-    const int w = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-    const int seg = P.desc[w].tail;
-    if (seg < 0)
+__global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnParams P) {
+    constexpr int LPR = HDP / 4, PAR = 64 / LPR, MANY = 16 * PAR; // threads of a record, a wave's records side by side
+    __shared__ pg_f4 so[PG_WAVES][64];
+    __shared__ float sl[PG_WAVES][64];
+    const uint32_t rec = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (rec >= *P.records)
         return;
-    const int items = P.n_kv * P.blocks, i = seg / items, item = seg - i * items, kvh = item / P.blocks;
-    const int block = item - kvh * P.blocks;
-    if (h >= P.group - block * PG_COLS)
+    const PgDesc desc = P.desc[rec];
+    if (desc.item < 0)
         return;
-    int n = 1; // records: this run's second and the next runs' first ones
-    for (int x = w + 1; x < runs; x += 64) {
-        const int k = __popcll(__ballot(x + lane < runs && P.desc[x + lane].head == seg));
-        n += k;
-        if (k < 64)
-            break;
-    }
-    const auto slot = [&](int r) { return r == 0 ? w * 2 + 1 : (w + r) * 2; };
-    float M = -__builtin_inff();
-    for (int r = lane; r < n; r += 64)
-        M = fmaxf(M, P.ml[slot(r) * PG_COLS + h].x);
-    M = wave_max(M);
-    const int g = tid / LPR, d = tid % LPR * 4;
-    float l = 0.0f;
-    pg_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int items = P.n_kv * P.blocks, i = desc.item / items, item = desc.item - i * items, kvh = item / P.blocks;
+    const int block = item - kvh * P.blocks, n = desc.pieces, h0 = blockIdx.y * PG_WAVES;
+    const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
+    const int g = lane / LPR, d = lane % LPR * 4;
+    float M, l;
+    pg_f4 o;
+    const auto sum = [&](int h, int first, int step) { // of head h's records first, first + step, ..
+        const size_t at = (size_t)rec * P.cols + h;    // of a piece's next: P.cols further
+        M = -__builtin_inff();
+        for (int r = lane; r < n; r += 64)
+            M = fmaxf(M, P.ml[at + (size_t)r * P.cols].x);
+        M = wave_max(M);
+        l = 0.0f;
+        o = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int r = g; r < n; r += PAR) {
-        const int s = slot(r) * PG_COLS + h;
-        const float2 ml = P.ml[s];
-        const pg_f4 v = d < P.hd ? *(const pg_f4 *)(P.part + (size_t)s * P.hd + d) : pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        l += ml.y * f;
-        o += v * f;
-    }
-    so[g][tid % LPR] = o;
-    if (d == 0)
-        sl[g] = l;
-    __syncthreads();
-    if (g == 0 && d < P.hd) {
+        for (int r = first; r < n; r += step) {
+            const size_t s = at + (size_t)r * P.cols;
+            const float2 ml = P.ml[s];
+            const pg_f4 v = d < P.hd ? *(const pg_f4 *)(P.part + s * P.hd + d) : pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            l += ml.y * f;
+            o += v * f;
+        }
 #pragma unroll
-        for (int x = 1; x < PAR; x++)
-            o += so[x][tid], l += sl[x];
-        *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + kvh * P.group + block * PG_COLS + h) * P.hd + d) = pg_result(o, l);
+        for (int x = LPR; x < 64; x *= 2) {
+            l += __shfl_xor(l, x);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                o[e] += __shfl_xor(o[e], x);
+        }
+    };
+    const auto write = [&](int h) {
+        if (g == 0 && d < P.hd)
+            *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + kvh * P.group + block * PG_COLS + h) * P.hd + d) = pg_result(o, l);
+    };
+    if (n <= MANY) {
+        if (h0 + wave < heads) {
+            sum(h0 + wave, g, PAR);
+            write(h0 + wave);
+        }
+        return;
+    }
+    for (int h = h0; h < h0 + PG_WAVES && h < heads; h++) {
+        sum(h, wave * PAR + g, PG_WAVES * PAR);
+        so[wave][lane] = o;
+        sl[wave][lane] = l;
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int x = 1; x < PG_WAVES; x++)
+                o += so[x][lane], l += sl[x][lane];
+            write(h);
+        }
+        __syncthreads();
     }
 }
 
-// Work groups that run at a time.
-static int pg_runs(size_t hd) { return hd > 128 ? 256 : 512; }
-constexpr size_t PG_WHOLE = 256; // rows up to which a lane is not cut
-static size_t pg_ws_bytes(size_t max_rows, size_t hd) {
-    return max_rows <= PG_WHOLE ? 0 : (size_t)pg_runs(hd) * (sizeof(PgDesc) + 2 * PG_COLS * (hd * 4 + sizeof(float2)));
+// How a call runs.
+struct PgPlan {
+    int room;       // work groups that run at a time
+    size_t records; // at most; 0: no lane is cut, one launch
+};
+static PgPlan pg_plan(size_t max_rows, size_t items, size_t hd) {
+    PgPlan p;
+    p.room = hd > 128 ? 256 : 512;
+    // Pieces at twice the share: an item's rounding up and half of the chip's work groups.  Otherwise a piece of a cut lane
+    // has more than half of L, and L is at least half of the share.
+    p.records = items <= (size_t)p.room / 2 ? p.room : 4 * (size_t)p.room;
+    if (max_rows <= (hd > 128 ? PG_WHOLE / 2 : PG_WHOLE))
+        p.records = 0;
+    return p;
+}
+static size_t pg_ws_bytes(const PgPlan &p, size_t hd, size_t cols) {
+    return p.records ? 16 + p.records * (sizeof(PgDesc) + cols * (hd * 4 + sizeof(float2))) : 0;
+}
+static size_t pg_cols(size_t n_heads, size_t n_kv) { return n_heads / n_kv < PG_COLS ? n_heads / n_kv : PG_COLS; }
+static size_t pg_items(size_t n, size_t n_heads, size_t n_kv) {
+    return n * n_kv * ((n_heads / n_kv + PG_COLS - 1) / PG_COLS);
 }
 
 } // namespace lh
 
 using namespace lh;
 
+constexpr size_t PG_MAX_ROWS = (size_t)1 << 38; // positions of all lanes: their units are counted in 32 bits
 // The sizes the kernels index in 32 bits.
 static bool pg_served(size_t n, size_t n_heads, size_t n_kv, size_t hd) {
     return n && n <= 65535 && n_heads && n_kv && n_heads % n_kv == 0 && hd && hd % 8 == 0 && hd <= PG_MAX_HD &&
@@ -532,7 +595,9 @@ static bool pg_served(size_t n, size_t n_heads, size_t n_kv, size_t hd) {
 extern "C" {
 
 size_t loomhip_paged_attn_ws(size_t max_rows, size_t n, size_t n_heads, size_t n_kv_heads, size_t head_dim) {
-    return pg_served(n, n_heads, n_kv_heads, head_dim) ? pg_ws_bytes(max_rows, head_dim) : 0;
+    if (!pg_served(n, n_heads, n_kv_heads, head_dim))
+        return 0;
+    return pg_ws_bytes(pg_plan(max_rows, pg_items(n, n_heads, n_kv_heads), head_dim), head_dim, pg_cols(n_heads, n_kv_heads));
 }
 
 int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
@@ -547,13 +612,17 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
         return fail(LOOMHIP_DECLINED, "%s: %zu lanes of %zu heads of %zu not served", fn, n, n_heads, head_dim);
     if (int rc = pages_check(c, n_kv_heads, head_dim, fn))
         return rc;
+    if (n * (c->page_size * c->table_width) > PG_MAX_ROWS)
+        return fail(LOOMHIP_DECLINED, "%s: %zu lanes of %zu positions not served", fn, n, c->page_size * c->table_width);
     if (n > c->n_lanes)
         return fail(LOOMHIP_ERR_ARG, "%s: %zu lanes, a table of %zu", fn, n, c->n_lanes);
     if ((uintptr_t)len % 4)
         return fail(LOOMHIP_ERR_ARG, "%s: lengths not aligned to their elements", fn);
     if ((uintptr_t)q % 16 || (uintptr_t)out % 16)
         return fail(LOOMHIP_DECLINED, "%s: q or out not at a multiple of 16 bytes", fn);
-    const size_t need = pg_ws_bytes(c->page_size * c->table_width, head_dim);
+    const size_t max_rows = c->page_size * c->table_width, items = pg_items(n, n_heads, n_kv_heads);
+    const PgPlan plan = pg_plan(max_rows, items, head_dim);
+    const size_t need = pg_ws_bytes(plan, head_dim, pg_cols(n_heads, n_kv_heads));
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16))
         return fail(LOOMHIP_ERR_ARG, "%s: the workspace takes %zu bytes at a multiple of 16, got %zu", fn, need, ws_bytes);
     if (int rc = require_device())
@@ -572,23 +641,28 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
     P.scale = scale;
     P.out = out;
     hipStream_t st = stream_of(stream);
-    const int runs = pg_runs(head_dim);
+    P.room = plan.room;
+    P.cols = (int)pg_cols(n_heads, n_kv_heads);
     if (need) {
-        P.desc = (PgDesc *)ws;
-        P.ml = (float2 *)(P.desc + runs);
-        P.part = (float *)(P.ml + runs * 2 * PG_COLS);
+        P.records = (uint32_t *)ws;
+        P.part = (float *)((char *)ws + 16);
+        P.ml = (float2 *)(P.part + plan.records * P.cols * head_dim);
+        P.desc = (PgDesc *)(P.ml + plan.records * P.cols);
     }
     const auto run = [&](auto type, auto size) {
         using T = decltype(type);
         constexpr int HDP = decltype(size)::value;
         if (!need) {
-            hipLaunchKernelGGL((paged_attn_kernel<T, HDP>), dim3(n * n_kv_heads * P.blocks), dim3(PG_THREADS), 0, st, P);
+            hipLaunchKernelGGL((paged_attn_kernel<T, HDP>), dim3(items), dim3(PG_THREADS), 0, st, P);
             note_launch();
             return;
         }
-        hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP>), dim3(runs), dim3(PG_THREADS), 0, st, P);
-        hipLaunchKernelGGL((paged_attn_join_kernel<HDP>), dim3(runs, P.group < PG_COLS ? P.group : PG_COLS),
-                           dim3(PG_THREADS), 0, st, P, runs);
+        // as many work groups as run at a time, or as there can be pieces
+        const size_t unit = PG_WAVES * PgCfg<HDP>::KT, most = items * ((max_rows + unit - 1) / unit);
+        hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP>), dim3(most < (size_t)plan.room ? most : plan.room),
+                           dim3(PG_THREADS), 0, st, P);
+        hipLaunchKernelGGL((paged_attn_join_kernel<HDP>), dim3(plan.records, (P.cols + PG_WAVES - 1) / PG_WAVES),
+                           dim3(PG_THREADS), 0, st, P);
         note_launch();
         note_launch();
     };

@@ -331,6 +331,36 @@ def test_paged_attn_many_lanes(sv, n):
     assert (got[c["lens"] == 0] == 0).all()
 
 
+@pytest.mark.parametrize("shape", [
+    # heads, key heads, head size, lanes, longest: in more items than run at a time, in fewer, with one long lane
+    (8, 4, 32, 200, 1300, "f16"), (4, 4, 16, 130, 700, "bf16"), (3, 1, 128, 90, 1100, "f16"), (20, 1, 256, 70, 600, "bf16"),
+    (2, 2, 64, 65, 900, "f16"),
+], ids=lambda s: "x".join(map(str, s)))
+def test_paged_attn_many_lanes_are_cut(sv, shape):
+    H, KV, hd, n, longest, kind = shape
+    r = _rng(n, longest)
+    lens = [int(x) for x in r.integers(0, longest, n)]
+    lens[3:9] = [0] * 6
+    lens[n - 2] = 20 * longest
+    c = _attn_case(H, KV, hd, 16, lens, kind, "rows")
+    want, bound = _attn_ref(c)
+    got = _attn(sv, c).cpu().numpy()
+    _within(got, want, bound)
+    assert (got[c["lens"] == 0] == 0).all()
+    c["window"] = 300
+    _within(_attn(sv, c).cpu().numpy(), *_attn_ref(c), "window")
+
+
+def test_paged_attn_empty_batch_in_a_wide_table(sv):
+    c = _attn_case(8, 2, 64, 16, [40, 0, 3], "f16", "rows", width=400)
+    for lens in ([0, 0, 0], [0, 0, 1], [40, 0, 3]):
+        c["lens"] = np.array(lens, np.int32)
+        want, bound = _attn_ref(c)
+        got = _attn(sv, c).cpu().numpy()
+        _within(got, want, bound, lens)
+        assert (got[c["lens"] == 0] == 0).all()
+
+
 def test_paged_attn_lengths_past_the_table(sv):
     """A length is clamped into what the table can hold; a table wider than the lengths changes nothing."""
     import torch
@@ -545,7 +575,7 @@ def test_token_logprobs_temperatures(sv, V):
         _lp_check(sv, x, tokens, top, t, top)
 
 
-@pytest.mark.parametrize("V,threads", [(4000, 256), (32000, 1024), (151936, 256)])
+@pytest.mark.parametrize("V,threads", [(4000, 256), (32000, 256), (32000, 1024), (151936, 256)])
 def test_token_logprobs_where_few_threads_hold_the_largest(sv, V, threads):
     """Every value of half of the threads above all others: more reach the bound than are collected."""
     r = _rng(V, 3)

@@ -145,6 +145,10 @@ def _attn(pages=None, q=FAKE, lens=FAKE, n=2, heads=4, kv=2, hd=64, window=0, ou
     (DECLINED, dict(n=1 << 20)),
     (DECLINED, dict(q=FAKE + 4)),
     (DECLINED, dict(out=FAKE + 8)),
+    (ARG, dict(pages=_pages(page_size=256, page_stride=32768), ws=None)),
+    (ARG, dict(pages=_pages(page_size=256, page_stride=32768), ws=FAKE + 8)),
+    (ARG, dict(pages=_pages(page_size=256, page_stride=32768), ws_bytes=4096)),
+    (DECLINED, dict(pages=_pages(table_width=1 << 26, table_stride=1 << 26, n_lanes=1 << 9), n=1 << 9)),
 ])
 def test_paged_attn_refuses(rc, args):
     assert _attn(**args) == rc
@@ -185,6 +189,30 @@ def test_nothing_to_do_is_ok():
     L = loom_amd.lib()
     assert _rope(n=0) == OK and _append(n=0) == OK and _attn(n=0) == OK and _logprobs(n=0) == OK
     assert L.loomhip_token_logprobs_ws(0, 151936, 20) == 0 and L.loomhip_paged_attn_ws(4096, 0, 32, 4, 128) == 0
+
+
+def test_attn_workspace():
+    """None where no lane is cut; else room for the records of every cut that the lengths can lead to."""
+    ws = loom_amd.lib().loomhip_paged_attn_ws
+    assert ws(512, 64, 32, 4, 128) == 0 and ws(256, 64, 32, 4, 256) == 0
+    for rows, n, heads, kv, hd in ((513, 1, 32, 4, 128), (1 << 20, 64, 32, 4, 128), (1 << 20, 65535, 32, 32, 64), (300, 9, 40, 1, 256)):
+        items = n * kv * -(-(heads // kv) // 16)
+        room = 256 if hd > 128 else 512
+        records, cols = room * (1 if items <= room // 2 else 4), min(heads // kv, 16)
+        assert ws(rows, n, heads, kv, hd) == 16 + records * (8 + cols * (hd * 4 + 8))
+        # the plan's own bounds, over lengths drawn at random: lanes of u units in pieces of at most L
+        r = np.random.default_rng(rows)
+        for spread in (1, 30, 3000):
+            u = r.integers(0, spread + 1, min(n, 3000))
+            it = items // n
+            share = -(-int(u.sum()) * it // room)
+            pieces = lambda L: np.maximum(1, -(-u // L))
+            cuts = [max(1, -(-share * s // 16)) for s in (16, 17, 18, 20, 24, 32)]
+            L = next((c for c in cuts if pieces(c).sum() * it <= room), max(1, (share + 1) // 2))
+            p = pieces(L)
+            assert p[p > 1].sum() * it <= 4 * room
+            if len(u) * it <= room // 2:
+                assert p.sum() * it <= room
 
 
 def test_logprobs_workspace():
