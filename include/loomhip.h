@@ -912,7 +912,7 @@ typedef struct {
 } loomhip_rope;
 /* Queries and keys of n tokens, each head normed (x / sqrt(mean x^2 + eps) *
  * norm, where it has a norm), then rotated.  k may be NULL.  head_dim a
- * multiple of 8 up to 256, up to 4096 heads each and 2^24 tokens; DECLINED
+ * multiple of 8 up to 256, up to 4096 heads each and 2^23 tokens; DECLINED
  * otherwise. */
 int loomhip_qk_norm_rope_dev(const loomhip_heads *q, const loomhip_heads *k, const loomhip_rope *r, size_t n,
                              size_t head_dim, void *stream);
@@ -956,9 +956,9 @@ int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, con
  * sees nothing.  Rows that are not seen are not part of the result whatever they hold;
  * for the heads that see it, a value that is NaN or infinite makes its element
  * of the result NaN, a key with a NaN all of it, and a key with an infinity
- * too, unless its score is minus infinity.  The work is cut on the device by
- * len, not by the table's width.  n lanes of the table's n_lanes; head_dim a
- * multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^24, n times the
+ * too, unless its score is minus infinity: then it may also count as a row not
+ * seen.  The work is cut on the device by len, not by the table's width.  n lanes of the table's n_lanes; head_dim a
+ * multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^23, n times the
  * table's positions up to 2^38; DECLINED otherwise. */
 int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
                            size_t n_kv_heads, size_t head_dim, float scale, size_t window, float *out, void *ws,

@@ -290,7 +290,8 @@ __device__ __forceinline__ void lp_write(const LogprobParams &P, size_t row, con
     } else if (tid == 64) {
         P.lp[row] = lp;
     } else { // nothing above -inf: no token has a probability
-        P.entropy[row] = sc.greedy || r.s == 0.0 ? 0.0f : (float)(log_s - r.z / r.s);
+        const double h = log_s - r.z / r.s;
+        P.entropy[row] = sc.greedy || r.s == 0.0 || h < 0.0 ? 0.0f : (float)h; // below 0 by rounding alone
     }
 }
 

@@ -217,7 +217,7 @@ static int rope_run(const RopeParams &P, const char *what, void *stream) {
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, what);
 }
 
-constexpr size_t RP_MAX_TOKENS = 1 << 24, RP_MAX_HEADS = 4096;
+constexpr size_t RP_MAX_TOKENS = 1 << 23, RP_MAX_HEADS = 4096; // a launch has fewer than 2^32 threads a dimension
 
 // heads of the tokens and where they go (out NULL: into pages)
 static int heads_check(const loomhip_heads *s, size_t n, size_t hd, bool out, const char *fn, const char *what) {

@@ -277,13 +277,13 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
             for (int b = 0; b < DB; b++)
                 o[b] *= f;
         }
-        const float sub = T::SHIFT - (m == -__builtin_inff() ? 0.0f : m);
+        const float top = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             typename T::v8 pp[T::PARTS];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float w = __builtin_amdgcn_exp2f(s[b][e] + sub);
+                const float w = __builtin_amdgcn_exp2f(s[b][e] - top + T::SHIFT); // in this order: 14 is lost in a large m
                 l += w;
                 pg_split<T>(w, e, pp);
             }
@@ -589,7 +589,7 @@ constexpr size_t PG_MAX_ROWS = (size_t)1 << 38; // positions of all lanes: their
 // The sizes the kernels index in 32 bits.
 static bool pg_served(size_t n, size_t n_heads, size_t n_kv, size_t hd) {
     return n && n <= 65535 && n_heads && n_kv && n_heads % n_kv == 0 && hd && hd % 8 == 0 && hd <= PG_MAX_HD &&
-           n_heads <= 65535 && n * n_heads <= (size_t)1 << 24;
+           n_heads <= 65535 && n * n_heads <= (size_t)1 << 23;
 }
 
 extern "C" {

@@ -320,13 +320,13 @@ def qk_norm_rope_dev(q, k, pos, freqs, q_norm=None, k_norm=None, eps: float = 1e
             raise ValueError("k, k_out: f32 [n, n_kv_heads, head_dim] as q, a token's heads one after the other")
     elif k_out is not None:
         raise ValueError("k_out without k")
-    dev, stream = _place(q, k, pos, freqs, q_norm, k_norm, q_out, k_out)
+    stream = _place(q, k, pos, freqs, q_norm, k_norm, q_out, k_out)[1]
     if q_out is None:
-        q_out = torch.empty((n, heads, hd), dtype=_F32, device=dev)
+        q_out = q.new_empty((n, heads, hd))
     kd = None
     if k is not None:
         if k_out is None:
-            k_out = torch.empty((n, kv, hd), dtype=_F32, device=dev)
+            k_out = k.new_empty((n, kv, hd))
         kd = C.byref(HeadsDesc(k.data_ptr(), ks, k_out.data_ptr(), kos, kn, kv))
     rc = lib().loomhip_qk_norm_rope_dev(C.byref(HeadsDesc(q.data_ptr(), qs, q_out.data_ptr(), qos, qn, heads)), kd,
                                         C.byref(rope), n, hd, stream)
@@ -388,11 +388,11 @@ def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None,
             raise ValueError("q, q_out: f32 [n, n_heads, head_dim], a token's heads one after the other")
     elif q_out is not None:
         raise ValueError("q_out without q")
-    dev, stream = _place(k, v, k_pages, v_pages, table, pos, lanes, freqs, k_norm, q, q_norm, q_out)
+    stream = _place(k, v, k_pages, v_pages, table, pos, lanes, freqs, k_norm, q, q_norm, q_out)[1]
     qd = None
     if q is not None:
         if q_out is None:
-            q_out = torch.empty((n, heads, hd), dtype=_F32, device=dev)
+            q_out = q.new_empty((n, heads, hd))
         qd = C.byref(HeadsDesc(q.data_ptr(), qs, q_out.data_ptr(), qos, qn, heads))
     rc = lib().loomhip_paged_append_dev(C.byref(pages), qd, C.byref(HeadsDesc(k.data_ptr(), ks, None, 0, kn, kv)),
                                         v.data_ptr(), vs, None if lanes is None else lanes.data_ptr(), C.byref(rope), n, hd,
@@ -423,11 +423,11 @@ def paged_attn_dev(q, k_pages, v_pages, table, lens, scale: float, window: int =
         raise ValueError("window: 0 or more")
     if out is not None and not _is(out, _F32, *shape):
         raise ValueError("out: as q")
-    dev, stream = _place(q, k_pages, v_pages, table, lens, out)
+    stream = _place(q, k_pages, v_pages, table, lens, out)[1]
     if out is None:
         out = torch.empty_like(q)
     nb = _paged_attn_ws(pages.page_size * pages.table_width, n, heads, kv, hd)
-    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    ws = q.new_empty((nb + 3) // 4) if nb else None
     rc = lib().loomhip_paged_attn_dev(C.byref(pages), q.data_ptr(), lens.data_ptr(), n, heads, kv, hd, scale, window,
                                       out.data_ptr(), ws.data_ptr() if nb else None, nb, stream)
     if rc != OK:
@@ -454,11 +454,12 @@ def token_logprobs_dev(logits, tokens, top: int = 0, temperature=None):
         raise ValueError("temperature: f32, one a row")
     if top < 0:
         raise ValueError("top: 0 or more")
-    dev, stream = _place(logits, tokens, temperature)
-    lp, entropy = torch.empty(lead, dtype=_F32, device=dev), torch.empty(lead, dtype=_F32, device=dev)
-    ids, tops = torch.empty((*lead, top), dtype=_I32, device=dev), torch.empty((*lead, top), dtype=_F32, device=dev)
+    stream = _place(logits, tokens, temperature)[1]
+    lp = torch.empty_like(tokens, dtype=_F32)
+    entropy = torch.empty_like(lp)
+    ids, tops = tokens.new_empty((*lead, top)), logits.new_empty((*lead, top))
     nb = _logprobs_ws(n, vocab, top)
-    ws = torch.empty(nb, dtype=_U8, device=dev) if nb else None
+    ws = logits.new_empty((nb + 3) // 4) if nb else None
     rc = lib().loomhip_token_logprobs_dev(logits.data_ptr(), n, vocab, vocab, tokens.data_ptr(),
                                           None if temperature is None else temperature.data_ptr(), top, lp.data_ptr(),
                                           entropy.data_ptr(), ids.data_ptr(), tops.data_ptr(),

@@ -448,6 +448,25 @@ def test_paged_attn_queries_of_any_size(sv, size):
         _within(_attn(sv, c).cpu().numpy(), *_attn_ref(c), (size, kind))
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [3e6, 1e9, 1e30])
+def test_paged_attn_of_one_row_that_outweighs_all(sv, kind, size):
+    """Scores of millions and more: the row of the largest alone, its value exactly."""
+    c = _attn_case(4, 2, 64, 16, [700, 90], kind, "rows")
+    want = _np(_attn(sv, c)) * 0
+    r = _rng(5)
+    for i, n in enumerate((700, 90)):
+        for h in range(4):
+            k = _np(c["kp"])[c["table"][i][np.arange(n) // 16], np.arange(n) % 16, h // 2]
+            best = int(r.integers(0, n))
+            c["q"][i, h] = k[best] * size  # |k|^2 against k . k': the largest by some units, times size
+            s = k @ k[best]
+            assert s[best] - np.delete(s, best).max() > 0.5
+            want[i, h] = _np(c["vp"])[c["table"][i][best // 16], best % 16, h // 2]
+    c["scale"] = 1.0
+    assert (_np(_attn(sv, c)) == want).all()
+
+
 def test_paged_attn_growing_maxima(sv):
     """Scores that rise over hundreds of units along the cache: the running maximum moves in every tile."""
     c = _attn_case(4, 2, 64, 16, [2000, 900], "f16", "rows")
@@ -586,6 +605,19 @@ def test_token_logprobs_where_few_threads_hold_the_largest(sv, V, threads):
     tokens = np.zeros(2, np.int32)
     for top in (3, 32):
         _lp_check(sv, x, tokens, top, None, top)
+
+
+def test_token_logprobs_entropy_is_never_negative(sv):
+    x = np.full((4, 40000), -40.0, np.float32)
+    x[:, 5] = 30.0
+    x[1, 6] = 29.9999
+    x[2] = -100.0
+    x[2, 9] = 0.0
+    x[3] = -np.inf
+    x[3, 0] = 1.0
+    ent = _lp(sv, x, np.zeros(4, np.int32), 0, None)[1].cpu().numpy()
+    assert (ent >= 0).all()
+    _lp_check(sv, x, np.full(4, 5, np.int32), 3, None)
 
 
 def test_token_logprobs_shapes_and_strides(sv):

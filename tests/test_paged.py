@@ -38,7 +38,7 @@ def _rope(n=4, hd=64, q=None, k=None, pos=FAKE, freqs=FAKE, rot=64):
     (DECLINED, dict(hd=0, rot=0)),
     (DECLINED, dict(hd=60, rot=0)),
     (DECLINED, dict(hd=264)),
-    (DECLINED, dict(n=1 << 25)),
+    (DECLINED, dict(n=(1 << 23) + 1)),
     (ARG, dict(q=(None, 256, 0x200000, 256, None, 4))),
     (ARG, dict(q=(0x100000, 256, None, 256, None, 4))),
     (ARG, dict(q=(0x100000, 256, 0x200000, 256, None, 0))),
@@ -143,6 +143,7 @@ def _attn(pages=None, q=FAKE, lens=FAKE, n=2, heads=4, kv=2, hd=64, window=0, ou
     (DECLINED, dict(hd=60)),
     (DECLINED, dict(hd=264)),
     (DECLINED, dict(n=1 << 20)),
+    (DECLINED, dict(n=1 << 15, heads=(1 << 8) + 2, pages=_pages(n_lanes=1 << 15))),
     (DECLINED, dict(q=FAKE + 4)),
     (DECLINED, dict(out=FAKE + 8)),
     (ARG, dict(pages=_pages(page_size=256, page_stride=32768), ws=None)),
