@@ -124,7 +124,7 @@ struct PgCfg {
 
 // Query heads [h0, h0 + heads) of lane i, which read key head kvh, against its
 // rows [r0, r1): the four waves' (m, l, o), in LDS.
-template <class T, int HDP>
+template <class T, int HDP, bool ONCE>
 __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh, int h0, int heads, uint32_t r0,
                                         uint32_t r1, char *smem, float (*sm)[PG_COLS], float (*sl)[PG_COLS]) {
     using C = PgCfg<HDP>;
@@ -186,14 +186,26 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         unit = in ? (uint32_t)((size_t)page * (P.c.page_stride / 8) + (size_t)(r % ps) * row_units) : 0u;
         return __ballot(in);
     };
-    // The rows' chunks, their places from the lanes that have them.  Read once, past the caches: 604 MB take 117 us, with
-    // plain loads 130.
+    // The rows' chunks, their places from the lanes that have them.  Rows that one item alone reads (ONCE) pass the caches
+    // by: 604 MB take 114 us, with plain loads 126.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (50
+    // with the blocks on one XCD, pg_turn).
     const auto load = [&](uint32_t unit) {
+        uint32_t from[C::NL];
 #pragma unroll
-        for (int c = 0; c < C::NL; c++) {
-            const size_t at = (size_t)(uint32_t)__shfl((int)unit, c * C::RPI + lane / C::CH) * 8;
-            rk[c] = __builtin_nontemporal_load((const pg_u4 *)(kb + at));
-            rv[c] = __builtin_nontemporal_load((const pg_u4 *)(vb + at));
+        for (int c = 0; c < C::NL; c++)
+            from[c] = (uint32_t)__shfl((int)unit, c * C::RPI + lane / C::CH);
+        if constexpr (ONCE) {
+#pragma unroll
+            for (int c = 0; c < C::NL; c++) {
+                rk[c] = __builtin_nontemporal_load((const pg_u4 *)(kb + (size_t)from[c] * 8));
+                rv[c] = __builtin_nontemporal_load((const pg_u4 *)(vb + (size_t)from[c] * 8));
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C::NL; c++) {
+                rk[c] = *(const pg_u4 *)(kb + (size_t)from[c] * 8);
+                rv[c] = *(const pg_u4 *)(vb + (size_t)from[c] * 8);
+            }
         }
     };
 
@@ -335,21 +347,29 @@ __device__ __forceinline__ pg_f4 pg_result(pg_f4 a, float L) {
     return a + a * 0.0f;
 }
 
+// Which of `all` pieces work group x takes: those of the blocks of heads that read the same rows (side by side in the
+// pieces' order) on one of the eight XCDs, to which work groups go in turn.
+__device__ __forceinline__ uint32_t pg_turn(const PagedAttnParams &P, uint32_t x, uint32_t all) {
+    const uint32_t blocks = (uint32_t)P.blocks, span = 8 * blocks, g = x / span, r = x - g * span;
+    return blocks == 1 || (g + 1) * span > all ? x : g * span + r % 8 * blocks + r / 8;
+}
+
 template <int HDP>
 constexpr int pg_groups = HDP == 256 ? 1 : 2; // work groups of a CU (LDS and registers)
 
 // One item (lane, key head, block of its query heads) a work group: all of the lane's rows.
-template <class T, int HDP>
+template <class T, int HDP, bool ONCE>
 __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
-    const int block = blockIdx.x % P.blocks, ik = blockIdx.x / P.blocks, i = ik / P.n_kv, kvh = ik - i * P.n_kv;
+    const int w = (int)pg_turn(P, blockIdx.x, gridDim.x);
+    const int block = w % P.blocks, ik = w / P.blocks, i = ik / P.n_kv, kvh = ik - i * P.n_kv;
     const int h0 = kvh * P.group + block * PG_COLS;
     const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
     uint32_t r0, r1;
     pg_span(P, i, r0, r1);
-    pg_rows<T, HDP>(P, i, kvh, h0, heads, r0, r1, smem, sm, sl);
+    pg_rows<T, HDP, ONCE>(P, i, kvh, h0, heads, r0, r1, smem, sm, sl);
     for (int x = threadIdx.x; x < heads * (HDP / 4); x += PG_THREADS) {
         const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
         float M, L;
@@ -379,7 +399,7 @@ __device__ __forceinline__ uint32_t pg_wave_sum(uint32_t v) {
 // pieces in turn).  Pieces are numbered lane by lane, [piece][item], so that
 // the blocks of query heads that read the same rows run side by side.  A piece
 // of a lane that is cut leaves a record (m, l, o).
-template <class T, int HDP>
+template <class T, int HDP, bool ONCE>
 __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
     constexpr uint32_t UNIT = PG_WAVES * C::KT;
@@ -442,7 +462,8 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to_p, 63) * items;
     if (blockIdx.x == 0 && tid == 63)
         *P.records = to_r * items;
-    for (uint32_t w = blockIdx.x; w < all; w += gridDim.x) {
+    for (uint32_t x = blockIdx.x; x < all; x += gridDim.x) {
+        const uint32_t w = pg_turn(P, x, all);
         // its lane, by the thread that has it: the lane's pieces, those before it and the records before them
         const bool has = (to_p - np) * items <= w && w < to_p * items;
         uint32_t sum = to_p - np, rec = to_r - nr, p = 1, first = 0, end = 0;
@@ -465,7 +486,7 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         const uint32_t a = u / p * piece + (piece < u % p ? piece : u % p), b = a + u / p + (piece < u % p);
         const int kvh = item / P.blocks, block = item - kvh * P.blocks, h0 = kvh * P.group + block * PG_COLS;
         const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
-        pg_rows<T, HDP>(P, i, kvh, h0, heads, first + a * UNIT, b == u ? end : first + b * UNIT, smem, sm, sl);
+        pg_rows<T, HDP, ONCE>(P, i, kvh, h0, heads, first + a * UNIT, b == u ? end : first + b * UNIT, smem, sm, sl);
         rec = rec * items + item * p + piece;
         for (int x = tid; x < heads * (HDP / 4); x += PG_THREADS) {
             const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
@@ -649,35 +670,37 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
         P.ml = (float2 *)(P.part + plan.records * P.cols * head_dim);
         P.desc = (PgDesc *)(P.ml + plan.records * P.cols);
     }
-    const auto run = [&](auto type, auto size) {
+    const auto run = [&](auto type, auto size, auto once) {
         using T = decltype(type);
         constexpr int HDP = decltype(size)::value;
+        constexpr bool ONCE = decltype(once)::value;
         if (!need) {
-            hipLaunchKernelGGL((paged_attn_kernel<T, HDP>), dim3(items), dim3(PG_THREADS), 0, st, P);
+            hipLaunchKernelGGL((paged_attn_kernel<T, HDP, ONCE>), dim3(items), dim3(PG_THREADS), 0, st, P);
             note_launch();
             return;
         }
         // as many work groups as run at a time, or as there can be pieces
         const size_t unit = PG_WAVES * PgCfg<HDP>::KT, most = items * ((max_rows + unit - 1) / unit);
-        hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP>), dim3(most < (size_t)plan.room ? most : plan.room),
+        hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP, ONCE>), dim3(most < (size_t)plan.room ? most : plan.room),
                            dim3(PG_THREADS), 0, st, P);
         hipLaunchKernelGGL((paged_attn_join_kernel<HDP>), dim3(plan.records, (P.cols + PG_WAVES - 1) / PG_WAVES),
                            dim3(PG_THREADS), 0, st, P);
         note_launch();
         note_launch();
     };
-    const auto sized = [&](auto type) {
+    const auto sized = [&](auto type, auto once) {
         if (head_dim <= 64)
-            run(type, std::integral_constant<int, 64>{});
+            run(type, std::integral_constant<int, 64>{}, once);
         else if (head_dim <= 128)
-            run(type, std::integral_constant<int, 128>{});
+            run(type, std::integral_constant<int, 128>{}, once);
         else
-            run(type, std::integral_constant<int, 256>{});
+            run(type, std::integral_constant<int, 256>{}, once);
     };
-    if (c->type == LH_F16)
-        sized(PgF16{});
+    const auto typed = [&](auto once) { c->type == LH_F16 ? sized(PgF16{}, once) : sized(PgBf16{}, once); };
+    if (P.blocks == 1)
+        typed(std::true_type{});
     else
-        sized(PgBf16{});
+        typed(std::false_type{});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? LOOMHIP_OK : hip_fail(e, "paged_attn launch");
 }
