@@ -77,15 +77,22 @@ struct PagedAttnParams {
     const int32_t *len;
     int n, n_heads, n_kv, hd, group, blocks; // group: query heads of a key head, in `blocks` blocks of PG_COLS
     uint32_t window;                         // 0: none
+    uint32_t page_mul, page_shift;           // pg_page
+    uint32_t page_units, row_units;          // from page to page and row to row, in 16 bytes
     float scale;
     float *out;
-    int room, cols;    // work groups that run at a time; query heads of a record
+    int cols;          // query heads of a record
     uint32_t *records; // how many were left
     PgDesc *desc;      // [records]
     float2 *ml;        // [records][cols]
     float *part;       // [records][cols][hd]
 };
 
+// r / page_size for r < 2^31: with 2^(l - 1) < page_size <= 2^l and m = floor(2^(31 + l) / page_size) + 1, which has 32
+// bits, m page_size is past 2^(31 + l) by at most 2^l, so r m / 2^(31 + l) is past r / page_size by less than 1 / page_size.
+__device__ __forceinline__ uint32_t pg_page(const PagedAttnParams &P, uint32_t r) {
+    return P.page_mul ? __umulhi(r, P.page_mul) >> P.page_shift : r;
+}
 // Rows [first, end) that lane i sees.
 __device__ __forceinline__ void pg_span(const PagedAttnParams &P, int i, uint32_t &first, uint32_t &end) {
     const uint32_t most = (uint32_t)(P.c.page_size * P.c.table_width);
@@ -133,25 +140,41 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
     const int hd = P.hd;
     char *tile = smem + wave * C::WAVE;
 
+    // the page of the lane's row (lane % KT) of the tile that starts at row `at`; the first two tiles' are on their way
+    // while the query is split
+    const int32_t *table = P.c.table + (size_t)i * P.c.table_stride;
+    const auto page_of = [&](uint32_t at) {
+        const uint32_t r = at + lane % C::KT;
+        return r < r1 ? table[pg_page(P, r)] : -1;
+    };
+    uint32_t at = r0 + wave * C::KT, unit;
+    const int32_t page = page_of(at);
+    int32_t next = page_of(at + PG_WAVES * C::KT);
+
     // the query's parts: 8 (lane / 16) + j of every 32 values
-    typename T::v8 qp[STEPS][T::PARTS];
-    float cs = P.scale * 0x1.715476p+0f; // scores in log2 units
+    pg_f4 qv[STEPS][2];
     {
         const float *q = P.q + ((size_t)i * P.n_heads + h0 + (col < heads ? col : 0)) * hd;
-        float v[STEPS][8], amax = 0.0f;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             const int d = s * 32 + quad * 8;
-            const bool in = col < heads && d < hd;
-            const pg_f4 a = *(const pg_f4 *)(q + (d < hd ? d : 0)), b = *(const pg_f4 *)(q + (d < hd ? d : 0) + 4);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                v[s][e] = in ? a[e] : 0.0f;
-                v[s][e + 4] = in ? b[e] : 0.0f;
-                amax = fmaxf(amax, fmaxf(fabsf(v[s][e]), fabsf(v[s][e + 4])));
-            }
+            qv[s][0] = *(const pg_f4 *)(q + (d < hd ? d : 0));
+            qv[s][1] = *(const pg_f4 *)(q + (d < hd ? d : 0) + 4);
         }
-        float f = 1.0f;
+    }
+
+    typename T::v8 qp[STEPS][T::PARTS];
+    float cs = P.scale * 0x1.715476p+0f; // scores in log2 units
+    {
+        float amax = 0.0f, f = 1.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const bool in = col < heads && s * 32 + quad * 8 < hd;
+                qv[s][e / 4][e % 4] = in ? qv[s][e / 4][e % 4] : 0.0f;
+                amax = fmaxf(amax, fabsf(qv[s][e / 4][e % 4]));
+            }
         if (T::PARTS == 2) { // the largest element brought to 2^13 .. 2^14
             amax = pg_max4(amax);
             const int e = (int)(__float_as_uint(amax) >> 23);
@@ -163,27 +186,20 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         for (int s = 0; s < STEPS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                pg_split<T>(v[s][e] * f, e, qp[s]);
+                pg_split<T>(qv[s][e / 4][e % 4] * f, e, qp[s]);
     }
 
     // staging: the lane's chunk of a row, the first of its rows
     const int chunk = (lane % C::CH) * 8 < hd ? lane % C::CH : hd / 8 - 1; // past the head's end: the last one again
     const uint16_t *kb = (const uint16_t *)P.c.k + (size_t)kvh * P.c.head_stride + chunk * 8;
     const uint16_t *vb = (const uint16_t *)P.c.v + (size_t)kvh * P.c.head_stride + chunk * 8;
-    const int32_t *table = P.c.table + (size_t)i * P.c.table_stride;
-    const uint32_t ps = (uint32_t)P.c.page_size;
-    const uint32_t row_units = (uint32_t)(P.c.row_stride / 8);
     pg_u4 rk[C::NL], rv[C::NL];
-    // The tile that starts at row `at`: where the lane's row (lane % KT) begins, in 16-byte units, and which rows are
-    // there.  A row that is not (past the end, on no page) is loaded as the pool's first.
-    const auto page_of = [&](uint32_t at) {
-        const uint32_t r = at + lane % C::KT;
-        return r < r1 ? table[r / ps] : -1;
-    };
+    // The tile that starts at row `at`: where the lane's row begins, in 16-byte units, and which rows are there.  A row
+    // that is not (past the end, on no page) is loaded as the pool's first.
     const auto place = [&](uint32_t at, int32_t page, uint32_t &unit) {
         const uint32_t r = at + lane % C::KT;
         const bool in = r < r1 && page >= 0 && (uint32_t)page < (uint32_t)P.c.n_pages;
-        unit = in ? (uint32_t)((size_t)page * (P.c.page_stride / 8) + (size_t)(r % ps) * row_units) : 0u;
+        unit = in ? (uint32_t)page * P.page_units + (r - pg_page(P, r) * (uint32_t)P.c.page_size) * P.row_units : 0u;
         return __ballot(in);
     };
     // The rows' chunks, their places from the lanes that have them.  Rows that one item alone reads (ONCE) pass the caches
@@ -209,12 +225,12 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         }
     };
 
+    constexpr uint64_t ALL = C::KT == 64 ? ~0ull : (1ull << 32) - 1;
     pg_f4 o[DB];
 #pragma unroll
     for (int b = 0; b < DB; b++)
         o[b] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -__builtin_inff(), l = 0.0f;
-    constexpr uint64_t ALL = C::KT == 64 ? ~0ull : (1ull << 32) - 1;
 
     const int st = (lane / C::CH) * C::KS + (lane % C::CH) * 16, vt = C::VO + (lane / C::CH) * C::VS + (lane % C::CH) * 16;
     const int k_at = col * C::KS + quad * 16, v_at = C::VO + (4 * quad + (col >> 2)) * C::VS + 8 * (col & 3);
@@ -225,14 +241,9 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         return __builtin_bit_cast(typename T::v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
-    uint32_t at = r0 + wave * C::KT, unit;
-    uint64_t live = 0;
-    int32_t next = -1;
-    if (at < r1) {
-        live = place(at, page_of(at), unit) & ALL;
-        next = page_of(at + PG_WAVES * C::KT);
+    uint64_t live = place(at, page, unit) & ALL;
+    if (at < r1)
         load(unit);
-    }
     for (; at < r1; at += PG_WAVES * C::KT) {
         const uint64_t here = live;
         live = place(at + PG_WAVES * C::KT, next, unit) & ALL;
@@ -355,7 +366,8 @@ __device__ __forceinline__ uint32_t pg_turn(const PagedAttnParams &P, uint32_t x
 }
 
 template <int HDP>
-constexpr int pg_groups = HDP == 256 ? 1 : 2; // work groups of a CU (LDS and registers)
+constexpr int pg_groups = HDP == 256 ? 1 : 2;                        // work groups of a CU (LDS and registers)
+constexpr int pg_room(size_t hd) { return hd > 128 ? 256 : 512; } // work groups that run at a time
 
 // One item (lane, key head, block of its query heads) a work group: all of the lane's rows.
 template <class T, int HDP, bool ONCE>
@@ -402,10 +414,11 @@ __device__ __forceinline__ uint32_t pg_wave_sum(uint32_t v) {
 template <class T, int HDP, bool ONCE>
 __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
-    constexpr uint32_t UNIT = PG_WAVES * C::KT;
+    constexpr uint32_t UNIT = PG_WAVES * C::KT, ROOM = pg_room(HDP);
     constexpr int CUTS = 6, SIXTEENTHS[CUTS] = {16, 17, 18, 20, 24, 32}; // of the share
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
+    __shared__ uint32_t before[2][65], firsts[64]; // pieces and records before a thread's lanes, its first lane's units
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t items = (uint32_t)P.n_kv * P.blocks; // of a lane
     // every thread's lanes, a run of them
@@ -425,9 +438,13 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     uint32_t total = 0;
     each([&](uint32_t u, int) { total += u; });
     total = pg_wave_sum(total);
-    const uint64_t share = ((uint64_t)total * items + P.room - 1) / P.room;
+    const uint64_t share = ((uint64_t)total * items + ROOM - 1) / ROOM;
     constexpr uint64_t MOST = 1 << 28; // longer than any lane
-    const auto pieces = [](uint32_t u, uint32_t L) { return u ? (u + L - 1) / L : 1; };
+    // ceil(u / L), at least 1; within a rounding of whole numbers it may be one off, which unsettles nothing: whoever counts
+    // pieces counts them so
+    const auto pieces = [](uint32_t u, uint32_t L) {
+        return u ? (uint32_t)((float)u * __builtin_amdgcn_rcpf((float)L) * 0x1.fffffp-1f) + 1 : 1;
+    };
     uint32_t cut[CUTS], count[CUTS];
 #pragma unroll
     for (int x = 0; x < CUTS; x++) {
@@ -444,7 +461,7 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     L = L < 1 ? 1 : L;
 #pragma unroll
     for (int x = CUTS - 1; x >= 0; x--)
-        if ((uint64_t)pg_wave_sum(count[x]) * items <= (uint64_t)P.room)
+        if ((uint64_t)pg_wave_sum(count[x]) * items <= (uint64_t)ROOM)
             L = cut[x];
     // pieces and records of the lanes up to this thread's last
     uint32_t np = 0, nr = 0;
@@ -462,15 +479,22 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to_p, 63) * items;
     if (blockIdx.x == 0 && tid == 63)
         *P.records = to_r * items;
+    if (tid < 64) { // out of the registers
+        before[0][lane] = to_p - np, before[1][lane] = to_r - nr;
+        if (lane == 63)
+            before[0][64] = to_p;
+        firsts[lane] = u0;
+    }
+    __syncthreads();
     for (uint32_t x = blockIdx.x; x < all; x += gridDim.x) {
         const uint32_t w = pg_turn(P, x, all);
         // its lane, by the thread that has it: the lane's pieces, those before it and the records before them
-        const bool has = (to_p - np) * items <= w && w < to_p * items;
-        uint32_t sum = to_p - np, rec = to_r - nr, p = 1, first = 0, end = 0;
-        int i = i0;
+        uint32_t sum = before[0][lane], rec = before[1][lane], p = 1, first = 0, end = 0;
+        const bool has = sum * items <= w && w < before[0][lane + 1] * items;
+        int i = lane * per;
         if (has) {
-            for (;; i++) {
-                p = pieces(i == i0 ? u0 : units(i), L);
+            for (uint32_t u = firsts[lane];; u = units(++i)) {
+                p = pieces(u, L);
                 if (w < (sum + p) * items)
                     break;
                 sum += p;
@@ -481,10 +505,11 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         const int src = __builtin_ctzll(__ballot(has));
         const auto from = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, src); };
         i = (int)from((uint32_t)i), p = from(p), sum = from(sum), rec = from(rec), first = from(first), end = from(end);
-        const uint32_t piece = (w - sum * items) / items, item = w - sum * items - piece * items;
+        const uint32_t piece = w / items - sum, item = w - w / items * items; // sum * items are before it
         const uint32_t u = (end - first + UNIT - 1) / UNIT;
         const uint32_t a = u / p * piece + (piece < u % p ? piece : u % p), b = a + u / p + (piece < u % p);
-        const int kvh = item / P.blocks, block = item - kvh * P.blocks, h0 = kvh * P.group + block * PG_COLS;
+        const int kvh = ONCE ? item : item / P.blocks, block = ONCE ? 0 : item - kvh * P.blocks;
+        const int h0 = kvh * P.group + block * PG_COLS;
         const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
         pg_rows<T, HDP, ONCE>(P, i, kvh, h0, heads, first + a * UNIT, b == u ? end : first + b * UNIT, smem, sm, sl);
         rec = rec * items + item * p + piece;
@@ -517,10 +542,9 @@ __global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnPa
     __shared__ float sl[PG_WAVES][64];
     const uint32_t rec = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (rec >= *P.records)
-        return;
-    const PgDesc desc = P.desc[rec];
-    if (desc.item < 0)
+    const uint32_t records = *P.records;
+    const PgDesc desc = P.desc[rec]; // undefined past the records
+    if (rec >= records || desc.item < 0)
         return;
     const int items = P.n_kv * P.blocks, i = desc.item / items, item = desc.item - i * items, kvh = item / P.blocks;
     const int block = item - kvh * P.blocks, n = desc.pieces, h0 = blockIdx.y * PG_WAVES;
@@ -581,12 +605,12 @@ __global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnPa
 
 // How a call runs.
 struct PgPlan {
-    int room;       // work groups that run at a time
+    int room;
     size_t records; // at most; 0: no lane is cut, one launch
 };
 static PgPlan pg_plan(size_t max_rows, size_t items, size_t hd) {
     PgPlan p;
-    p.room = hd > 128 ? 256 : 512;
+    p.room = pg_room(hd);
     // Pieces at twice the share: an item's rounding up and half of the chip's work groups.  Otherwise a piece of a cut lane
     // has more than half of L, and L is at least half of the share.
     p.records = items <= (size_t)p.room / 2 ? p.room : 4 * (size_t)p.room;
@@ -658,11 +682,15 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
     P.hd = (int)head_dim;
     P.group = (int)(n_heads / n_kv_heads);
     P.blocks = (P.group + PG_COLS - 1) / PG_COLS;
+    const int bits = c->page_size > 1 ? 64 - __builtin_clzll(c->page_size - 1) : 0; // 2^bits >= page_size
+    P.page_mul = bits ? (uint32_t)(((uint64_t)1 << (31 + bits)) / c->page_size + 1) : 0;
+    P.page_shift = bits ? bits - 1 : 0;
+    P.page_units = (uint32_t)(c->page_stride / 8);
+    P.row_units = (uint32_t)(c->row_stride / 8);
     P.window = window > 0x7fffffff ? 0 : (uint32_t)window; // longer than any lane: none
     P.scale = scale;
     P.out = out;
     hipStream_t st = stream_of(stream);
-    P.room = plan.room;
     P.cols = (int)pg_cols(n_heads, n_kv_heads);
     if (need) {
         P.records = (uint32_t *)ws;
