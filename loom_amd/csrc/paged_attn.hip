@@ -18,6 +18,17 @@
 // contracted indices mean those rows; the A operand's lane then needs the same
 // rows of one value column, which two LDS transpose reads (ds_read_b64_tr_b16)
 // give from row-major values.
+//
+// Bound by the bytes of the rows: a wave's tile is loaded into registers (a
+// page's rows wherever they lie, 16 bytes a thread), put into LDS when the wave
+// is through with the one before, and the next tile's loads go out; two work
+// groups a CU keep up to 128 KB in flight, and the products (512 cycles of a
+// tile's 11000) hide behind them.  Measured, 32 heads of 128 over 4 key heads:
+// 8 lanes of up to 65536 rows, bf16, 106 us (604 MB, 5.7 TB/s, where a plain read
+// of that many bytes runs at 7.0: work groups start and end together, and
+// pieces are up to a twentieth longer than the share), 32 lanes of up to 4096,
+// f16, 30 us (139 MB; about 6 of them the look-up of lengths, pages and first
+// tiles, and the joins) and 4.6 for the records; one lane of 256 rows 6.9.
 #include "runtime.hpp"
 
 #include <type_traits>
@@ -203,7 +214,7 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         return __ballot(in);
     };
     // The rows' chunks, their places from the lanes that have them.  Rows that one item alone reads (ONCE) pass the caches
-    // by: 604 MB take 114 us, with plain loads 126.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (50
+    // by: 604 MB take 114 us, with plain loads 126.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (48
     // with the blocks on one XCD, pg_turn).
     const auto load = [&](uint32_t unit) {
         uint32_t from[C::NL];
@@ -532,12 +543,11 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     }
 }
 
-// An item's records joined, a wave for a query head of the item whose first
-// record is blockIdx.x, all four for each of their heads where there are many:
-// M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
-template <int HDP>
+// The records of the item whose first one is blockIdx.x joined, WPH waves for
+// a query head: M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
+template <int HDP, int WPH>
 __global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnParams P) {
-    constexpr int LPR = HDP / 4, PAR = 64 / LPR, MANY = 16 * PAR; // threads of a record, a wave's records side by side
+    constexpr int LPR = HDP / 4, PAR = 64 / LPR; // threads of a record, a wave's records side by side
     __shared__ pg_f4 so[PG_WAVES][64];
     __shared__ float sl[PG_WAVES][64];
     const uint32_t rec = blockIdx.x;
@@ -547,21 +557,18 @@ __global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnPa
     if (rec >= records || desc.item < 0)
         return;
     const int items = P.n_kv * P.blocks, i = desc.item / items, item = desc.item - i * items, kvh = item / P.blocks;
-    const int block = item - kvh * P.blocks, n = desc.pieces, h0 = blockIdx.y * PG_WAVES;
+    const int block = item - kvh * P.blocks, n = desc.pieces, h = blockIdx.y * (PG_WAVES / WPH) + wave / WPH;
     const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
     const int g = lane / LPR, d = lane % LPR * 4;
-    float M, l;
-    pg_f4 o;
-    const auto sum = [&](int h, int first, int step) { // of head h's records first, first + step, ..
-        const size_t at = (size_t)rec * P.cols + h;    // of a piece's next: P.cols further
-        M = -__builtin_inff();
+    float M = -__builtin_inff(), l = 0.0f;
+    pg_f4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (h < heads) {
+        const size_t at = (size_t)rec * P.cols + h; // of a piece's next: P.cols further
         for (int r = lane; r < n; r += 64)
             M = fmaxf(M, P.ml[at + (size_t)r * P.cols].x);
         M = wave_max(M);
-        l = 0.0f;
-        o = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int r = first; r < n; r += step) {
+#pragma unroll 8
+        for (int r = wave % WPH * PAR + g; r < n; r += WPH * PAR) {
             const size_t s = at + (size_t)r * P.cols;
             const float2 ml = P.ml[s];
             const pg_f4 v = d < P.hd ? *(const pg_f4 *)(P.part + s * P.hd + d) : pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -576,31 +583,19 @@ __global__ __launch_bounds__(PG_THREADS) void paged_attn_join_kernel(PagedAttnPa
             for (int e = 0; e < 4; e++)
                 o[e] += __shfl_xor(o[e], x);
         }
-    };
-    const auto write = [&](int h) {
-        if (g == 0 && d < P.hd)
-            *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + kvh * P.group + block * PG_COLS + h) * P.hd + d) = pg_result(o, l);
-    };
-    if (n <= MANY) {
-        if (h0 + wave < heads) {
-            sum(h0 + wave, g, PAR);
-            write(h0 + wave);
-        }
-        return;
     }
-    for (int h = h0; h < h0 + PG_WAVES && h < heads; h++) {
-        sum(h, wave * PAR + g, PG_WAVES * PAR);
+    if constexpr (WPH > 1) {
         so[wave][lane] = o;
         sl[wave][lane] = l;
         __syncthreads();
-        if (wave == 0) {
+        if (wave % WPH)
+            return;
 #pragma unroll
-            for (int x = 1; x < PG_WAVES; x++)
-                o += so[x][lane], l += sl[x][lane];
-            write(h);
-        }
-        __syncthreads();
+        for (int x = 1; x < WPH; x++)
+            o += so[wave + x][lane], l += sl[wave + x][lane];
     }
+    if (h < heads && g == 0 && d < P.hd)
+        *(pg_f4 *)(P.out + ((size_t)i * P.n_heads + kvh * P.group + block * PG_COLS + h) * P.hd + d) = pg_result(o, l);
 }
 
 // How a call runs.
@@ -711,8 +706,17 @@ int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t
         const size_t unit = PG_WAVES * PgCfg<HDP>::KT, most = items * ((max_rows + unit - 1) / unit);
         hipLaunchKernelGGL((paged_attn_cut_kernel<T, HDP, ONCE>), dim3(most < (size_t)plan.room ? most : plan.room),
                            dim3(PG_THREADS), 0, st, P);
-        hipLaunchKernelGGL((paged_attn_join_kernel<HDP>), dim3(plan.records, (P.cols + PG_WAVES - 1) / PG_WAVES),
-                           dim3(PG_THREADS), 0, st, P);
+        // with few items there may be hundreds of an item's records: two waves for a head.  Measured, 64 records of heads of
+        // 128 and 256, and about four of 112 items: one wave 10.3 us, 29 and 5.0, two 7.1, 6.2 and 4.6, four 5.6, 10 and 5.9.
+        const auto join = [&](auto waves) {
+            constexpr int WPH = decltype(waves)::value, EACH = PG_WAVES / WPH;
+            hipLaunchKernelGGL((paged_attn_join_kernel<HDP, WPH>), dim3(plan.records, (P.cols + EACH - 1) / EACH),
+                               dim3(PG_THREADS), 0, st, P);
+        };
+        if (plan.records > (size_t)plan.room)
+            join(std::integral_constant<int, 1>{});
+        else
+            join(std::integral_constant<int, 2>{});
         note_launch();
         note_launch();
     };
