@@ -935,7 +935,7 @@ typedef struct {
     size_t n_lanes, table_width, table_stride;
 } loomhip_pages;
 /* Keys and values of n tokens into the cache: token t at position r->pos[t] of
- * lane lanes[t] (int32; NULL: lane t), keys normed and rotated as by
+ * lane lanes[t] (int32; NULL: lane t of at least n), keys normed and rotated as by
  * loomhip_qk_norm_rope_dev (k->out unused), values as they are (f32
  * [n][k->n_heads][head_dim], tokens v_stride apart), each rounded once to the
  * cache's type (f16 past 65504 is infinite).  A token whose position has no
@@ -957,7 +957,8 @@ int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, con
  * for the heads that see it, a value that is NaN or infinite makes its element
  * of the result NaN, a key with a NaN all of it, and a key with an infinity
  * too, unless its score is minus infinity: then it may also count as a row not
- * seen.  The work is cut on the device by len, not by the table's width.  n lanes of the table's n_lanes; head_dim a
+ * seen.  The work is cut on the device by len, not by the table's width; the
+ * workspace is for max_rows = page_size * table_width.  n lanes of the table's n_lanes; head_dim a
  * multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^23, n times the
  * table's positions up to 2^38; DECLINED otherwise. */
 int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
@@ -979,7 +980,8 @@ size_t loomhip_paged_attn_ws(size_t max_rows, size_t n, size_t n_heads, size_t n
  * so small that 1/T passes f32): the first maximum has probability 1, as in
  * loomhip_token_probs_dev (its lp 0, every other -inf, the entropy 0); an
  * infinite one weighs finite logits alike and -inf as nothing.  A row of -inf
- * alone: -inf, entropy 0.  top up to 32, n up to 65535; DECLINED otherwise. */
+ * alone: -inf, entropy 0.  top up to 32, vocab up to 2^21, n up to 65535;
+ * DECLINED otherwise. */
 int loomhip_token_logprobs_dev(const float *logits, size_t n, size_t vocab, size_t stride, const int32_t *tokens,
                                const float *temperature, size_t top, float *logprobs, float *entropy, int32_t *top_ids,
                                float *top_logprobs, void *ws, size_t ws_bytes, void *stream);

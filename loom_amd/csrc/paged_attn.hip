@@ -173,7 +173,6 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
             qv[s][1] = *(const pg_f4 *)(q + (d < hd ? d : 0) + 4);
         }
     }
-
     typename T::v8 qp[STEPS][T::PARTS];
     float cs = P.scale * 0x1.715476p+0f; // scores in log2 units
     {
@@ -413,13 +412,14 @@ __device__ __forceinline__ uint32_t pg_wave_sum(uint32_t v) {
     v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+
 // The same with long items cut into pieces, a work group a piece.  How, every
 // wave works out by itself from the lengths: a lane of u units (a tile for each
 // wave) is cut into p = ceil(u / L) pieces of equal length, L the smallest of
 // some lengths from the chip's share (all units over the work groups that run
-// at a time) to twice that at which the pieces run in one round of the chip; half the
-// share where there are too many items for that (the work groups then take
-// pieces in turn).  Pieces are numbered lane by lane, [piece][item], so that
+// at a time) to twice that at which the pieces run in one round of the chip;
+// half the share where there are too many items for that (the work groups then
+// take pieces in turn).  Pieces are numbered lane by lane, [piece][item], so that
 // the blocks of query heads that read the same rows run side by side.  A piece
 // of a lane that is cut leaves a record (m, l, o).
 template <class T, int HDP, bool ONCE>

@@ -351,6 +351,37 @@ def test_paged_attn_many_lanes_are_cut(sv, shape):
     _within(_attn(sv, c).cpu().numpy(), *_attn_ref(c), "window")
 
 
+def test_paged_attn_thousands_of_lanes_are_cut(sv):
+    """More lanes than a wave has threads, many times over, most of them short; a page each that holds more than is left
+    whole."""
+    n = 2500
+    r = _rng(n)
+    lens = r.integers(0, 30, n)
+    lens[r.permutation(n)[:12]] = r.integers(300, 601, 12)
+    kp, vp = _cache(n, 600, 1, 8, "f16")
+    c = {"q": r.standard_normal((n, 2, 8)).astype(np.float32), "kp": kp, "vp": vp,
+         "table": r.permutation(n).astype(np.int32)[:, None], "lens": lens.astype(np.int32), "scale": 0.5, "window": 0}
+    want, bound = _attn_ref(c)
+    got = _attn(sv, c).cpu().numpy()
+    _within(got, want, bound)
+    assert (got[c["lens"] == 0] == 0).all()
+
+
+def test_paged_attn_of_a_decoders_caches(sv):
+    """Contiguous caches are pages of one lane each: [n, layers, ctx, kvd] at a layer."""
+    import torch
+
+    n, layers, ctx, KV, hd = 3, 4, 700, 2, 64
+    r = _rng(3)
+    cache = torch.from_numpy(r.standard_normal((2, n, layers, ctx, KV * hd)).astype(np.float32)).half().cuda()
+    for layer in (0, 3):
+        kp, vp = (x[:, layer].unflatten(-1, (KV, hd)) for x in cache)
+        c = {"q": r.standard_normal((n, 8, hd)).astype(np.float32), "kp": kp, "vp": vp,
+             "table": np.arange(n, dtype=np.int32)[:, None], "lens": np.array([700, 1, 333], np.int32), "scale": hd ** -0.5,
+             "window": 0}
+        _within(_attn(sv, c).cpu().numpy(), *_attn_ref(c), layer)
+
+
 def test_paged_attn_empty_batch_in_a_wide_table(sv):
     c = _attn_case(8, 2, 64, 16, [40, 0, 3], "f16", "rows", width=400)
     for lens in ([0, 0, 0], [0, 0, 1], [40, 0, 3]):

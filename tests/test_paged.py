@@ -116,6 +116,7 @@ def test_pages_are_refused(rc, args):
     (ARG, dict(vs=127)),
     (ARG, dict(v=0x400001)),
     (ARG, dict(lanes=FAKE + 1)),
+    (ARG, dict(n=5)),
     (ARG, dict(q=(0x100000, 256, None, 256, None, 4))),
     (ARG, dict(q=(0x100000, 256, 0x300000, 256, None, 4))),
     (ARG, dict(q=(0x100000, 256, 0x400000, 256, None, 4))),
