@@ -10,7 +10,8 @@
 // Products on the matrix cores, in the cache's own type (mfma 16x16x32), exact
 // in the cached values and near f32 in the others: an f16 cache takes the query
 // (scaled by a power of two of its own) and the weights in two f16 parts (22
-// bits), a bf16 cache in three bf16 parts (24).  The sums are f32.
+// bits; what is far below the largest of them to within 2^-38 of that), a bf16
+// cache in three bf16 parts (24).  The sums are f32.
 //
 // S^T = K Q^T: a lane holds one query head (column lane % 16) and, of each 32
 // rows, the rows 4 (lane / 16) + i and 16 + 4 (lane / 16) + i, i < 4.  These
@@ -46,7 +47,11 @@ int pages_check(const loomhip_pages *c, size_t n_kv, size_t hd, const char *fn);
 constexpr int PG_THREADS = 256, PG_WAVES = PG_THREADS / 64;
 constexpr int PG_MAX_HD = 256;
 constexpr int PG_COLS = 16; // query heads of an item
-constexpr size_t PG_WHOLE = 512; // rows up to which no lane is cut; half as many at head sizes over 128
+// Rows up to which no lane is cut (a launch less, but an item's rows one tile of a wave after the other); half as many at
+// head sizes over 128.  Measured, in a graph, 1, 8 and 64 lanes of 32 heads of 128 over 4, whole against cut: 256 rows
+// 6.7, 7.3, 8.3 us for 10.3, 10.9, 14.6; 512 rows 9.5, 11.2, 12.9 for 10.5, 11.3, 18; 1024 rows 17, 20, 23 for 11, 12,
+// 24.  Of 8 heads of 256 over 2: 256 rows 11.5, 12.8, 13.9 for 14.1, 15.1, 16.1; 512 rows 21, 22, 23 for 14.8, 16, 21.
+constexpr size_t PG_WHOLE = 512;
 
 // f16: two parts of a value, of a size that the second is normal; bf16: three, of f32's own range.
 struct PgF16 {
@@ -426,7 +431,9 @@ template <class T, int HDP, bool ONCE>
 __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_kernel(PagedAttnParams P) {
     using C = PgCfg<HDP>;
     constexpr uint32_t UNIT = PG_WAVES * C::KT, ROOM = pg_room(HDP);
-    constexpr int CUTS = 6, SIXTEENTHS[CUTS] = {16, 17, 18, 20, 24, 32}; // of the share
+    // L in sixteenths of the share.  Every quarter alone cut eight long lanes of 18 units a work group at 23 (126 us), these
+    // at 19 (114).
+    constexpr int CUTS = 6, SIXTEENTHS[CUTS] = {16, 17, 18, 20, 24, 32};
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
     __shared__ uint32_t before[2][65], firsts[64]; // pieces and records before a thread's lanes, its first lane's units

@@ -55,7 +55,9 @@ def attn(q, k_pages, v_pages, table, lens, scale, window):
     bits: four more) times the scale and log2 e (two), and the exponential's own two; with S = max_t |scale| sum_d |q_d
     k_d| a score is off by (hd + 8) EPS S, its exponential by the same relative amount, numerator and denominator by it
     each.  The weights are held to 22 bits (four), the sums run over T rows (T roundings each, worst case), the joins and
-    the division another 32.  All relative to sum_t p_t |v_t|."""
+    the division another 32.  All relative to sum_t p_t |v_t|.  Both are held in f16 parts, of which the second has no
+    digits below 2^-24: a query element, scaled so that the row's largest is 2^13 at least, and a weight, of which the
+    largest is 2^14, are off by up to 2^-25, 2^-38 and 2^-39 of the largest, however small they are themselves."""
     q, k_pages, v_pages = (np.asarray(a, np.float64) for a in (q, k_pages, v_pages))
     n, H, hd = q.shape
     pages, ps, KV = k_pages.shape[:3]
@@ -73,10 +75,12 @@ def attn(q, k_pages, v_pages, table, lens, scale, window):
             kh, vh = k[:, h // G], v[:, h // G]
             s = kh @ q[i, h] * scale
             S = np.max(np.abs(kh) @ np.abs(q[i, h])) * abs(scale)
+            small = np.max(np.abs(kh).sum(-1)) * np.abs(q[i, h]).max() * abs(scale) * 2.0 ** -38
             p = np.exp(s - s.max())
             p /= p.sum()
             out[i, h] = p @ vh
-            bound[i, h] = EPS * (2 * (hd + 8) * S + 4 + 2 * len(t) + 32) * (p @ np.abs(vh))
+            bound[i, h] = (EPS * (2 * (hd + 8) * S + 4 + 2 * len(t) + 32) + 2 * small) * (p @ np.abs(vh))
+            bound[i, h] += 2.0 ** -39 * np.abs(vh).sum(0)
     return out, bound
 
 
