@@ -406,16 +406,27 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_kernel(
     }
 }
 
-// A value's sum over the wave, in all of it.
-__device__ __forceinline__ uint32_t pg_wave_sum(uint32_t v) {
-    const auto add = [](uint32_t a, int b) { return a + (uint32_t)b; };
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, false));
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, false));
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, false));
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xF, 0xF, false));
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));
-    v = add(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));
-    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+// The sum of a value over the wave's lanes up to this one: shifts by 1, 2, 4 and 8 in the rows of 16 lanes, then the rows'
+// totals carried on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t pg_dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t pg_scan(uint32_t v) {
+    v += pg_dpp<0x111, 0xF>(v);
+    v += pg_dpp<0x112, 0xF>(v);
+    v += pg_dpp<0x114, 0xF>(v);
+    v += pg_dpp<0x118, 0xF>(v);
+    v += pg_dpp<0x142, 0xA>(v);
+    v += pg_dpp<0x143, 0xC>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t pg_last(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+// a / b for a < 2^24 (their quotient in f32 is off by less than 1 / 2)
+__device__ __forceinline__ uint32_t pg_div(uint32_t a, uint32_t b) {
+    const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+    const uint32_t r = a - q * b;
+    return (int32_t)r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
 // The same with long items cut into pieces, a work group a piece.  How, every
@@ -436,7 +447,7 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     constexpr int CUTS = 6, SIXTEENTHS[CUTS] = {16, 17, 18, 20, 24, 32};
     __shared__ __attribute__((aligned(16))) char smem[C::BYTES];
     __shared__ float sm[PG_WAVES][PG_COLS], sl[PG_WAVES][PG_COLS];
-    __shared__ uint32_t before[2][65], firsts[64]; // pieces and records before a thread's lanes, its first lane's units
+    __shared__ uint32_t before[2][65], firsts[2][64]; // pieces and records before a thread's lanes, its first lane's rows
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t items = (uint32_t)P.n_kv * P.blocks; // of a lane
     // every thread's lanes, a run of them
@@ -446,7 +457,10 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         pg_span(P, i, first, end);
         return (end - first + UNIT - 1) / UNIT;
     };
-    const uint32_t u0 = i0 < i1 ? units(i0) : 0; // most often the only one
+    uint32_t first0 = 0, end0 = 0; // of the first one, which is most often the only one
+    if (i0 < i1)
+        pg_span(P, i0, first0, end0);
+    const uint32_t u0 = (end0 - first0 + UNIT - 1) / UNIT;
     const auto each = [&](auto f) {
         if (i0 < i1)
             f(u0, i0);
@@ -455,9 +469,10 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     };
     uint32_t total = 0;
     each([&](uint32_t u, int) { total += u; });
-    total = pg_wave_sum(total);
-    const uint64_t share = ((uint64_t)total * items + ROOM - 1) / ROOM;
-    constexpr uint64_t MOST = 1 << 28; // longer than any lane
+    total = pg_last(pg_scan(total));
+    constexpr uint32_t MOST = 1 << 26; // longer than any lane
+    const uint64_t exact = ((uint64_t)total * items + ROOM - 1) / ROOM;
+    const uint32_t share = exact < 1 ? 1 : exact > MOST ? MOST : (uint32_t)exact;
     // ceil(u / L), at least 1; within a rounding of whole numbers it may be one off, which unsettles nothing: whoever counts
     // pieces counts them so
     const auto pieces = [](uint32_t u, uint32_t L) {
@@ -466,8 +481,7 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
     uint32_t cut[CUTS], count[CUTS];
 #pragma unroll
     for (int x = 0; x < CUTS; x++) {
-        const uint64_t c = (share * SIXTEENTHS[x] + 15) / 16;
-        cut[x] = c < 1 ? 1 : c > MOST ? (uint32_t)MOST : (uint32_t)c;
+        cut[x] = (share * SIXTEENTHS[x] + 15) / 16;
         count[x] = 0;
     }
     each([&](uint32_t u, int) {
@@ -475,11 +489,13 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         for (int x = 0; x < CUTS; x++)
             count[x] += pieces(u, cut[x]);
     });
-    uint32_t L = (share + 1) / 2 > MOST ? (uint32_t)MOST : (uint32_t)((share + 1) / 2);
-    L = L < 1 ? 1 : L;
+#pragma unroll
+    for (int x = 0; x < CUTS; x++)
+        count[x] = pg_scan(count[x]);
+    uint32_t L = (share + 1) / 2;
 #pragma unroll
     for (int x = CUTS - 1; x >= 0; x--)
-        if ((uint64_t)pg_wave_sum(count[x]) * items <= (uint64_t)ROOM)
+        if (pg_last(count[x]) * items <= ROOM)
             L = cut[x];
     // pieces and records of the lanes up to this thread's last
     uint32_t np = 0, nr = 0;
@@ -488,44 +504,36 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         np += p;
         nr += p > 1 ? p : 0;
     });
-    uint32_t to_p = np, to_r = nr;
-    for (int o = 1; o < 64; o *= 2) {
-        const uint32_t x = __shfl_up(to_p, o), y = __shfl_up(to_r, o);
-        to_p += lane >= o ? x : 0;
-        to_r += lane >= o ? y : 0;
-    }
-    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to_p, 63) * items;
+    const uint32_t to_p = pg_scan(np), to_r = pg_scan(nr), all = pg_last(to_p) * items;
     if (blockIdx.x == 0 && tid == 63)
         *P.records = to_r * items;
     if (tid < 64) { // out of the registers
         before[0][lane] = to_p - np, before[1][lane] = to_r - nr;
         if (lane == 63)
             before[0][64] = to_p;
-        firsts[lane] = u0;
+        firsts[0][lane] = first0, firsts[1][lane] = end0;
     }
     __syncthreads();
     for (uint32_t x = blockIdx.x; x < all; x += gridDim.x) {
-        const uint32_t w = pg_turn(P, x, all);
+        const uint32_t w = ONCE ? x : pg_turn(P, x, all);
         // its lane, by the thread that has it: the lane's pieces, those before it and the records before them
-        uint32_t sum = before[0][lane], rec = before[1][lane], p = 1, first = 0, end = 0;
+        uint32_t sum = before[0][lane], rec = before[1][lane], p = 1, first = firsts[0][lane], end = firsts[1][lane];
         const bool has = sum * items <= w && w < before[0][lane + 1] * items;
         int i = lane * per;
-        if (has) {
-            for (uint32_t u = firsts[lane];; u = units(++i)) {
-                p = pieces(u, L);
+        if (has)
+            for (;; pg_span(P, ++i, first, end)) {
+                p = pieces((end - first + UNIT - 1) / UNIT, L);
                 if (w < (sum + p) * items)
                     break;
                 sum += p;
                 rec += p > 1 ? p : 0;
             }
-            pg_span(P, i, first, end);
-        }
         const int src = __builtin_ctzll(__ballot(has));
         const auto from = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, src); };
         i = (int)from((uint32_t)i), p = from(p), sum = from(sum), rec = from(rec), first = from(first), end = from(end);
-        const uint32_t piece = w / items - sum, item = w - w / items * items; // sum * items are before it
-        const uint32_t u = (end - first + UNIT - 1) / UNIT;
-        const uint32_t a = u / p * piece + (piece < u % p ? piece : u % p), b = a + u / p + (piece < u % p);
+        const uint32_t turn = pg_div(w, items), piece = turn - sum, item = w - turn * items; // sum * items are before it
+        const uint32_t u = (end - first + UNIT - 1) / UNIT, base = pg_div(u, p), more = u - base * p;
+        const uint32_t a = base * piece + (piece < more ? piece : more), b = a + base + (piece < more);
         const int kvh = ONCE ? item : item / P.blocks, block = ONCE ? 0 : item - kvh * P.blocks;
         const int h0 = kvh * P.group + block * PG_COLS;
         const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
