@@ -14,9 +14,9 @@
 // where parts and their join take 10.7); of a longer one each part leaves (m, S,
 // Z) and its own k, which a second launch joins.
 //
-// Bound by bytes without alternatives (509 rows of 151936 50 us, 6.2 TB/s, and 5
+// Bound by bytes without alternatives (509 rows of 151936 48 us, 6.4 TB/s, and 5
 // for the join); with them by what a work group does one step after the other
-// once it has its part: 64 rows with 20 best 14.7 us, without 9.2, and 6.6 for
+// once it has its part: 64 rows with 20 best 14.8 us, without 9.2, and 6.6 for
 // the join, 4.
 #include "sampling.hpp"
 

@@ -11,9 +11,9 @@
 // 1e-7) for the library's sine and cosine.  Everything else is in f32; keys and
 // values are rounded once, to the nearest, on their way into the cache.
 //
-// Bound by bytes.  Measured: 4096 tokens of 32 and 4 heads of 128 29.8 us (151
+// Bound by bytes.  Measured: 4096 tokens of 32 and 4 heads of 128 29.9 us (151
 // MB, 5.1 TB/s: a large copy runs at 4.8), 4101 tokens with queries into the pages
-// 31.0 (160 MB), one token 3.3, a launch.  Norm weights as loads of single values
+// 31.0 (160 MB), one token 3.4, a launch.  Norm weights as loads of single values
 // and pointers indexed by a lane's kind of head took 47; several tokens a work
 // group, with loops over their heads, 33 to 35.
 #include "runtime.hpp"

@@ -24,12 +24,12 @@
 // page's rows wherever they lie, 16 bytes a thread), put into LDS when the wave
 // is through with the one before, and the next tile's loads go out; two work
 // groups a CU keep up to 128 KB in flight, and the products (512 cycles of a
-// tile's 11000) hide behind them.  Measured, 32 heads of 128 over 4 key heads:
-// 8 lanes of up to 65536 rows, bf16, 106 us (604 MB, 5.7 TB/s, where a plain read
+// tile's 7500) hide behind them.  Measured, 32 heads of 128 over 4 key heads: 8
+// lanes of up to 65536 rows, bf16, 103 us (604 MB, 5.9 TB/s, where a plain read
 // of that many bytes runs at 7.0: work groups start and end together, and
 // pieces are up to a twentieth longer than the share), 32 lanes of up to 4096,
-// f16, 30 us (139 MB; about 6 of them the look-up of lengths, pages and first
-// tiles, and the joins) and 4.6 for the records; one lane of 256 rows 6.9.
+// f16, 29 us (139 MB; 5 of them until the first tiles are asked for: lengths,
+// plan, pages) and 5 for the records; one lane of 256 rows 6.9.
 #include "runtime.hpp"
 
 #include <type_traits>
@@ -225,7 +225,7 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         return __ballot(in);
     };
     // The rows' chunks, their places from the lanes that have them.  Rows that one item alone reads (ONCE) pass the caches
-    // by: 604 MB take 114 us, with plain loads 126.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (48
+    // by: 604 MB take 110 us, with plain loads 10 % more.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (41
     // with the blocks on one XCD, pg_turn).
     const auto load = [&](uint32_t unit) {
         uint32_t from[C::NL];
