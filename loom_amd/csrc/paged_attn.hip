@@ -28,8 +28,8 @@
 // lanes of up to 65536 rows, bf16, 103 us (604 MB, 5.9 TB/s, where a plain read
 // of that many bytes runs at 7.0: work groups start and end together, and
 // pieces are up to a twentieth longer than the share), 32 lanes of up to 4096,
-// f16, 29 us (139 MB; 5 of them until the first tiles are asked for: lengths,
-// plan, pages) and 5 for the records; one lane of 256 rows 6.9.
+// f16, 29 us (139 MB, 4.8 TB/s: lengths, plan and pages one after the other stand
+// before the first tiles) and 5 for the records; one lane of 256 rows 6.9.
 #include "runtime.hpp"
 
 #include <type_traits>
@@ -225,8 +225,8 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
         return __ballot(in);
     };
     // The rows' chunks, their places from the lanes that have them.  Rows that one item alone reads (ONCE) pass the caches
-    // by: 604 MB take 110 us, with plain loads 10 % more.  Where four blocks of heads share them, 307 MB in all, 70 us and 65 (41
-    // with the blocks on one XCD, pg_turn).
+    // by: 604 MB and the records take 111 us, with plain loads 121; 139 MB 34.4 and 37.3.  Where four blocks of heads share
+    // them, 307 MB in all, 70 us and 65 (41 with the blocks on one XCD, pg_turn).
     const auto load = [&](uint32_t unit) {
         uint32_t from[C::NL];
 #pragma unroll
