@@ -434,7 +434,10 @@ __device__ __forceinline__ uint32_t pg_scan(uint32_t v) {
     return v;
 }
 __device__ __forceinline__ uint32_t pg_last(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
-// a / b for a < 2^24 (their quotient in f32 is off by less than 1 / 2)
+// a / b for a <= 2^24, which has f32's digits: a reciprocal of a unit in the last place and the product's rounding take the
+// quotient at most 3 * 2^-24 of itself off, 1 at b = 3, and nothing where b is a power of two; so it is one off at most.
+// A lane has at most 2^31 / 128 units, a call at most 2^23 items and 4 records for each work group that runs at a time.
+// Every a with every b up to 70000 was compared with the division of whole numbers.
 __device__ __forceinline__ uint32_t pg_div(uint32_t a, uint32_t b) {
     const uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
     const uint32_t r = a - q * b;
