@@ -131,8 +131,6 @@ __global__ __launch_bounds__(RP_THREADS) void rope_kernel(RopeParams P) {
         float s, c;
         sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
         cosines[tid] = c, sines[tid] = s;
-    } else if (tid < PAIRS) {
-        cosines[tid] = 1.0f, sines[tid] = 0.0f;
     }
     __syncthreads();
     rp_f4 a = va, b = vb;
@@ -158,6 +156,8 @@ __global__ __launch_bounds__(RP_THREADS) void rope_kernel(RopeParams P) {
         const rp_f4 c = *(const rp_f4 *)(cosines + p0), s = *(const rp_f4 *)(sines + p0);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
+            if (!VEC && p0 + e >= half) // behind the last rotated pair: not by a cosine of 1, for infinity times 0 is NaN
+                break;
             const float u = a[e];
             a[e] = __builtin_fmaf(u, c[e], -(b[e] * s[e]));
             b[e] = __builtin_fmaf(b[e], c[e], u * s[e]);

@@ -146,6 +146,36 @@ def test_qk_norm_rope_of_nothing_and_of_no_number(sv):
     assert sv.qk_norm_rope_dev(e, None, args[0][:0], args[1])[0].shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("inter", [False, True], ids=["halves", "neighbours"])
+@pytest.mark.parametrize("hd,rot", [(64, 20), (64, 2), (24, 12), (128, 126), (256, 250), (64, 32)])
+def test_what_is_not_rotated_stays_as_it_is(sv, hd, rot, inter):
+    """Infinities, NaN and -0 right behind the rotated values leave their neighbours alone, in q, k and the pages."""
+    import torch
+
+    n, H, KV, ps = 6, 3, 2, 4
+    c = _rope_case(n, H, KV, hd, rot, norm=False)
+    c["pos"] = np.arange(n, dtype=np.int32)
+    for x in (c["q"], c["k"]):
+        for t, odd in enumerate((np.inf, -np.inf, np.nan, -0.0)):
+            for h in range(x.shape[1]):
+                x[t, h, rot + (h + t) % min(6, hd - rot)] = odd  # in the same four pairs as the last rotated ones, and behind
+        x[4, :, rot:] = -0.0
+    q0, k0 = _dev(c["q"]), _dev(c["k"])
+    q, k = sv.qk_norm_rope_dev(q0, k0, _dev(c["pos"]), _dev(c["freqs"]), interleaved=inter)
+    for name, x, got in (("q", q0, q), ("k", k0, k)):
+        assert torch.equal(got[..., rot:].contiguous().view(torch.int32), x[..., rot:].contiguous().view(torch.int32)), name
+        part = {"x": c[name][..., :rot], "pos": c["pos"], "freqs": c["freqs"], "w": None, "eps": 0, "interleaved": inter}
+        _within(_np(got[..., :rot]), *ref.norm_rope(**part), name)
+    for kind, dt in (("f16", torch.float16), ("bf16", torch.bfloat16)):
+        kp, vp = _cache(2, ps, KV, hd, kind)
+        sv.paged_append_dev(k0, k0, kp, vp, _dev(np.array([[1, 0]], np.int32)), _dev(c["pos"]), freqs=_dev(c["freqs"]),
+                            lanes=_dev(np.zeros(n, np.int32)), interleaved=inter)
+        for t in range(n):
+            got, want = kp[1 - t // ps, t % ps, :, rot:].float(), k0[t, :, rot:].to(dt).float()
+            assert torch.equal(got.isnan(), want.isnan())
+            assert ((got == want) & (got.signbit() == want.signbit()) | want.isnan()).all(), (kind, t)
+
+
 # ---- into the pages ---------------------------------------------------------------
 
 
