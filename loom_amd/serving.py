@@ -447,9 +447,11 @@ def token_logprobs_dev(logits, tokens, top: int = 0, temperature=None):
     if not shape or logits.dtype is not _F32 or not logits.is_contiguous():
         raise ValueError("logits: contiguous f32")
     lead, vocab = shape[:-1], shape[-1]
-    n = logits.numel() // vocab if vocab else 0
     if not _is(tokens, _I32, *lead):
         raise ValueError("tokens: int32, one a row")
+    n = tokens.numel()
+    if n and not vocab:
+        raise ValueError("logits: rows of no values")
     if temperature is not None and not _is(temperature, _F32, *lead):
         raise ValueError("temperature: f32, one a row")
     if top < 0:

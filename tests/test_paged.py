@@ -262,6 +262,15 @@ def test_python_checks():
             assert "on the GPU" not in str(e.value), x
 
 
+def test_log_probabilities_of_no_vocabulary_are_refused():
+    """Rows without values have no results that could be left unwritten; no rows are nothing to do, whatever their length."""
+    for shape in ((3, 0), (2, 3, 0), (0,)):
+        with pytest.raises(ValueError, match="no values"):
+            serving.token_logprobs_dev(_t(*shape), _t(*shape[:-1], dtype=torch.int32), top=2)
+    with pytest.raises(ValueError, match="not on the GPU"):
+        serving.token_logprobs_dev(_t(0, 0), _t(0, dtype=torch.int32), top=2)
+
+
 def test_rotation_keeps_lengths_and_relative_angles():
     """The definition: rotated pairs keep their length, and (q at p) . (k at r) hangs on p - r alone."""
     r = np.random.default_rng(1)
