@@ -336,28 +336,29 @@ __device__ __forceinline__ LpRec lp_sums(const smp_f4 (&v)[NV], size_t v0, const
     if (sc.greedy)
         return {m, 1.0f, 0.0f, at};
     // (x - m) / T log2 e = d hi + d lo; d no further below than where the exponential has long been 0, so that neither
-    // product is infinite.  At a T that no f32 is that far below, -inf is told apart.
+    // product is infinite.  At a T past which d is of halves (1e30) that may be further than f32 reaches, and -inf is told
+    // apart.
     const float from = m == -__builtin_inff() ? 0.0f : m, least = -300.0f / sc.hi;
     float s = 0.0f, z = 0.0f;
-    const auto add = [&](float x, bool finite) {
-        const float d = finite ? fmaxf(x - from, least) : x - from, h = __builtin_fmaf(d, sc.hi, d * sc.lo);
+    const auto add = [&](float d) {
+        const float h = __builtin_fmaf(d, sc.hi, d * sc.lo);
         const float e = __builtin_amdgcn_exp2f(h);
         s += e;
         z = __builtin_fmaf(e, h, z);
     };
-    if (least > -3.0e38f) {
+    if (sc.part == 1.0f) {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++)
-                add(v[i][c], true);
+                add(fmaxf(v[i][c] - from, least));
     } else {
 #pragma unroll
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++)
                 if (v[i][c] != -__builtin_inff())
-                    add(v[i][c], false);
+                    add(prob_diff(sc, v[i][c], from));
     }
     if (nan || m == __builtin_inff()) // lost on the way
         s = __builtin_nanf("");
@@ -461,7 +462,7 @@ __global__ __launch_bounds__(SMP_THREADS) void logprobs_join_kernel(LogprobParam
     double s = 0.0, z = 0.0;
     for (int i = tid; i < P.splits; i += SMP_THREADS) {
         const LpRec r = rec[i];
-        const float d = r.m - m;
+        const float d = prob_diff(sc, r.m, m);
         const double f = r.m == -__builtin_inff() ? 1.0 : (double)exp_scaled(d, sc.hi, sc.lo); // a part of -inf has 0 or NaN
         s += f * (double)r.s;
         z += f * ((double)r.z + (double)r.s * (double)fmaxf(d * sc.hi, -200.0f));

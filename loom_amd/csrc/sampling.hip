@@ -58,7 +58,7 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_reduce_kernel(const float *
     for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int c = 0; c < 4; c++)
-            l += exp_scaled(v[i][c] - from, sc.hi, sc.lo);
+            l += exp_scaled(prob_diff(sc, v[i][c], from), sc.hi, sc.lo);
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
     if (lane == 0)
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *l
     float l = 0.0f;
     for (int s = lane; s < splits; s += 64) {
         const ProbRec r = rec[row * splits + s];
-        l += r.m == -__builtin_inff() ? r.l : r.l * exp_scaled(r.m - m, sc.hi, sc.lo);
+        l += r.m == -__builtin_inff() ? r.l : r.l * exp_scaled(prob_diff(sc, r.m, m), sc.hi, sc.lo);
     }
     for (int o = 1; o < 64; o *= 2)
         l += __shfl_xor(l, o);
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(SMP_THREADS) void probs_write_kernel(const float *l
         smp_f4 e;
 #pragma unroll
         for (int c = 0; c < 4; c++)
-            e[c] = sc.greedy ? ((int64_t)(k + c) == at ? 1.0f : 0.0f) : exp_scaled(v[i][c] - m, sc.hi, sc.lo) * inv;
+            e[c] = sc.greedy ? ((int64_t)(k + c) == at ? 1.0f : 0.0f) : exp_scaled(prob_diff(sc, v[i][c], m), sc.hi, sc.lo) * inv;
         if (k + 4 <= vocab) {
             __builtin_nontemporal_store(e, (smp_f4u *)(p + k));
         } else {
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(THREADS) void probs_row_kernel(const float *logits,
         for (int i = 0; i < NV; i++)
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                v[i][c] = exp_scaled(v[i][c] - m, sc.hi, sc.lo);
+                v[i][c] = exp_scaled(prob_diff(sc, v[i][c], m), sc.hi, sc.lo);
                 l += v[i][c];
             }
         for (int o = 1; o < 64; o *= 2)

@@ -46,8 +46,8 @@ __device__ __forceinline__ void row_part(const float *x, size_t v0, size_t vocab
         v[i] = row_four(x, v0 + ((size_t)i * THREADS + threadIdx.x) * 4, vocab, fill);
 }
 
-// exp((x - m) / T) with c = 1/T * log2 e split into a float and its remainder,
-// so that the exponent's rounding does not grow with |x - m| / T.
+// 2^(d c), d a difference of logits (prob_diff) and c its factor, split into a
+// float and its remainder so that the exponent's rounding does not grow with d c.
 __device__ __forceinline__ float exp_scaled(float d, float c_hi, float c_lo) {
     const float h = d * c_hi;
     const float r = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c_hi, -h));
@@ -56,16 +56,24 @@ __device__ __forceinline__ float exp_scaled(float d, float c_hi, float c_lo) {
     return h > -150.0f || h != h ? __builtin_fmaf(e, r * 0.69314718f, e) : 0.0f;
 }
 
+// (x - m) / T log2 e = prob_diff(x, m) (hi + lo)
 struct ProbScale {
-    float hi, lo;
+    float hi, lo, part;
     bool greedy;
 };
 __device__ __forceinline__ ProbScale prob_scale(const float *temperature, size_t row) {
     const float t = temperature ? temperature[row] : 1.0f;
-    const double c = 0x1.71547652b82fep+0 / (double)t;
+    double c = 0x1.71547652b82fep+0 / (double)t;
+    // Past a T of 1e30 a difference of logits that f32 does not hold is no longer where the exponential is 0: the
+    // difference of their halves is, with twice the factor.
+    const float part = c < 1e-30 ? 0.5f : 1.0f;
+    c = part == 0.5f ? 2.0 * c : c;
     // an infinite T weighs finite logits alike: the smallest factor there is, not 0, which times a masked -inf is NaN
     const float hi = (float)c == 0.0f ? 0x1p-149f : (float)c;
-    return {hi, (float)(c - (double)hi), !(t > 0.0f) || !(hi < __builtin_inff())};
+    return {hi, (float)(c - (double)hi), part, !(t > 0.0f) || !(hi < __builtin_inff())};
+}
+__device__ __forceinline__ float prob_diff(const ProbScale &sc, float x, float m) {
+    return __builtin_fmaf(x, sc.part, -(m * sc.part));
 }
 
 __device__ __forceinline__ void max_first(float &m, int &at, float m2, int at2) {

@@ -655,6 +655,24 @@ def test_token_logprobs_temperatures(sv, V):
         _lp_check(sv, x, tokens, top, t, top)
 
 
+@pytest.mark.parametrize("V", [700, 20000, 32000, 40001, 151936])
+def test_token_logprobs_of_logits_further_apart_than_f32_reaches(sv, V):
+    """Finite logits whose difference passes f32's range, at temperatures at which it counts and at ordinary ones."""
+    t = np.float32([np.inf, np.inf, 3.2e38, 1e38, 1e37, 2e36, 1e36, 1e31, 1e30, 9e29, 1.0, 0.5])
+    x = (_rng(V, 4).uniform(-1, 1, (len(t), V)) * 3.4e38).astype(np.float32)
+    x[1, :V - V // 3] = -3.4e38  # whole parts of a long row far below its maximum
+    x[1, V - V // 3:] = 3.4e38
+    x[2, :V // 2] = -3.3e38
+    x[4, ::2] = -3.4e38
+    x[4, 1::2] = 3.4e38
+    tokens = np.array([0, V - 1] * (len(t) // 2), np.int32)
+    for top in (0, 6):
+        _lp_check(sv, x, tokens, top, t, top)
+    x[:, 3::5] = -np.inf  # masked ones have no part in it
+    for top in (0, 6):
+        _lp_check(sv, x, tokens, top, t, top)
+
+
 @pytest.mark.parametrize("V,threads", [(4000, 256), (32000, 256), (32000, 1024), (151936, 256)])
 def test_token_logprobs_where_few_threads_hold_the_largest(sv, V, threads):
     """Every value of half of the threads above all others: more reach the bound than are collected."""

@@ -55,6 +55,19 @@ def test_token_probs_infinite_temperature(sv, vocab):
     _within(got, want, bound)
 
 
+@pytest.mark.parametrize("vocab", [700, 4097, 20000, 40001, 151936])
+def test_token_probs_of_logits_further_apart_than_f32_reaches(sv, vocab):
+    """Finite logits whose difference passes f32's range, at temperatures at which it counts and at ordinary ones."""
+    t = np.float32([np.inf, np.inf, 3.2e38, 1e38, 1e37, 2e36, 1e36, 1e31, 1e30, 9e29, 1.0, 0.5])
+    x = (_rng(vocab, 6).uniform(-1, 1, (len(t), vocab)) * 3.4e38).astype(np.float32)
+    x[1, :vocab - vocab // 3] = -3.4e38
+    x[1, vocab - vocab // 3:] = 3.4e38
+    x[4, ::2] = -3.4e38
+    x[4, 1::2] = 3.4e38
+    got = sv.token_probs_dev(_dev(x), _dev(t)).cpu().numpy().astype(np.float64)
+    _within(got, *ref.token_probs(x, t))
+
+
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("lanes", [1, 40])
