@@ -58,7 +58,8 @@ struct PgF16 {
     typedef pg_h8 v8;
     typedef _Float16 elem;
     static constexpr int PARTS = 2;
-    static constexpr float SHIFT = 14.0f; // weights are 2^(s - m + SHIFT), at most 2^14: their second parts stay normal
+    // weights are 2^(s - m + shift), at most 2^14: their second parts stay normal
+    static __device__ __forceinline__ float shift(uint32_t) { return 14.0f; }
     static __device__ __forceinline__ pg_f4 mfma(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -67,7 +68,9 @@ struct PgBf16 {
     typedef pg_b8 v8;
     typedef __bf16 elem;
     static constexpr int PARTS = 3;
-    static constexpr float SHIFT = 0.0f;
+    // Values reach as far as f32: all weights of a lane's rows together are less than 1/2, so that no sum of products is
+    // larger than the largest value.  No smaller than that takes, for the weights themselves end at 2^-126.
+    static __device__ __forceinline__ float shift(uint32_t rows) { return (float)(__clz((int)rows) - 33); }
     static __device__ __forceinline__ pg_f4 mfma(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -145,15 +148,17 @@ struct PgCfg {
     static constexpr int BYTES = PG_WAVES * (WAVE > JOIN ? WAVE : JOIN);
 };
 
-// Query heads [h0, h0 + heads) of lane i, which read key head kvh, against its
-// rows [r0, r1): the four waves' (m, l, o), in LDS.
+// Query heads [h0, h0 + heads) of lane i, which sees `rows` rows and reads key
+// head kvh, against its rows [r0, r1): the four waves' (m, l, o), in LDS.
 template <class T, int HDP, bool ONCE, bool EARLY>
-__device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh, int h0, int heads, uint32_t r0,
-                                        uint32_t r1, char *smem, float (*sm)[PG_COLS], float (*sl)[PG_COLS]) {
+__device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh, int h0, int heads, uint32_t rows,
+                                        uint32_t r0, uint32_t r1, char *smem, float (*sm)[PG_COLS],
+                                        float (*sl)[PG_COLS]) {
     using C = PgCfg<HDP>;
     constexpr int STEPS = HDP / 32, DB = HDP / 16, NB = C::KT / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quad = lane >> 4, col = lane & 15;
     const int hd = P.hd;
+    const float shift = T::shift(rows);
     char *tile = smem + wave * C::WAVE;
 
     // the page of the lane's row (lane % KT) of the tile that starts at row `at`; the first two tiles' are on their way
@@ -333,7 +338,7 @@ __device__ __forceinline__ void pg_rows(const PagedAttnParams &P, int i, int kvh
             typename T::v8 pp[T::PARTS];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float w = __builtin_amdgcn_exp2f(s[b][e] - top + T::SHIFT); // in this order: 14 is lost in a large m
+                const float w = __builtin_amdgcn_exp2f(s[b][e] - top + shift); // in this order: the shift is lost in a large m
                 l += w;
                 pg_split<T>(w, e, pp);
             }
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_kernel(
     const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
     uint32_t r0, r1;
     pg_span(P, i, r0, r1);
-    pg_rows<T, HDP, ONCE, false>(P, i, kvh, h0, heads, r0, r1, smem, sm, sl);
+    pg_rows<T, HDP, ONCE, false>(P, i, kvh, h0, heads, r1 - r0, r0, r1, smem, sm, sl);
     for (int x = threadIdx.x; x < heads * (HDP / 4); x += PG_THREADS) {
         const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;
         float M, L;
@@ -552,7 +557,8 @@ __global__ __launch_bounds__(PG_THREADS, pg_groups<HDP>) void paged_attn_cut_ker
         const int kvh = ONCE ? item : item / P.blocks, block = ONCE ? 0 : item - kvh * P.blocks;
         const int h0 = kvh * P.group + block * PG_COLS;
         const int heads = P.group - block * PG_COLS < PG_COLS ? P.group - block * PG_COLS : PG_COLS;
-        pg_rows<T, HDP, ONCE, HDP <= 128>(P, i, kvh, h0, heads, first + a * UNIT, b == u ? end : first + b * UNIT, smem, sm, sl);
+        pg_rows<T, HDP, ONCE, HDP <= 128>(P, i, kvh, h0, heads, end - first, first + a * UNIT, b == u ? end : first + b * UNIT, smem,
+                                             sm, sl);
         rec = rec * items + item * p + piece;
         for (int x = tid; x < heads * (HDP / 4); x += PG_THREADS) {
             const int h = x / (HDP / 4), d = x % (HDP / 4) * 4;

@@ -528,6 +528,55 @@ def test_paged_attn_of_one_row_that_outweighs_all(sv, kind, size):
     assert (_np(_attn(sv, c)) == want).all()
 
 
+BIG = [
+    # heads, key heads, head size, page size, lens: whole lanes, and lanes that are cut
+    (8, 2, 64, 16, [4, 1, 100, 3, 64]), (8, 2, 256, 16, [2, 90, 0, 127]), (4, 1, 128, 16, [5000, 4, 700]),
+    (2, 1, 256, 32, [3000, 2]), (20, 1, 48, 16, [40000, 65, 4096]),
+]
+
+
+@pytest.mark.parametrize("kind,big", [("bf16", 3.38e38), ("f16", 65504.0)])
+@pytest.mark.parametrize("shape", BIG, ids=lambda s: "x".join(map(str, s[:4])) + f"x{max(s[4])}")
+def test_paged_attn_values_at_the_end_of_the_range(sv, shape, kind, big):
+    """A weighted mean is no larger than its largest value: finite values have finite results, whatever their sums."""
+    c = _attn_case(*shape, kind, "rows")
+    r = _rng(5, *shape[:4])
+    signs = [np.ones(c["vp"].shape), -np.ones(c["vp"].shape), r.choice([-1.0, 1.0], c["vp"].shape)]
+    for q in (0.0, 1.0):  # equal weights, others
+        c["q"] = c["q"] * np.float32(q)
+        for s in signs + [r.uniform(-1, 1, c["vp"].shape)]:
+            c["vp"].copy_(_half(s * big, kind))
+            _within(_attn(sv, c).cpu().numpy(), *_attn_ref(c), q)
+        c["q"] = r.standard_normal(c["q"].shape).astype(np.float32)
+    c["vp"].copy_(_half(signs[0] * big, kind))
+    c["q"][:] = 0
+    top = _np(c["vp"][0, 0, 0, 0])
+    got = _np(_attn(sv, c))[c["lens"] > 0]
+    # the sum of T weights of 2^-k, the products of the value, the quotient: off by the sums' roundings, T EPS at most
+    assert (np.abs(got / top - 1) <= (max(shape[4]) + 40) * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("lens", [[33, 2, 200], [9000, 700]], ids=["whole", "cut"])
+def test_paged_attn_weights_far_below_the_largest(sv, lens):
+    """One row of nearly all the weight and the value 0; the result is the others' share, 2^-90 of their values."""
+    hd = 64
+    c = _attn_case(2, 1, hd, 16, lens, "bf16", "rows")
+    c["kp"][:], c["vp"][:] = 0, float(2.0 ** 100)
+    for i, n in enumerate(lens):
+        t = n // 2
+        c["kp"][int(c["table"][i, t // 16]), t % 16, 0, 3] = 1.0
+        c["vp"][int(c["table"][i, t // 16]), t % 16] = 0
+    c["q"][:] = 0
+    c["q"][:, :, 3] = 1.0
+    c["scale"] = 90 * np.log(2.0)
+    got = _np(_attn(sv, c))
+    for i, n in enumerate(lens):
+        # a score of 90 in units of 2: the scale in f32, the factor log2 e, their products: 6 roundings of 90, times log 2;
+        # sums of n weights
+        want = (n - 1) * 2.0 ** 10
+        assert (np.abs(got[i] / want - 1) <= (6 * 90 + n + 40) * 2.0 ** -24).all(), (n, got[i].min(), got[i].max(), want)
+
+
 def test_paged_attn_growing_maxima(sv):
     """Scores that rise over hundreds of units along the cache: the running maximum moves in every tile."""
     c = _attn_case(4, 2, 64, 16, [2000, 900], "f16", "rows")
