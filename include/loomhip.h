@@ -940,9 +940,10 @@ typedef struct {
  * [n][k->n_heads][head_dim], tokens v_stride apart), each rounded once to the
  * cache's type (f16 past 65504 is infinite).  A token whose position has no
  * page, or whose lane is outside the table, is not stored.  Two tokens at one
- * position of one lane leave a row of unspecified ones of their values.  q, if
- * not NULL: the tokens' queries, normed and rotated to q->out in the same
- * launch (q->out may be q->x). */
+ * position of one lane leave a row of unspecified ones of their values; so do
+ * pools that share elements, of k and v (which may not be the same) or of two
+ * rows.  q, if not NULL: the tokens' queries, normed and rotated to q->out in
+ * the same launch (q->out may be q->x). */
 int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, const loomhip_heads *k, const float *v,
                              size_t v_stride, const int32_t *lanes, const loomhip_rope *r, size_t n, size_t head_dim,
                              void *stream);

@@ -370,6 +370,8 @@ int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, con
         return fail(LOOMHIP_ERR_ARG, "%s: lanes not aligned to their elements", fn);
     if (!lanes && n > c->n_lanes)
         return fail(LOOMHIP_ERR_ARG, "%s: %zu tokens without their lanes, a table of %zu", fn, n, c->n_lanes);
+    if (c->k == c->v) // attention may read one pool as both
+        return fail(LOOMHIP_ERR_ARG, "%s: keys and values go to one pool", fn);
     RopeParams P = {};
     rope_set(P, r, n, head_dim);
     heads_set(P, 1, k);

@@ -363,8 +363,9 @@ def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None,
     strides that are multiples of 8; the values of a head one after the other); table int32 [lanes, pages of a lane];
     token t goes to position pos[t] of lane lanes[t] (int32 [n]; None: lane t).  A token of a negative position is
     padding; one whose position has no page in the table (an entry outside the pool, a position past it) is not stored.
-    Two tokens must not have one position of one lane.  q f32 [n, n_heads, head_dim]: the tokens' queries, normed and
-    rotated in the same launch; returns q_out (``q_out=q``: in place), None without q.
+    Two tokens must not have one position of one lane, nor k_pages and v_pages share elements.  q f32 [n, n_heads,
+    head_dim]: the tokens' queries, normed and rotated in the same launch; returns q_out (``q_out=q``: in place), None
+    without q.
     """
     if k.dim() != 3:
         raise ValueError("k [n, n_kv_heads, head_dim]")

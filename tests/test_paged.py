@@ -127,6 +127,12 @@ def test_paged_append_refuses(rc, args):
     assert "paged_append" in loom_amd.last_error()
 
 
+def test_paged_append_refuses_one_pool_for_keys_and_values():
+    """Their rows would be written by two threads each."""
+    assert _append(pages=_pages(k=0x600000, v=0x600000)) == ARG
+    assert "one pool" in loom_amd.last_error()
+
+
 def _attn(pages=None, q=FAKE, lens=FAKE, n=2, heads=4, kv=2, hd=64, window=0, out=FAKE, ws=FAKE, ws_bytes=1 << 40):
     return loom_amd.lib().loomhip_paged_attn_dev(C.byref(pages or _pages()), q, lens, n, heads, kv, hd, 0.125, window, out, ws,
                                                  ws_bytes, None)
