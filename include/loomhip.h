@@ -959,8 +959,8 @@ int loomhip_paged_append_dev(const loomhip_pages *c, const loomhip_heads *q, con
  * of the result NaN, a key with a NaN all of it, and a key with an infinity
  * too, unless its score is minus infinity: then it may also count as a row not
  * seen.  The work is cut on the device by len, not by the table's width; the
- * workspace is for max_rows = page_size * table_width.  n lanes of the table's n_lanes; head_dim a
- * multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^23, n times the
+ * workspace is for max_rows = page_size * table_width.  n lanes of the table's n_lanes; q and out at
+ * multiples of 16 bytes, head_dim a multiple of 8 up to 256, n up to 65535, n * n_heads up to 2^23, n times the
  * table's positions up to 2^38; DECLINED otherwise. */
 int loomhip_paged_attn_dev(const loomhip_pages *c, const float *q, const int32_t *len, size_t n, size_t n_heads,
                            size_t n_kv_heads, size_t head_dim, float scale, size_t window, float *out, void *ws,

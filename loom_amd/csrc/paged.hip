@@ -8,12 +8,14 @@
 // The angle is taken in 64 bits, as turns t / 2 pi without their whole part:
 // a position of a million leaves an f32 angle no digits below 2^-4.  The rest,
 // at most half a turn, is rounded to f32 (off by up to 2^-26 turns, an angle of
-// 1e-7) for the library's sine and cosine.  Everything else is in f32; keys and
-// values are rounded once, to the nearest, on their way into the cache.
+// 1e-7) for the library's sine and cosine: results are off by 8e-8 of their size
+// in the mean square, 6.5e-8 with both in 64 bits.  Everything else is in f32;
+// keys and values are rounded once, to the nearest, on their way into the cache.
 //
-// Bound by bytes.  Measured: 4096 tokens of 32 and 4 heads of 128 29.9 us (151
+// Bound by bytes.  Measured: 4096 tokens of 32 and 4 heads of 128 29.8 us (151
 // MB, 5.1 TB/s: a large copy runs at 4.8), 4101 tokens with queries into the pages
-// 31.0 (160 MB), one token 3.4, a launch.  Norm weights as loads of single values
+// 31.1 (160 MB), one token 3.2, a launch.  With 100 values rotated, loaded and
+// stored one by one, 67 where 128 take 35, in a graph.  Norm weights as loads of single values
 // and pointers indexed by a lane's kind of head took 47; several tokens a work
 // group, with loops over their heads, 33 to 35.
 #include "runtime.hpp"

@@ -383,8 +383,8 @@ __device__ __forceinline__ pg_f4 pg_join(const char *smem, float (*sm)[PG_COLS],
     }
     return a;
 }
-// The result of sums a and L: zero where nothing was seen.  An infinity here comes from a cached one, which the
-// weights' second parts turn into NaN for some heads and not for others: NaN for all.
+// The result of sums a and L: zero where nothing was seen.  An infinity here comes from a cached one (sums of finite values
+// stay finite), which the weights' second parts turn into NaN for some heads and not for others: NaN for all.
 __device__ __forceinline__ pg_f4 pg_result(pg_f4 a, float L) {
     a *= L == 0.0f ? 0.0f : 1.0f / L;
     return a + a * 0.0f;

@@ -364,8 +364,8 @@ def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None,
     token t goes to position pos[t] of lane lanes[t] (int32 [n]; None: lane t).  A token of a negative position is
     padding; one whose position has no page in the table (an entry outside the pool, a position past it) is not stored.
     Two tokens must not have one position of one lane, nor k_pages and v_pages share elements.  q f32 [n, n_heads,
-    head_dim]: the tokens' queries, normed and rotated in the same launch; returns q_out (``q_out=q``: in place), None
-    without q.
+    head_dim]: the tokens' queries, normed and rotated in the same launch; returns q_out (``q_out=q``: in place; one made
+    here is contiguous, as `paged_attn_dev` takes it), None without q.
     """
     if k.dim() != 3:
         raise ValueError("k [n, n_kv_heads, head_dim]")
@@ -406,7 +406,7 @@ def paged_append_dev(k, v, k_pages, v_pages, table, pos, lanes=None, freqs=None,
 def paged_attn_dev(q, k_pages, v_pages, table, lens, scale: float, window: int = 0, out=None):
     """Attention of one new token of each of n lanes over its pages.
 
-    q f32 [n, n_heads, head_dim] (rotated); pages and table as `paged_append_dev` fills them, n lanes or more; lane i
+    q f32 [n, n_heads, head_dim] (rotated, contiguous); pages and table as `paged_append_dev` fills them, n lanes or more; lane i
     sees its first lens[i] (int32) positions, its new token's own among them, of those the last ``window`` where that is
     not 0, and none of a page that the table does not have.  Zero where it sees nothing.  Returns out f32 as q.
     """
